@@ -178,6 +178,58 @@ TH_API int th_argmax(th_device *dev, const th_buffer *logits, uint32_t *token);
 TH_API int th_sample(th_device *dev, const th_buffer *logits, float temperature, size_t top_k, float top_p,
                      uint64_t *rng, uint32_t *token);
 
+/* ---- 8-bit rows (no counterpart in model/device.rs) ---- */
+
+/* A matrix of 8-bit rows, weights or activations: integers q and an f32 scale
+ * s for each row, standing for the values q s. Of a row v with A = max |v| the
+ * integers are those nearest to 127 v / A, ties to even (decided in 64 bits, so
+ * that they depend on v alone), and s is A / 127 in f32; where that is
+ * zero, so are the integers. A row that holds a NaN or an infinity, or whose A / 127 is past f32,
+ * has s = NaN and zeros, and so what is computed from it is NaN. The rows are
+ * kept in the order in which the matrix cores take them; th_q8_read and
+ * th_q8_write give and take them row-major.
+ *
+ * A projection over 8-bit rows reads half of what th_matmul reads of its
+ * weights. A layer in this form (model/model.rs:103-143): th_add_rmsnorm_q8,
+ * th_matmul_q8 x 3, the q/k norms, rotations and attention as before,
+ * th_quantize_q8, th_matmul_q8, th_add_rmsnorm_q8, th_matmul_q8 x 2,
+ * th_silu_mul_q8, th_matmul_q8.
+ *
+ * The compute calls can be captured (th_graph_begin) at any size; alloc, free,
+ * read and write are refused then. */
+typedef struct th_q8 th_q8;
+/* `rows` rows of `cols` (1 to 131071, the most whose sums of products fit 32
+ * bits) zeros, of scale 0. Takes ceil(rows / 16) * ceil(cols / 128) * 2 KB. */
+TH_API int th_q8_alloc(th_device *dev, size_t rows, size_t cols, th_q8 **out);
+TH_API void th_q8_free(th_device *dev, th_q8 *q);
+TH_API int th_q8_shape(const th_q8 *q, size_t *rows, size_t *cols);
+/* rows <= the allocated rows; contents gained are undefined. */
+TH_API int th_q8_resize(th_device *dev, th_q8 *q, size_t rows);
+/* Copies out (blocking) the integers, row-major, and the scales. */
+TH_API int th_q8_read(th_device *dev, const th_q8 *q, int8_t *values, float *scales);
+/* The reverse (blocking), for weights that were quantized elsewhere: any
+ * integers and scales. */
+TH_API int th_q8_write(th_device *dev, th_q8 *q, const int8_t *values, const float *scales);
+/* q = the rows of x (f32; x.len == rows * cols). */
+TH_API int th_quantize_q8(th_device *dev, th_q8 *q, const th_buffer *x);
+/* q = the rows of a [rows, cols] weight (each output channel with its scale). */
+TH_API int th_quantize_weight_q8(th_device *dev, th_q8 *q, const th_weight *w);
+/* out = the values q s, row-major (out.len == rows * cols). */
+TH_API int th_dequantize_q8(th_device *dev, th_buffer *out, const th_q8 *q);
+/* x += y in f32 (unless y is NULL), then q = the rows of rmsnorm(x) with
+ * `weight` (cols gains): th_add_rmsnorm with its output in 8 bits, rounded
+ * once. x.len == rows * cols; y holds at least as many and is not x. */
+TH_API int th_add_rmsnorm_q8(th_device *dev, th_buffer *x, const th_buffer *y, th_q8 *q, const th_weight *weight,
+                             float eps);
+/* q = the rows of silu(gate) * up: th_silu_mul with its output in 8 bits,
+ * rounded once; gate and up (rows * cols each, which may be one buffer) stay
+ * as they are. */
+TH_API int th_silu_mul_q8(th_device *dev, th_q8 *q, const th_buffer *gate, const th_buffer *up);
+/* out[t][r] = x.s[t] w.s[r] sum_k x.q[t][k] w.q[r][k]: th_matmul over 8-bit
+ * rows, the sum exact, converted to f32 and multiplied by x.s[t], then w.s[r].
+ * w.cols == x.cols, out.len == x.rows * w.rows. */
+TH_API int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x);
+
 /* ---- the forward pass (model/model.rs) ---- */
 
 /* Architecture (model/config.rs:9-36, head_dim resolved as config.rs:32-35 does). */

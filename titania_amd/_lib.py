@@ -84,6 +84,18 @@ SIGNATURES: dict[str, tuple] = {
     "th_gate_up_silu": (_I, [_P, _P, _P, _P, _P, _P]),
     "th_argmax": (_I, [_P, _P, C.POINTER(C.c_uint32)]),
     "th_sample": (_I, [_P, _P, C.c_float, _SZ, C.c_float, C.POINTER(C.c_uint64), C.POINTER(C.c_uint32)]),
+    "th_q8_alloc": (_I, [_P, _SZ, _SZ, C.POINTER(_P)]),
+    "th_q8_free": (None, [_P, _P]),
+    "th_q8_shape": (_I, [_P, C.POINTER(_SZ), C.POINTER(_SZ)]),
+    "th_q8_resize": (_I, [_P, _P, _SZ]),
+    "th_q8_read": (_I, [_P, _P, _P, _P]),
+    "th_q8_write": (_I, [_P, _P, _P, _P]),
+    "th_quantize_q8": (_I, [_P, _P, _P]),
+    "th_quantize_weight_q8": (_I, [_P, _P, _P]),
+    "th_dequantize_q8": (_I, [_P, _P, _P]),
+    "th_add_rmsnorm_q8": (_I, [_P, _P, _P, _P, _P, C.c_float]),
+    "th_silu_mul_q8": (_I, [_P, _P, _P, _P]),
+    "th_matmul_q8": (_I, [_P, _P, _P, _P]),
     "th_model_create": (_I, [_P, C.POINTER(ThConfig), C.POINTER(_P), _SZ, C.POINTER(_P)]),
     "th_model_destroy": (None, [_P]),
     "th_config_load": (_I, [C.c_char_p, C.POINTER(ThConfig)]),

@@ -1,0 +1,46 @@
+// 8-bit rows (th_q8): their layout, and the launchers of their kernels.
+#pragma once
+
+#include "common.h"
+
+// Rows of 8-bit integers with an f32 scale each. A wave's matrix-core operand
+// of 16 rows x 64 columns (a fragment) is 1 KB of consecutive memory, lane
+// l = row % 16 + 16 * (column % 64 / 16) having 16 consecutive columns, so
+// that operands are loaded, staged in LDS and read back 16 consecutive bytes a
+// lane, with neither a transposition nor a bank conflict. The fragments of 16
+// rows lie side by side. Columns past `cols` of a row are zero, always.
+struct th_q8 {
+    int8_t *ptr = nullptr;
+    float *scale = nullptr;  // behind the integers, in the same allocation
+    size_t rows = 0;         // current rows
+    size_t cap = 0;          // rows it was allocated with
+    size_t cols = 0;
+    int ordinal = 0;         // the GPU that holds it
+};
+
+namespace th {
+
+// Sums of cols products of two 8-bit integers stay below 2^31.
+constexpr size_t kQ8MaxCols = 131071;
+
+// Fragments of a row block: an even number, for kernels that step by 128 columns.
+constexpr size_t q8_frags(size_t cols) { return (cols + 127) / 128 * 2; }
+constexpr size_t q8_blocks(size_t rows) { return (rows + 15) / 16; }
+// Byte of (row, col) in a matrix of `frags` fragments a row block.
+__host__ __device__ constexpr size_t q8_at(size_t row, size_t col, size_t frags) {
+    return ((row >> 4) * frags + (col >> 6)) * 1024 + ((row & 15) + (col >> 4 & 3) * 16) * 16 + (col & 15);
+}
+
+// q = 8-bit rows of x [rows][cols] (f32, or bf16 weights).
+hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x);
+hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16_t *w);
+// out [rows][cols] = the values that q stands for.
+hipError_t launch_dequantize_q8(hipStream_t s, float *out, const th_q8 &q);
+// x += y (unless y is null), q = 8-bit rows of rmsnorm(x).
+hipError_t launch_add_rmsnorm_q8(hipStream_t s, float *x, const float *y, const th_q8 &q, const uint16_t *w, float eps);
+// q = 8-bit rows of silu(gate) * up.
+hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, const float *up);
+// out[t * w.rows + r] = x.scale[t] w.scale[r] sum_k x[t][k] w[r][k].
+hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x);
+
+}  // namespace th

@@ -102,6 +102,34 @@ class Buffer:
             pass
 
 
+class Q8:
+    """A matrix of 8-bit rows in device memory (th_q8), weights or activations:
+    integers and an f32 scale for each row, whose product is the value."""
+
+    def __init__(self, dev: "Hip", handle: int):
+        self._dev = dev
+        self.handle = handle
+
+    @property
+    def shape(self) -> tuple:
+        rows, cols = C.c_size_t(), C.c_size_t()
+        check(lib().th_q8_shape(self.handle, C.byref(rows), C.byref(cols)))
+        return int(rows.value), int(cols.value)
+
+    def free(self) -> None:
+        if self.handle:
+            self._dev._refuse_while_capturing("free 8-bit rows")
+            lib().th_q8_free(self._dev.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self._dev.handle:
+                self.free()
+        except Exception:
+            pass
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32).reshape(-1)
 
@@ -235,6 +263,59 @@ class Hip:
         """gate = silu(w_gate . xb) * (w_up . xb) (model.rs:137-139); up is scratch."""
         check(lib().th_gate_up_silu(self.handle, gate.handle, up.handle, w_gate.handle, w_up.handle, xb.handle))
 
+    # ---- 8-bit rows ----
+
+    def alloc_q8(self, rows: int, cols: int) -> Q8:
+        out = C.c_void_p()
+        check(lib().th_q8_alloc(self.handle, int(rows), int(cols), C.byref(out)))
+        return Q8(self, out.value)
+
+    def resize_q8(self, q: Q8, rows: int) -> None:
+        check(lib().th_q8_resize(self.handle, q.handle, int(rows)))
+
+    def read_q8(self, q: Q8) -> tuple[np.ndarray, np.ndarray]:
+        """The integers [rows, cols] and the scales [rows]."""
+        rows, cols = q.shape
+        values, scales = np.empty((rows, cols), dtype=np.int8), np.empty(rows, dtype=np.float32)
+        check(lib().th_q8_read(self.handle, q.handle, values.ctypes.data, scales.ctypes.data))
+        return values, scales
+
+    def write_q8(self, q: Q8, values, scales) -> None:
+        v, s = np.asarray(values), _f32(scales)
+        if v.dtype != np.int8:
+            raise TypeError(f"8-bit rows are int8, not {v.dtype}")
+        if v.size != q.shape[0] * q.shape[1] or s.size != q.shape[0]:
+            raise ValueError(f"{v.size} integers and {s.size} scales for 8-bit rows of shape {q.shape}")
+        v = np.ascontiguousarray(v)
+        check(lib().th_q8_write(self.handle, q.handle, v.ctypes.data, s.ctypes.data))
+
+    def quantize_q8(self, q: Q8, x: Buffer) -> None:
+        """q = the rows of x."""
+        check(lib().th_quantize_q8(self.handle, q.handle, x.handle))
+
+    def quantize_weight_q8(self, q: Q8, w: Weight) -> None:
+        """q = the rows of w, each output channel with its scale."""
+        check(lib().th_quantize_weight_q8(self.handle, q.handle, w.handle))
+
+    def dequantize_q8(self, out: Buffer, q: Q8) -> None:
+        """out = the values that q stands for."""
+        check(lib().th_dequantize_q8(self.handle, out.handle, q.handle))
+
+    def add_rmsnorm_q8(self, x: Buffer, y: Buffer | None, q: Q8, weight: Weight, eps: float) -> None:
+        """x += y (unless y is None), then q = the rows of rmsnorm(x)."""
+        check(lib().th_add_rmsnorm_q8(self.handle, x.handle, y.handle if y is not None else None, q.handle,
+                                      weight.handle, float(eps)))
+
+    def silu_mul_q8(self, q: Q8, gate: Buffer, up: Buffer) -> None:
+        """q = the rows of silu(gate) * up."""
+        check(lib().th_silu_mul_q8(self.handle, q.handle, gate.handle, up.handle))
+
+    def matmul_q8(self, out: Buffer, w: Q8, x: Q8) -> None:
+        """matmul() over 8-bit rows: sums of integer products, times both scales."""
+        check(lib().th_matmul_q8(self.handle, out.handle, w.handle, x.handle))
+
+    # ---- the next token ----
+
     def argmax(self, logits: Buffer) -> int:
         tok = C.c_uint32()
         check(lib().th_argmax(self.handle, logits.handle, C.byref(tok)))
@@ -251,4 +332,4 @@ class Hip:
         return int(tok.value)
 
 
-__all__ = ["Hip", "Tensor", "Weight", "Buffer", "_lib"]
+__all__ = ["Hip", "Tensor", "Weight", "Buffer", "Q8", "_lib"]

@@ -30,6 +30,11 @@ pub struct th_graph {
     _p: [u8; 0],
 }
 
+#[repr(C)]
+pub struct th_q8 {
+    _p: [u8; 0],
+}
+
 /// model/config.rs:9-36 with head_dim resolved.
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
@@ -113,6 +118,21 @@ unsafe extern "C" {
     pub fn th_argmax(dev: *mut th_device, logits: *const th_buffer, token: *mut u32) -> c_int;
     pub fn th_sample(dev: *mut th_device, logits: *const th_buffer, temperature: f32, top_k: usize, top_p: f32,
                      rng: *mut u64, token: *mut u32) -> c_int;
+
+    // 8-bit rows.
+    pub fn th_q8_alloc(dev: *mut th_device, rows: usize, cols: usize, out: *mut *mut th_q8) -> c_int;
+    pub fn th_q8_free(dev: *mut th_device, q: *mut th_q8);
+    pub fn th_q8_shape(q: *const th_q8, rows: *mut usize, cols: *mut usize) -> c_int;
+    pub fn th_q8_resize(dev: *mut th_device, q: *mut th_q8, rows: usize) -> c_int;
+    pub fn th_q8_read(dev: *mut th_device, q: *const th_q8, values: *mut i8, scales: *mut f32) -> c_int;
+    pub fn th_q8_write(dev: *mut th_device, q: *mut th_q8, values: *const i8, scales: *const f32) -> c_int;
+    pub fn th_quantize_q8(dev: *mut th_device, q: *mut th_q8, x: *const th_buffer) -> c_int;
+    pub fn th_quantize_weight_q8(dev: *mut th_device, q: *mut th_q8, w: *const th_weight) -> c_int;
+    pub fn th_dequantize_q8(dev: *mut th_device, out: *mut th_buffer, q: *const th_q8) -> c_int;
+    pub fn th_add_rmsnorm_q8(dev: *mut th_device, x: *mut th_buffer, y: *const th_buffer, q: *mut th_q8,
+                             weight: *const th_weight, eps: f32) -> c_int;
+    pub fn th_silu_mul_q8(dev: *mut th_device, q: *mut th_q8, gate: *const th_buffer, up: *const th_buffer) -> c_int;
+    pub fn th_matmul_q8(dev: *mut th_device, out: *mut th_buffer, w: *const th_q8, x: *const th_q8) -> c_int;
 
     // The forward pass (model/model.rs) and the decode loops on the device.
     pub fn th_model_create(dev: *mut th_device, config: *const th_config, weights: *const *const th_weight,
