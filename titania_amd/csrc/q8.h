@@ -40,7 +40,8 @@ hipError_t launch_dequantize_q8(hipStream_t s, float *out, const th_q8 &q);
 hipError_t launch_add_rmsnorm_q8(hipStream_t s, float *x, const float *y, const th_q8 &q, const uint16_t *w, float eps);
 // q = 8-bit rows of silu(gate) * up.
 hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, const float *up);
-// out[t * w.rows + r] = x.scale[t] w.scale[r] sum_k x[t][k] w[r][k].
-hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x);
+// out[t * w.rows + r] = x.scale[t] w.scale[r] sum_k x[t][k] w[r][k]. Where it
+// splits K, the sums of the parts go to part (part_len long).
+hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len);
 
 }  // namespace th

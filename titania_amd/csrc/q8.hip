@@ -1,8 +1,10 @@
 // The C ABI's 8-bit rows (th_q8): handles, host copies and argument checks.
+#include <algorithm>
 #include <cstring>
 #include <new>
 
 #include "common.h"
+#include "gemm.h"
 #include "q8.h"
 
 using th::fail;
@@ -178,7 +180,8 @@ int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x)
     TH_Q8_HERE(dev, w);
     TH_Q8_HERE(dev, x);
     TH_HIP(hipSetDevice(dev->ordinal));
-    TH_HIP(th::launch_matmul_q8(dev->stream, out->ptr, *w, *x));
+    TH_HIP(th::launch_matmul_q8(dev->stream, out->ptr, *w, *x, reinterpret_cast<int *>(dev->part),
+                                std::max(th::kPartFloats, th::kAttnRoundFloats)));
     return TH_OK;
 }
 

@@ -2,7 +2,18 @@
 // out[t][r] = x.scale[t] w.scale[r] sum_k x[t][k] w[r][k].
 //
 // The sums are exact (32-bit integers), so that neither the order nor a split
-// of K changes a result; then one conversion to f32 and two products.
+// of K changes a result; then one conversion to f32 and two products. The
+// weights' fragment is the first operand of every product, so that lane l ends
+// with weight rows 4 (l / 16) .. + 3 of token l % 16.
+//
+// Operands are whole fragments (q8.h), 1 KB of consecutive memory each: a wave
+// loads one with 16 bytes a lane, into registers or straight into LDS, and
+// reads it back from LDS the same way, without bank conflicts and without a
+// swizzle. Loads go through a buffer descriptor that ends with the matrix:
+// row blocks past its end read as zeros.
+#include <algorithm>
+#include <cmath>
+
 #include "device_util.h"
 #include "q8.h"
 
@@ -10,39 +21,407 @@ namespace th {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct Args {
     const int8_t *w, *x;
     const float *w_scale, *x_scale;
     float *out;
     int n, rows, frags;
+    // A split of K (ksplit > 1): part z's sums go to part[z][n][rows].
+    int *part;
+    int ksplit;
 };
 
-// A wave a 16 rows x 16 tokens: the weights' fragment is the first operand, so
-// lane l ends with rows 4 (l / 16) .. + 3 of token l % 16.
-__global__ __launch_bounds__(256) void matmul_kernel(Args a) {
-    const int lane = threadIdx.x & 63;
-    const int quads = (a.rows + 63) / 64;
-    const int rb = (int)(blockIdx.x % quads) * 4 + (threadIdx.x >> 6), tb = blockIdx.x / quads;
-    if (rb * 16 >= a.rows) return;
-    const i32x4 *w = reinterpret_cast<const i32x4 *>(a.w) + (size_t)rb * a.frags * 64 + lane;
-    const i32x4 *x = reinterpret_cast<const i32x4 *>(a.x) + (size_t)tb * a.frags * 64 + lane;
-    i32x4 sum = {0, 0, 0, 0};
-    for (int f = 0; f < a.frags; ++f)
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[(size_t)f * 64], x[(size_t)f * 64], sum, 0, 0, 0);
-    const int t = tb * 16 + (lane & 15), r = rb * 16 + (lane >> 4) * 4;
-    if (t >= a.n) return;
-    const float xs = a.x_scale[t];
-    for (int i = 0; i < 4; ++i)
-        if (r + i < a.rows) a.out[(size_t)t * a.rows + r + i] = (float)sum[i] * xs * a.w_scale[r + i];
+constexpr unsigned kMostBytes = 0x40000000u;  // a descriptor's range: more than any block's row blocks take
+constexpr unsigned kPastEnd = 0xf0000000u;    // an offset past every range: the load gives zero
+
+// The matrix from row block b0 on. (A block of threads reads at most 64 row
+// blocks of at most 2 MB.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t blocks_from(const int8_t *p, int rows, int b0, int frags) {
+    const size_t block = (size_t)frags * 1024, left = (size_t)((rows + 15) / 16 - b0) * block;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(p) + b0 * block, 0,
+                                             (int)(left < kMostBytes ? left : kMostBytes), kBufferRsrcWord3);
+}
+
+__device__ __forceinline__ i32x4 load_frag(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+
+__device__ __forceinline__ i32x4 mfma(i32x4 w, i32x4 x, i32x4 sum) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, sum, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x4 scaled(i32x4 sum, float xs, float4 ws) {
+    return f32x4{(float)sum[0] * xs * ws.x, (float)sum[1] * xs * ws.y, (float)sum[2] * xs * ws.z,
+                 (float)sum[3] * xs * ws.w};
+}
+
+// Few tokens. A block takes RB row blocks and TB token blocks, its W waves the
+// fragments in turn (so that the block reads consecutive memory), U of them in
+// flight a wave; the waves' sums meet in LDS.
+//
+// Bound by the weights' bytes, each read once. The matrix cores take 16 tokens
+// at a quarter of the rate at which HBM delivers, so that one token is no
+// other case than 16.
+template <int RB, int TB, int W, int U>
+__global__ __launch_bounds__(64 * W) void few_kernel(Args a) {
+    __shared__ i32x4 red[W * RB * TB * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Blocks of the same weights and other tokens run on one XCD (blocks are
+    // dealt to the 8 XCDs in turn), so that its L2 has the weights once.
+    const int tbs = ((a.n + 15) / 16 + TB - 1) / TB, lin = blockIdx.x;
+    const int rb0 = (lin / (8 * tbs) * 8 + lin % 8) * RB, tb0 = lin % (8 * tbs) / 8 * TB;
+    if (rb0 * 16 >= a.rows) return;
+    const unsigned block = (unsigned)a.frags * 1024;
+    const __amdgpu_buffer_rsrc_t rw = blocks_from(a.w, a.rows, rb0, a.frags), rx = blocks_from(a.x, a.n, tb0, a.frags);
+    unsigned xo[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) xo[t] = (tb0 + t) * 16 + (lane & 15) < a.n ? t * block + lane * 16 : kPastEnd;
+    i32x4 acc[RB][TB] = {};
+    for (int f0 = wave; f0 < a.frags; f0 += W * U) {
+        i32x4 w[U][RB], x[U][TB];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int f = f0 + u * W;
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+                w[u][i] = load_frag(rw, f < a.frags ? i * block + f * 1024u + lane * 16 : kPastEnd);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int f = f0 + u * W;
+#pragma unroll
+            for (int t = 0; t < TB; ++t) x[u][t] = load_frag(rx, f < a.frags ? xo[t] + f * 1024u : kPastEnd);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int t = 0; t < TB; ++t) acc[i][t] = mfma(w[u][i], x[u][t], acc[i][t]);
+    }
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) red[((wave * RB + i) * TB + t) * 64 + lane] = acc[i][t];
+    __syncthreads();
+    for (int e = threadIdx.x; e < RB * TB * 64; e += 64 * W) {
+        const int q = e >> 6, l = e & 63, t = (tb0 + q % TB) * 16 + (l & 15), r = (rb0 + q / TB) * 16 + (l >> 4) * 4;
+        if (t >= a.n || r >= a.rows) continue;
+        i32x4 sum = red[e];
+#pragma unroll
+        for (int k = 1; k < W; ++k) sum += red[k * RB * TB * 64 + e];
+        const f32x4 v = scaled(sum, a.x_scale[t], *reinterpret_cast<const float4 *>(a.w_scale + r));
+        float *o = a.out + (size_t)t * a.rows + r;
+        if (a.rows % 4 == 0) {
+            *reinterpret_cast<f32x4 *>(o) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r + i < a.rows) o[i] = v[i];
+        }
+    }
+}
+
+// The tile of a block: blocks are dealt to the 8 XCDs in turn, and each XCD
+// takes a contiguous range of tiles, in panels of 8 tiles of tokens, so that
+// the tiles that it has in work share operands in its L2.
+__device__ __forceinline__ void tile_of_block(int lin, int gr, int gt, int &tr, int &tt) {
+    const int tiles = gr * gt, xcd = lin & 7, q = tiles >> 3, rest = tiles & 7;
+    const int i = xcd * q + (xcd < rest ? xcd : rest) + (lin >> 3);
+    const int high = gt < 8 ? gt : 8, panel = i / (high * gr), in = i % (high * gr);
+    const int height = gt - panel * high < high ? gt - panel * high : high;
+    tr = in / height;
+    tt = panel * high + in % height;
+}
+
+// A barrier that does not wait for loads in flight: every wave has waited for
+// its own that the others are about to read, and for its reads of what is
+// about to be overwritten.
+__device__ __forceinline__ void stage_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Waits until at most VM loads and no LDS reads are outstanding.
+template <int VM>
+__device__ __forceinline__ void wait_loads_and_lds() {
+    static_assert(VM >= 0 && VM < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt((VM & 15) | (0x7 << 4) | (VM >> 4) << 14);
+}
+
+// Many tokens. A block of WM x WN waves takes a tile of BM x BN row blocks
+// (weights x tokens), each wave FM x FN of them, K in steps of 128 columns
+// (two fragments) through a ring of NS stages in LDS, filled by direct loads
+// (1 KB each) that run NS - 1 steps ahead.
+//
+// A wave goes through a step row by row: FN products with one weight
+// fragment, the fragment of two rows on being read meanwhile, and one load
+// issued, so that neither LDS nor the memory path sees bursts. The barrier of a
+// step comes two rows before its end: by then everything of the stage is in
+// registers, its slot is free for new loads, and the first fragments of the
+// next stage are read under the last rows' products.
+template <int FM_, int FN_, int WM_, int WN_, int NS_>
+struct Tile {
+    static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, NS = NS_, BM = FM * WM, BN = FN * WN;
+    static constexpr int kWaves = WM * WN, kFrags = 2 * (BM + BN);                         // of a stage
+    static constexpr int kLoads = kFrags / kWaves, kMostLoads = (kFrags + kWaves - 1) / kWaves;  // a wave's
+    static constexpr int kRows = 2 * FM, kAhead = 2;
+    static constexpr int kLine = FM * 16 + 4;  // floats of a token in the epilogue, off the banks' period
+    static_assert(kMostLoads <= kRows && kWaves * 16 * kLine * 4 <= NS * kFrags * 1024 && NS * kFrags <= 160, "");
+    static_assert(kMostLoads >= kAhead, "the prologue issues kAhead loads of the last stage");
+};
+
+template <class T>
+__global__ __launch_bounds__(64 * T::kWaves) void tile_kernel(Args a, int gr, int gt) {
+    constexpr int FM = T::FM, FN = T::FN, NS = T::NS, BM = T::BM, R = T::kRows, D = T::kAhead, L = T::kLoads;
+    __shared__ i32x4 ring[NS][T::kFrags][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int tr, tt;
+    const int z = a.ksplit > 1 ? blockIdx.x / (gr * gt) : 0;
+    tile_of_block(blockIdx.x - z * (gr * gt), gr, gt, tr, tt);
+    const int all = a.frags / 2, s0 = (int)((long long)all * z / a.ksplit);
+    const int rb0 = tr * BM, tb0 = tt * T::BN, steps = (int)((long long)all * (z + 1) / a.ksplit) - s0;
+    const unsigned block = (unsigned)a.frags * 1024;
+    const __amdgpu_buffer_rsrc_t rw = blocks_from(a.w, a.rows, rb0, a.frags), rx = blocks_from(a.x, a.n, tb0, a.frags);
+    // Load j of this wave's for a step: fragment wave + kWaves j of the stage.
+    auto load = [&](int step, int slot, int j) {
+        const int f = wave + T::kWaves * j, b = f / 2;
+        if (j >= L && f >= T::kFrags) return;
+        const unsigned col = (unsigned)(2 * (s0 + step) + f % 2) * 1024 + lane * 16;
+        auto *to = (__attribute__((address_space(3))) void *)&ring[slot][f][0];
+        const bool weights = 2 * BM % T::kWaves == 0 ? j < 2 * BM / T::kWaves : b < BM;
+        if (weights) __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, to, 16, (int)(b * block + col), 0, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, to, 16, (int)((b - BM) * block + col), 0, 0, 0);
+    };
+    const int wm = wave % T::WM * FM, wn = wave / T::WM * FN;  // this wave's first row block and token block
+    auto read_w = [&](int slot, int r) { return ring[slot][(wm + r % FM) * 2 + r / FM][lane]; };
+    auto read_x = [&](int slot, int k, int j) { return ring[slot][(BM + wn + j) * 2 + k][lane]; };
+
+    i32x4 acc[FM][FN] = {};
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+        if (s < steps) {
+#pragma unroll
+            for (int j = 0; j < T::kMostLoads; ++j) load(s, s, j);
+        }
+    if (NS - 1 < steps) {
+#pragma unroll
+        for (int j = 0; j < D; ++j) load(NS - 1, NS - 1, j);
+        wait_loads_and_lds<(NS - 2) * L + (D < L ? D : L)>();
+    } else {
+        wait_loads_and_lds<0>();
+    }
+    stage_barrier();
+    i32x4 x[2][FN], w[R], next[D];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) x[0][j] = read_x(0, 0, j);
+#pragma unroll
+    for (int r = 0; r < D; ++r) w[r] = read_w(0, r);
+    int cur = 0;
+    for (int step = 0; step < steps; ++step) {
+        const int nxt = cur + 1 == NS ? 0 : cur + 1, prv = cur == 0 ? NS - 1 : cur - 1;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int k = r / FM, i = r % FM;
+            if (r == R - D) {
+                if (step + NS - 1 < steps) wait_loads_and_lds<(NS - 2) * L>();
+                else wait_loads_and_lds<0>();
+                stage_barrier();
+#pragma unroll
+                for (int j = 0; j < FN; ++j) x[0][j] = read_x(nxt, 0, j);
+            }
+            if (r == 0) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) x[1][j] = read_x(cur, 1, j);
+            }
+            if (r + D < R) w[r + D] = read_w(cur, r + D);
+            else next[r + D - R] = read_w(nxt, r + D - R);
+            // The loads of step + NS go where this step was, from its barrier on.
+            if (r >= R - D) {
+                if (step + NS < steps) load(step + NS, cur, r - (R - D));
+            } else if (r + D < T::kMostLoads) {
+                if (step - 1 + NS < steps) load(step - 1 + NS, prv, r + D);
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma(w[r], x[k][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int r = 0; r < D; ++r) w[r] = next[r];
+        cur = nxt;
+    }
+
+    // 16 tokens at a time through LDS, so that a token's FM * 16 values are
+    // stored side by side: whole lines, where a lane's own four would be a
+    // part of one (a 256 x 256 tile's stores took 10 us, now 5).
+    const int lt = lane & 15, lr = lane >> 4 << 2, r0 = (rb0 + wm) * 16, t0 = (tb0 + wn) * 16;
+    const int last = (a.rows + 15) / 16 * 16 - 4;
+    float4 ws[FM];
+    float xs[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) ws[i] = *reinterpret_cast<const float4 *>(a.w_scale + min(r0 + i * 16 + lr, last));
+#pragma unroll
+    for (int j = 0; j < FN; ++j) xs[j] = a.x_scale[min(t0 + j * 16 + lt, a.n - 1)];
+    __syncthreads();
+    float *lines = reinterpret_cast<float *>(ring) + wave * 16 * T::kLine;
+    float *out = a.ksplit > 1 ? reinterpret_cast<float *>(a.part + (size_t)z * a.n * a.rows) : a.out;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            *reinterpret_cast<f32x4 *>(lines + lt * T::kLine + i * 16 + lr) =
+                a.ksplit > 1 ? __builtin_bit_cast(f32x4, acc[i][j]) : scaled(acc[i][j], xs[j], ws[i]);
+        if (a.rows % 4 == 0) {
+#pragma unroll
+            for (int q = 0; q < FM; ++q) {
+                const int e = q * 64 + lane, t = e / (FM * 4), c = e % (FM * 4) * 4;
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(lines + t * T::kLine + c);
+                if (t0 + j * 16 + t < a.n && r0 + c < a.rows)
+                    __builtin_nontemporal_store(
+                        v, reinterpret_cast<f32x4 *>(out + (size_t)(t0 + j * 16 + t) * a.rows + r0 + c));
+            }
+        } else {
+            for (int e = lane; e < 16 * 16 * FM; e += 64) {
+                const int t = e / (FM * 16), c = e % (FM * 16);
+                if (t0 + j * 16 + t < a.n && r0 + c < a.rows)
+                    out[(size_t)(t0 + j * 16 + t) * a.rows + r0 + c] = lines[t * T::kLine + c];
+            }
+        }
+    }
+}
+
+// The sums of a split of K, four rows of a token a thread (rows % 4 == 0) or one.
+template <int V>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V, m = (size_t)a.n * a.rows;
+    if (i >= m) return;
+    const int t = (int)(i / a.rows), r = (int)(i % a.rows);
+    if constexpr (V == 4) {
+        i32x4 sum = {};
+        for (int z = 0; z < a.ksplit; ++z) sum += *reinterpret_cast<const i32x4 *>(a.part + z * m + i);
+        *reinterpret_cast<f32x4 *>(a.out + i) =
+            scaled(sum, a.x_scale[t], *reinterpret_cast<const float4 *>(a.w_scale + r));
+    } else {
+        int sum = 0;
+        for (int z = 0; z < a.ksplit; ++z) sum += a.part[z * m + i];
+        a.out[i] = (float)sum * a.x_scale[t] * a.w_scale[r];
+    }
+}
+
+size_t blocks_of(int rows, int each) { return ((size_t)(rows + 15) / 16 + each - 1) / each; }
+
+template <int RB, int TB, int W>
+void few(hipStream_t s, const Args &a) {
+    const size_t rbs = blocks_of(a.rows, RB), tbs = blocks_of(a.n, TB);
+    few_kernel<RB, TB, W, 5><<<(unsigned)((rbs + 7) / 8 * 8 * tbs), 64 * W, 0, s>>>(a);
+}
+
+template <class T>
+void tiles(hipStream_t s, const Args &a) {
+    const int gr = (int)blocks_of(a.rows, T::BM), gt = (int)blocks_of(a.n, T::BN);
+    tile_kernel<T><<<(unsigned)gr * (unsigned)gt * (unsigned)a.ksplit, 64 * T::kWaves, 0, s>>>(a, gr, gt);
+    if (a.ksplit == 1) return;
+    const size_t m = (size_t)a.n * a.rows;
+    if (a.rows % 4 == 0) join_kernel<4><<<(unsigned)((m / 4 + 255) / 256), 256, 0, s>>>(a);
+    else join_kernel<1><<<(unsigned)((m + 255) / 256), 256, 0, s>>>(a);
+}
+
+// About how long a launch takes, in us, from its shape alone. The constants
+// are fitted to back-to-back launches of every variant over 9 matrices (1024 x
+// 1024 to 4096 x 16384) and 14 counts of tokens (20 to 8192): the variant that
+// they choose is 1.01 times the fastest one's time in the geometric mean, 1.16
+// at most.
+constexpr double kLaunch = 2.4;
+constexpr int kCus = 256;
+
+// The work of the CUs and the matrices' way from and to HBM, which mostly overlap.
+double overlapped(const Args &a, double work) {
+    const double hbm = (1024.0 * blocks_of(a.rows, 1) * a.frags + 4.0 * a.n * a.rows) / 5.6e6;
+    return kLaunch + std::max(work, hbm) + 0.16 * std::min(work, hbm);
+}
+
+// Few tokens: what a CU takes in through its memory path, block after block.
+double few_us(const Args &a, int rb, int tb) {
+    const double rounds = std::ceil((double)(blocks_of(a.rows, rb) * blocks_of(a.n, tb)) / kCus);
+    return overlapped(a, rounds * (a.frags * (rb + tb) / 113.0 + 0.4 + 0.05 * rb * tb));
+}
+
+struct TileVariant {
+    int bm, bn, products;  // row blocks, token blocks, products of a wave for 64 columns
+    int resident;          // tiles that a CU holds at once
+    void (*launch)(hipStream_t, const Args &);
+};
+template <int FM, int FN, int WM, int WN, int NS>
+constexpr TileVariant variant() {
+    using T = Tile<FM, FN, WM, WN, NS>;
+    return {T::BM, T::BN, FM * FN, T::kFrags * NS <= 80 ? 2 : 1, tiles<T>};
+}
+// Heights in small steps: as a CU holds one block, a launch takes whole rounds
+// of 256 tiles, and the height that leaves the least of the last round idle
+// wins (8192 tokens x 2560 x 9728: 320 x 256 tiles, one round, 148 us; 256 x
+// 256, 1.25 rounds, 204 us; 224 x 256, 1.5 rounds, 188 us).
+constexpr TileVariant kTiles[] = {
+    variant<2, 1, 4, 2, 4>(), variant<2, 2, 4, 2, 4>(), variant<4, 2, 2, 4, 2>(), variant<4, 2, 2, 4, 4>(),
+    variant<5, 2, 2, 4, 4>(), variant<6, 2, 2, 4, 3>(), variant<4, 4, 2, 4, 3>(), variant<5, 4, 2, 4, 3>(),
+    variant<6, 4, 2, 4, 2>(), variant<7, 4, 2, 4, 2>(), variant<8, 4, 2, 4, 2>(), variant<10, 4, 2, 4, 2>(),
+};
+
+// Tiles: rounds of a tile a CU, each with its steps of K and its epilogue (the
+// variant of which a CU holds two: a round of both takes 1.37 times one tile's
+// time; with one it waits for its short ring). A split's sums go out and come
+// in again.
+double tile_us(const Args &a, const TileVariant &v, int ksplit) {
+    const double count = (double)(blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn)) * ksplit;
+    const double steps = std::ceil(a.frags / 2.0 / ksplit), rounds = std::ceil(count / (kCus * v.resident));
+    const double one = steps * (0.173 + 0.0262 * v.products) + 0.6 + 0.13 * v.products;
+    const double us = overlapped(a, rounds * one * (v.resident == 1 ? 1.0 : count > kCus ? 1.37 : 1.13));
+    return ksplit == 1 ? us : us + 3.4 + ksplit * 8.0 * a.n * a.rows / 3.9e6;
 }
 
 }  // namespace
 
-hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x) {
+hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len) {
     if (x.rows == 0 || w.rows == 0) return hipSuccess;
-    const Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols)};
-    matmul_kernel<<<(unsigned)((w.rows + 63) / 64 * q8_blocks(x.rows)), 256, 0, s>>>(a);
+    Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols), part, 1};
+    const size_t rbs = blocks_of(a.rows, 1);
+    if (a.n <= 16) {
+        // More waves where a block has much to read and the chip is not full,
+        // fewer where there is little (one token, us with 4 / 8 / 16 waves:
+        // 1024 x 1024 2.4 / 2.6 / 3.2, 2560 x 9728 7.2 / 6.1 / 5.7).
+        if (a.frags <= 24) few<1, 1, 4>(s, a);
+        else if (a.frags >= 128 && rbs <= kCus) few<1, 1, 16>(s, a);
+        else few<1, 1, 8>(s, a);
+        return hipGetLastError();
+    }
+    const TileVariant *tile = nullptr;
+    int pick = 0, ksplit = 1;
+    double best = 1e30;
+    if (a.n <= 512) {
+        const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}};
+        for (int i = 0; i < 4; ++i)
+            if (const double us = few_us(a, shapes[i][0], shapes[i][1]); us < best) best = us, pick = i;
+    }
+    for (const TileVariant &v : kTiles) {
+        const size_t count = blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn);
+        if (const double us = tile_us(a, v, 1); us < best) best = us, tile = &v, ksplit = 1;
+        // As many parts as fill the chip, of two steps at least.
+        const int z = (int)std::min<size_t>({count ? kCus / count : 1, (size_t)a.frags / 4, 16});
+        if (z < 2 || (size_t)z * a.n * a.rows > part_len) continue;
+        if (const double us = tile_us(a, v, z); us < best) best = us, tile = &v, ksplit = z;
+    }
+    if (tile) {
+        a.ksplit = ksplit;
+        tile->launch(s, a);
+    } else if (pick == 0) {
+        a.frags <= 24 ? few<1, 1, 4>(s, a) : few<1, 1, 8>(s, a);
+    } else if (pick == 1) {
+        few<1, 2, 8>(s, a);
+    } else {
+        pick == 2 ? few<2, 2, 8>(s, a) : few<2, 4, 8>(s, a);
+    }
     return hipGetLastError();
 }
 
