@@ -28,17 +28,23 @@ __device__ __forceinline__ void load4(const float *row, int c, int cols, float (
 
 // What a row is made of. value: the 64-bit value (of the norm without its
 // factor r) at flat index i, column c. load: a thread's f32 values; kOff is how
-// far they may be off, relative to the value. kMost: load has the largest
-// 64-bit value itself.
+// far they may be off, relative to the value; a and b have what value64 makes
+// the 64-bit value of.
 struct RowsSource {
-    static constexpr bool kNorm = false, kMost = false;
+    static constexpr bool kNorm = false;
     static constexpr float kOff = 0;
     const float *x;
+    static __device__ double value64(float a, float) { return (double)a; }
     __device__ double value(size_t i, size_t) const { return (double)x[i]; }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], double &, double &, int &) const {
+    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&)[N][4], double &,
+                         int &) const {
 #pragma unroll
-        for (int k = 0; k < N; ++k) load4(x + row * cols, 4 * (threadIdx.x + T * k), cols, v[k]);
+        for (int k = 0; k < N; ++k) {
+            load4(x + row * cols, 4 * (threadIdx.x + T * k), cols, v[k]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[k][j] = v[k][j];
+        }
     }
 };
 
@@ -49,42 +55,53 @@ struct WeightSource {
 };
 
 struct NormSource {
-    static constexpr bool kNorm = true, kMost = true;
+    static constexpr bool kNorm = true;
     static constexpr float kOff = 1.0f / (1 << 24);
     float *x;
     const float *y;
     const uint16_t *g;
     float eps;
-    __device__ double value(size_t i, size_t c) const { return (double)x[i] * (double)bf16_to_f32(g[c]); }
+    static __device__ double value64(float a, float b) { return (double)a * (double)b; }
+    __device__ double value(size_t i, size_t c) const { return value64(x[i], bf16_to_f32(g[c])); }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], double &most, double &sum, int &) const;
+    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4], double &sum,
+                         int &odd) const;
 };
 
 struct SiluSource {
-    static constexpr bool kNorm = false, kMost = false;
-    // expf within 2 units in the last place (2^-23 each at most), the sum, the
-    // quotient and the product within half of one.
-    static constexpr float kOff = 3.5f / (1 << 23);
+    static constexpr bool kNorm = false;
+    // The exponential and the reciprocal within 2^-23, the exponential's
+    // correction, its product, the sum and the two products within 2^-24: 4.5
+    // 2^-23 and a little for their products.
+    static constexpr float kOff = 5.0f / (1 << 23);
     const float *gate, *up;
-    __device__ double value(size_t i, size_t) const {
-        const double g = (double)gate[i];
-        return g / (1.0 + exp(-g)) * (double)up[i];
+    static __device__ double value64(float a, float b) {
+        const double g = (double)a;
+        return g / (1.0 + exp(-g)) * (double)b;
     }
+    __device__ double value(size_t i, size_t) const { return value64(gate[i], up[i]); }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], double &, double &, int &odd) const {
-        float u[N][4];
+    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4], double &,
+                         int &odd) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            load4(gate + row * cols, 4 * (threadIdx.x + T * k), cols, v[k]);
-            load4(up + row * cols, 4 * (threadIdx.x + T * k), cols, u[k]);
+            load4(gate + row * cols, 4 * (threadIdx.x + T * k), cols, a[k]);
+            load4(up + row * cols, 4 * (threadIdx.x + T * k), cols, b[k]);
         }
+        float least = 0;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                odd |= v[k][j] < -80.f;
-                v[k][j] = silu(v[k][j]) * u[k][j];
+                // exp(-g) = 2^t (1 + d ln 2): t = -g / ln 2 rounded, d what that
+                // left and what the f32 of 1 / ln 2 lacks.
+                const float g = a[k][j], t = g * -1.44269502f;
+                const float d = fmaf(g, -1.92596303e-8f, fmaf(g, -1.44269502f, -t));
+                const float e = __builtin_amdgcn_exp2f(t);
+                v[k][j] = g * __builtin_amdgcn_rcpf(1.f + fmaf(e, d * 0.693147182f, e)) * b[k][j];
+                least = fminf(least, g);
             }
+        odd |= least < -80.f;
     }
 };
 
@@ -188,14 +205,15 @@ __device__ __forceinline__ void load4(const float *row, int c, int cols, float (
 }
 
 template <int N, int T>
-__device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], double &most, double &sum, int &odd) const {
+__device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
+                                 double &sum, int &odd) const {
     float u[N][4];
     alignas(8) uint16_t gain[N][4];
     float *xr = x + row * cols;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int c = 4 * (threadIdx.x + T * k);
-        load4(xr, c, cols, v[k]);
+        load4(xr, c, cols, a[k]);
         if (y) load4(y + row * cols, c, cols, u[k]);
         if (c + 4 <= cols) {
             *reinterpret_cast<uint2 *>(gain[k]) = *reinterpret_cast<const uint2 *>(g + c);
@@ -210,7 +228,7 @@ __device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], double 
         if (y) {
             Loose4 l;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) l.v[j] = v[k][j] += u[k][j];
+            for (int j = 0; j < 4; ++j) l.v[j] = a[k][j] += u[k][j];
             if (c + 4 <= cols) {
                 *reinterpret_cast<Loose4 *>(xr + c) = l;
             } else {
@@ -221,22 +239,55 @@ __device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], double 
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const double d = (double)v[k][j];
-            const float f = bf16_to_f32(gain[k][j]);
-            odd |= !(fabsf(v[k][j]) <= FLT_MAX);
+            const double d = (double)a[k][j];
+            b[k][j] = bf16_to_f32(gain[k][j]);
             sum = fma(d, d, sum);
-            most = fmax(most, fabs(d * (double)f));
-            v[k][j] *= f;
+            v[k][j] = a[k][j] * b[k][j];
         }
     }
+}
+
+// x[i / 4][i % 4], of registers (by masks, which no compiler turns into an
+// array in memory).
+template <int N>
+__device__ __forceinline__ float pick(const float (&x)[N][4], int i) {
+    unsigned r = 0;
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) r |= __float_as_uint(x[e / 4][e % 4]) & (unsigned)-(int)(i == e);
+    return __uint_as_float(r);
+}
+
+// A barrier for what is in LDS: it waits for no store to memory.
+__device__ __forceinline__ void lds_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// A wave's sum in 64 bits, left in lane 63: wave_sum_dpp's steps.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+    const long long b = __double_as_longlong(v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROW_MASK, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROW_MASK, 0xf, false);
+    return v + __longlong_as_double((long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v = dpp_add_f64<0xB1, 0xf>(v);
+    v = dpp_add_f64<0x4E, 0xf>(v);
+    v = dpp_add_f64<0x124, 0xf>(v);
+    v = dpp_add_f64<0x128, 0xf>(v);
+    v = dpp_add_f64<0x142, 0xa>(v);
+    return dpp_add_f64<0x143, 0xc>(v);
 }
 
 // Rows of up to 256 W N columns, one block of W waves a row, N times four
 // columns a thread, held in registers, so that the row is read once.
 //
 // Bound by memory. What 64 bits decide is found in 32 first: a value's f32 is
-// off by at most Source::kOff of it and the quotient by 127 times that and two
-// roundings more, so only values within twice that of the largest are compared
+// off by at most Source::kOff of it and the quotient by 127 times that and four
+// roundings (the largest value's, its reciprocal's twice, the product's), so only values within twice that of the largest are compared
 // in 64 bits, and only quotients within 127 kNear of a border are formed again
 // (3 in 10000 for silu). Rows on which f32 does not hold what 64 bits do
 // (values past 1e38 or not finite, none as large as 1e-30, arguments whose
@@ -245,68 +296,102 @@ template <class Source, int W, int N>
 __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__restrict__ q, float *__restrict__ scale,
                                                       size_t rows, int cols, int frags, bool grouped) {
     constexpr int T = 64 * W;
-    constexpr float kNear = Source::kOff + 3.0f / (1 << 24);
-    __shared__ Reduced<W> sh[2];
+    constexpr float kNear = Source::kOff + 5.0f / (1 << 24);
+    __shared__ alignas(16) float red_max[W];
+    __shared__ alignas(16) double red_sum[W];
+    __shared__ alignas(16) unsigned long long red_exact[W];
     const size_t row = row_of_block(blockIdx.x, grouped);
     if (row >= rows) return;
-    float v[N][4];
-    double most = 0, sum = 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float v[N][4], a[N][4], b[N][4];
+    double sum = 0;
     int odd = 0;
-    src.template load<N, T>(row, cols, v, most, sum, odd);
-    float m = 0;
+    src.template load<N, T>(row, cols, v, a, b, sum, odd);
+    auto column = [](int i) { return 4 * (int)(threadIdx.x + T * (i >> 2)) + (i & 3); };
+    auto value64 = [&](int i) { return Source::value64(pick(a, i), pick(b, i)); };
+    float m = 0, none = 0;  // 0 * v: NaN where v is not finite
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float a = fabsf(v[k][j]);
-            odd |= !(a < 1e38f);
-            m = fmaxf(m, a);
+            none = fmaf(v[k][j], 0.f, none);
+            m = fmaxf(m, fabsf(v[k][j]));
         }
-    if constexpr (!Source::kMost) most = m;
-    reduce(sh[0], most, sum, odd);
-    odd |= most < 1e-30;
-    if (odd) {
+    const float own = odd || none != 0 || m >= 1e38f ? INFINITY : m;
+    m = wave_max_dpp(own);
+    if constexpr (Source::kNorm) sum = wave_sum_f64(sum);
+    if (lane == 63) {
+        red_max[wave] = m;
+        if constexpr (Source::kNorm) red_sum[wave] = sum;
+    }
+    if (lane == 0) red_exact[wave] = 0;
+    lds_barrier();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        m = fmaxf(m, red_max[w]);
+        if constexpr (Source::kNorm) sum += red_sum[w];
+    }
+    if (!(m < INFINITY && m >= 1e-30f)) {
+        __syncthreads();  // x, which other threads wrote
         any_row<Source, W>(src, row, q, scale, cols, frags, false);
         return;
     }
-    if constexpr (!Source::kMost && Source::kOff > 0) {
-        const float reach = (float)most * (1 - 2 * Source::kOff - 1.0f / (1 << 23));
-        double exact = 0, unused = 0;
-        int none = 0;
-        if (m >= reach) {
+    double most = m;
+    if constexpr (Source::kOff > 0) {
+        // The largest in 64 bits: nearly always one thread has a candidate, one.
+        // Positive doubles are ordered as their bits are.
+        const float reach = m * (1 - 2 * Source::kOff - 1.0f / (1 << 23));
+        if (own >= reach) {
+            uint64_t near = 0;
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (fabsf(v[k][j]) >= reach) {
-                        const int c = 4 * (threadIdx.x + T * k) + j;
-                        exact = fmax(exact, fabs(src.value(row * cols + c, c)));
-                    }
+            for (int i = 0; i < 4 * N; ++i) near |= (uint64_t)(fabsf(v[i / 4][i % 4]) >= reach) << i;
+            for (; near; near &= near - 1) {
+                const double d = fabs(value64(__builtin_ctzll(near)));
+                atomicMax(&red_exact[wave], (unsigned long long)__double_as_longlong(d));
+            }
         }
-        reduce(sh[1], exact, unused, none);
-        most = exact;
+        lds_barrier();
+        unsigned long long bits = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) bits = max_u64(bits, red_exact[w]);
+        most = __longlong_as_double((long long)bits);
     }
-    int bad = 0;
-    const float s = scale_of(src, most, sum, cols, bad);
-    if (threadIdx.x == 0) scale[row] = s;
-    const double inv = 127.0 / most;
-    const float inv32 = (float)inv;
+    const float inv32 = 127.0f / (float)most;
     char4 *out = reinterpret_cast<char4 *>(q);
+    constexpr float kBorder = 0.5f - 127 * kNear;
+    float furthest = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int c0 = 4 * (threadIdx.x + T * k);
-        if (c0 >= cols) break;
+        const int c = 4 * (threadIdx.x + T * k);
+        if (c >= cols) break;
         int n[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float t = v[k][j] * inv32, r = rintf(t);
             n[j] = (int)r;
-            if (fabsf(fabsf(t - r) - 0.5f) < 127 * kNear && c0 + j < cols)
-                n[j] = nearest(src.value(row * cols + c0 + j, c0 + j), most, inv);
-            if (bad || s == 0) n[j] = 0;
+            furthest = fmaxf(furthest, fabsf(t - r));
         }
-        out[q8_at(row, c0, frags) / 4] = make_char4((char)n[0], (char)n[1], (char)n[2], (char)n[3]);
+        out[q8_at(row, c, frags) / 4] = make_char4((char)n[0], (char)n[1], (char)n[2], (char)n[3]);
     }
+    if (furthest > kBorder) {
+        uint64_t near = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
+            const float t = v[i / 4][i % 4] * inv32;
+            near |= (uint64_t)(fabsf(t - rintf(t)) > kBorder && column(i) < cols) << i;
+        }
+        const double inv = 127.0 / most;
+        for (; near; near &= near - 1) {
+            const int i = __builtin_ctzll(near);
+            q[q8_at(row, column(i), frags)] = (int8_t)nearest(value64(i), most, inv);
+        }
+    }
+    int bad = 0;
+    const float s = scale_of(src, most, sum, cols, bad);
+    if (threadIdx.x == 0) scale[row] = s;
+    if (bad || s == 0)
+        for (int c = 4 * threadIdx.x; c < cols; c += 4 * T) out[q8_at(row, c, frags) / 4] = make_char4(0, 0, 0, 0);
 }
 
 // A block a 16 rows x 256 columns: four rows of four columns a thread.
@@ -347,30 +432,23 @@ void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
                                                                   (int)q8_frags(q.cols), grouped);
 }
 
-// Rows that fit a block's registers: few of them with 16 waves a row, which
-// have it sooner, many with 4, of which a CU runs several rows at once.
+// Rows that fit a block's registers: eight waves a row, more loads in flight
+// than four (us with 4 / 8 / 16 waves: silu 2048 x 9728 42 / 39 / 53, norm
+// 8192 x 2560 57 / 56 / 63, rows 8192 x 4096 34 / 31 / 42; one row: norm of
+// 2560 4.1 / 3.4 / 3.9).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
     const size_t c = q.cols;
-    if (q.rows > 256 && c <= 10240) {
-        if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
-        else if (c <= 2048) launch_held<Source, 4, 2>(s, q, src);
-        else if (c <= 3 * 1024) launch_held<Source, 4, 3>(s, q, src);
-        else if (c <= 4096) launch_held<Source, 4, 4>(s, q, src);
-        else if (c <= 6 * 1024) launch_held<Source, 4, 6>(s, q, src);
-        else if (c <= 8192) launch_held<Source, 4, 8>(s, q, src);
-        else launch_held<Source, 4, 10>(s, q, src);
-    } else if (c <= 20480) {
-        if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
-        else if (c <= 4096) launch_held<Source, 16, 1>(s, q, src);
-        else if (c <= 8192) launch_held<Source, 16, 2>(s, q, src);
-        else if (c <= 12288) launch_held<Source, 16, 3>(s, q, src);
-        else launch_held<Source, 16, 5>(s, q, src);
-    } else {
+    if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
+    else if (c <= 2048) launch_held<Source, 8, 1>(s, q, src);
+    else if (c <= 4096) launch_held<Source, 8, 2>(s, q, src);
+    else if (c <= 6144) launch_held<Source, 8, 3>(s, q, src);
+    else if (c <= 10240) launch_held<Source, 8, 5>(s, q, src);
+    else if (c <= 20480) launch_held<Source, 16, 5>(s, q, src);
+    else
         any_row_kernel<Source, 16><<<(unsigned)q.rows, 1024, 0, s>>>(src, q.ptr, q.scale, (int)q.cols,
                                                                      (int)q8_frags(q.cols), true);
-    }
     return hipGetLastError();
 }
 
