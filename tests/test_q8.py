@@ -111,6 +111,16 @@ def test_write_and_read(hip, rows, cols):
 
 
 @gpu
+def test_write_and_read_in_pieces(hip):
+    """More integers (71 MB) than the block that they go through holds."""
+    r = np.random.default_rng(9)
+    v, s = r.integers(-128, 128, (7001, 10101), dtype=np.int8), r.standard_normal(7001).astype(np.float32)
+    q = q8(hip, v, s)
+    got, scales = hip.read_q8(q)
+    assert np.array_equal(got, v) and np.array_equal(scales, s)
+
+
+@gpu
 def test_allocated_rows_are_zero(hip):
     q = hip.alloc_q8(5, 100)
     v, s = hip.read_q8(q)

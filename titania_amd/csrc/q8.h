@@ -31,6 +31,8 @@ __host__ __device__ constexpr size_t q8_at(size_t row, size_t col, size_t frags)
     return ((row >> 4) * frags + (col >> 6)) * 1024 + ((row & 15) + (col >> 4 & 3) * 16) * 16 + (col & 15);
 }
 
+// Rows row0 .. of q from `rows` of them row-major in plain (in), or to there.
+hipError_t launch_reorder_q8(hipStream_t s, const th_q8 &q, int8_t *plain, size_t row0, size_t rows, bool in);
 // q = 8-bit rows of x [rows][cols] (f32, or bf16 weights).
 hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x);
 hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16_t *w);

@@ -1,6 +1,5 @@
 // The C ABI's 8-bit rows (th_q8): handles, host copies and argument checks.
 #include <algorithm>
-#include <cstring>
 #include <new>
 
 #include "common.h"
@@ -17,6 +16,9 @@ namespace {
 
 // Bytes of the integers of `rows` rows.
 size_t value_bytes(size_t rows, size_t cols) { return th::q8_blocks(rows) * th::q8_frags(cols) * 1024; }
+
+// The device's block of partials, which calls use in the stream's order.
+constexpr size_t kPartBytes = std::max(th::kPartFloats, th::kAttnRoundFloats) * sizeof(float);
 
 }  // namespace
 
@@ -79,21 +81,20 @@ int th_q8_read(th_device *dev, const th_q8 *q, int8_t *values, float *scales) {
     TH_REQUIRE(q->rows == 0 || (values && scales), "th_q8_read: null output");
     TH_Q8_HERE(dev, q);
     TH_HIP(hipSetDevice(dev->ordinal));
-    const size_t bytes = value_bytes(q->rows, q->cols), frags = th::q8_frags(q->cols);
-    auto *raw = new (std::nothrow) int8_t[std::max<size_t>(bytes, 1)];
-    if (!raw) return fail(TH_ERR_NOMEM, "out of host memory");
+    // Through the device's block of partials, as many rows at a time as it holds.
+    auto *plain = reinterpret_cast<int8_t *>(dev->part);
+    const size_t most = kPartBytes / q->cols;
     hipError_t e = hipSuccess;
-    if (bytes) {
-        e = hipMemcpyAsync(raw, q->ptr, bytes, hipMemcpyDeviceToHost, dev->stream);
+    for (size_t r = 0; r < q->rows && e == hipSuccess; r += most) {
+        const size_t n = std::min(most, q->rows - r);
+        e = th::launch_reorder_q8(dev->stream, *q, plain, r, n, false);
         if (e == hipSuccess)
-            e = hipMemcpyAsync(scales, q->scale, q->rows * sizeof(float), hipMemcpyDeviceToHost, dev->stream);
+            e = hipMemcpyAsync(values + r * q->cols, plain, n * q->cols, hipMemcpyDeviceToHost, dev->stream);
     }
-    if (e == hipSuccess) e = hipStreamSynchronize(dev->stream);
-    if (e == hipSuccess)
-        for (size_t r = 0; r < q->rows; ++r)
-            for (size_t c = 0; c < q->cols; c += 16)
-                memcpy(values + r * q->cols + c, raw + th::q8_at(r, c, frags), std::min<size_t>(16, q->cols - c));
-    delete[] raw;
+    if (e == hipSuccess && q->rows)
+        e = hipMemcpyAsync(scales, q->scale, q->rows * sizeof(float), hipMemcpyDeviceToHost, dev->stream);
+    const hipError_t done = hipStreamSynchronize(dev->stream);
+    if (e == hipSuccess) e = done;
     if (e != hipSuccess) return fail(TH_ERR_HIP, "reading 8-bit rows failed: %s", hipGetErrorString(e));
     return TH_OK;
 }
@@ -104,18 +105,17 @@ int th_q8_write(th_device *dev, th_q8 *q, const int8_t *values, const float *sca
     TH_REQUIRE(q->rows == 0 || (values && scales), "th_q8_write: null data");
     TH_Q8_HERE(dev, q);
     TH_HIP(hipSetDevice(dev->ordinal));
-    const size_t bytes = value_bytes(q->rows, q->cols), frags = th::q8_frags(q->cols);
-    if (bytes == 0) return TH_OK;
-    auto *raw = new (std::nothrow) int8_t[bytes]();
-    if (!raw) return fail(TH_ERR_NOMEM, "out of host memory");
-    for (size_t r = 0; r < q->rows; ++r)
-        for (size_t c = 0; c < q->cols; c += 16)
-            memcpy(raw + th::q8_at(r, c, frags), values + r * q->cols + c, std::min<size_t>(16, q->cols - c));
-    hipError_t e = hipMemcpyAsync(q->ptr, raw, bytes, hipMemcpyHostToDevice, dev->stream);
-    if (e == hipSuccess)
+    auto *plain = reinterpret_cast<int8_t *>(dev->part);
+    const size_t most = kPartBytes / q->cols;
+    hipError_t e = hipSuccess;
+    for (size_t r = 0; r < q->rows && e == hipSuccess; r += most) {
+        const size_t n = std::min(most, q->rows - r);
+        e = hipMemcpyAsync(plain, values + r * q->cols, n * q->cols, hipMemcpyHostToDevice, dev->stream);
+        if (e == hipSuccess) e = th::launch_reorder_q8(dev->stream, *q, plain, r, n, true);
+    }
+    if (e == hipSuccess && q->rows)
         e = hipMemcpyAsync(q->scale, scales, q->rows * sizeof(float), hipMemcpyHostToDevice, dev->stream);
-    const hipError_t done = hipStreamSynchronize(dev->stream);  // raw is read until then
-    delete[] raw;
+    const hipError_t done = hipStreamSynchronize(dev->stream);  // the host's arrays are read until then
     if (e == hipSuccess) e = done;
     if (e != hipSuccess) return fail(TH_ERR_HIP, "writing 8-bit rows failed: %s", hipGetErrorString(e));
     return TH_OK;
@@ -181,7 +181,7 @@ int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x)
     TH_Q8_HERE(dev, x);
     TH_HIP(hipSetDevice(dev->ordinal));
     TH_HIP(th::launch_matmul_q8(dev->stream, out->ptr, *w, *x, reinterpret_cast<int *>(dev->part),
-                                std::max(th::kPartFloats, th::kAttnRoundFloats)));
+                                kPartBytes / sizeof(int)));
     return TH_OK;
 }
 

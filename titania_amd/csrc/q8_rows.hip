@@ -424,6 +424,27 @@ __global__ __launch_bounds__(256) void dequantize_kernel(float *__restrict__ out
     }
 }
 
+struct __attribute__((packed, aligned(1))) Loose16 {
+    uint32_t w[4];
+};
+
+// Row-major integers to the fragments' order (IN) or back, 16 columns a thread.
+template <bool IN>
+__global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, int8_t *__restrict__ plain, size_t row0,
+                                                      size_t rows, int cols, int frags) {
+    const int pieces = (cols + 15) / 16;
+    const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x, r = e / pieces;
+    if (r >= rows) return;
+    const int c = (int)(e % pieces) * 16;
+    int8_t *in = plain + r * cols + c, *at = q + q8_at(row0 + r, c, frags);
+    if (c + 16 <= cols) {
+        if (IN) *reinterpret_cast<Loose16 *>(at) = *reinterpret_cast<const Loose16 *>(in);
+        else *reinterpret_cast<Loose16 *>(in) = *reinterpret_cast<const Loose16 *>(at);
+    } else {
+        for (int j = 0; c + j < cols; ++j) (IN ? at : in)[j] = (IN ? in : at)[j];
+    }
+}
+
 template <class Source, int W, int N>
 void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
     const bool grouped = q.rows >= 128;
@@ -469,6 +490,15 @@ hipError_t launch_add_rmsnorm_q8(hipStream_t s, float *x, const float *y, const 
 
 hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, const float *up) {
     return launch_rows(s, q, SiluSource{gate, up});
+}
+
+hipError_t launch_reorder_q8(hipStream_t s, const th_q8 &q, int8_t *plain, size_t row0, size_t rows, bool in) {
+    if (rows == 0) return hipSuccess;
+    const unsigned blocks = (unsigned)((rows * ((q.cols + 15) / 16) + 255) / 256);
+    const int cols = (int)q.cols, frags = (int)q8_frags(q.cols);
+    if (in) reorder_kernel<true><<<blocks, 256, 0, s>>>(q.ptr, plain, row0, rows, cols, frags);
+    else reorder_kernel<false><<<blocks, 256, 0, s>>>(q.ptr, plain, row0, rows, cols, frags);
+    return hipGetLastError();
 }
 
 hipError_t launch_dequantize_q8(hipStream_t s, float *out, const th_q8 &q) {
