@@ -57,6 +57,29 @@ __device__ __forceinline__ f32x4 scaled(i32x4 sum, float xs, float4 ws) {
                  (float)sum[3] * xs * ws.w};
 }
 
+// Blocks are dealt to the 8 XCDs in turn: a permutation of `count` blocks by
+// which each XCD has a range of its own, whose neighbours share its L2.
+__device__ __forceinline__ int xcd_range(int lin, int count) {
+    const int xcd = lin & 7, q = count >> 3, rest = count & 7;
+    return xcd * q + (xcd < rest ? xcd : rest) + (lin >> 3);
+}
+
+// Four values of a row of which `left` are left, at any multiple of 4 bytes
+// (rows of a number that 4 does not divide): the memory path takes 16 bytes at
+// any of them.
+__device__ __forceinline__ void store4(float *o, f32x4 v, int left) {
+    struct __attribute__((packed, aligned(4))) Loose {
+        f32x4 v;
+    };
+    if (left >= 4) {
+        reinterpret_cast<Loose *>(o)->v = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < left) o[i] = v[i];
+    }
+}
+
 // Few tokens. A block takes RB row blocks and TB token blocks, its W waves the
 // fragments in turn (so that the block reads consecutive memory), U of them in
 // flight a wave; the waves' sums meet in LDS.
@@ -68,11 +91,8 @@ template <int RB, int TB, int W, int U>
 __global__ __launch_bounds__(64 * W) void few_kernel(Args a) {
     __shared__ i32x4 red[W * RB * TB * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // Blocks of the same weights and other tokens run on one XCD (blocks are
-    // dealt to the 8 XCDs in turn), so that its L2 has the weights once.
-    const int tbs = ((a.n + 15) / 16 + TB - 1) / TB, lin = blockIdx.x;
-    const int rb0 = (lin / (8 * tbs) * 8 + lin % 8) * RB, tb0 = lin % (8 * tbs) / 8 * TB;
-    if (rb0 * 16 >= a.rows) return;
+    const int tbs = ((a.n + 15) / 16 + TB - 1) / TB, of_xcd = xcd_range(blockIdx.x, gridDim.x);
+    const int rb0 = of_xcd / tbs * RB, tb0 = of_xcd % tbs * TB;
     const unsigned block = (unsigned)a.frags * 1024;
     const __amdgpu_buffer_rsrc_t rw = blocks_from(a.w, a.rows, rb0, a.frags), rx = blocks_from(a.x, a.n, tb0, a.frags);
     unsigned xo[TB];
@@ -113,23 +133,14 @@ __global__ __launch_bounds__(64 * W) void few_kernel(Args a) {
 #pragma unroll
         for (int k = 1; k < W; ++k) sum += red[k * RB * TB * 64 + e];
         const f32x4 v = scaled(sum, a.x_scale[t], *reinterpret_cast<const float4 *>(a.w_scale + r));
-        float *o = a.out + (size_t)t * a.rows + r;
-        if (a.rows % 4 == 0) {
-            *reinterpret_cast<f32x4 *>(o) = v;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r + i < a.rows) o[i] = v[i];
-        }
+        store4(a.out + (size_t)t * a.rows + r, v, a.rows - r);
     }
 }
 
-// The tile of a block: blocks are dealt to the 8 XCDs in turn, and each XCD
-// takes a contiguous range of tiles, in panels of 8 tiles of tokens, so that
-// the tiles that it has in work share operands in its L2.
+// The tile of a block: an XCD's tiles go in panels of 8 tiles of tokens, so
+// that those that it has in work share operands in its L2.
 __device__ __forceinline__ void tile_of_block(int lin, int gr, int gt, int &tr, int &tt) {
-    const int tiles = gr * gt, xcd = lin & 7, q = tiles >> 3, rest = tiles & 7;
-    const int i = xcd * q + (xcd < rest ? xcd : rest) + (lin >> 3);
+    const int i = xcd_range(lin, gr * gt);
     const int high = gt < 8 ? gt : 8, panel = i / (high * gr), in = i % (high * gr);
     const int height = gt - panel * high < high ? gt - panel * high : high;
     tr = in / height;
@@ -274,21 +285,14 @@ __global__ __launch_bounds__(64 * T::kWaves) void tile_kernel(Args a, int gr, in
         for (int i = 0; i < FM; ++i)
             *reinterpret_cast<f32x4 *>(lines + lt * T::kLine + i * 16 + lr) =
                 a.ksplit > 1 ? __builtin_bit_cast(f32x4, acc[i][j]) : scaled(acc[i][j], xs[j], ws[i]);
-        if (a.rows % 4 == 0) {
 #pragma unroll
-            for (int q = 0; q < FM; ++q) {
-                const int e = q * 64 + lane, t = e / (FM * 4), c = e % (FM * 4) * 4;
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(lines + t * T::kLine + c);
-                if (t0 + j * 16 + t < a.n && r0 + c < a.rows)
-                    __builtin_nontemporal_store(
-                        v, reinterpret_cast<f32x4 *>(out + (size_t)(t0 + j * 16 + t) * a.rows + r0 + c));
-            }
-        } else {
-            for (int e = lane; e < 16 * 16 * FM; e += 64) {
-                const int t = e / (FM * 16), c = e % (FM * 16);
-                if (t0 + j * 16 + t < a.n && r0 + c < a.rows)
-                    out[(size_t)(t0 + j * 16 + t) * a.rows + r0 + c] = lines[t * T::kLine + c];
-            }
+        for (int q = 0; q < FM; ++q) {
+            const int e = q * 64 + lane, t = e / (FM * 4), c = e % (FM * 4) * 4;
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(lines + t * T::kLine + c);
+            if (t0 + j * 16 + t >= a.n || r0 + c >= a.rows) continue;
+            float *o = out + (size_t)(t0 + j * 16 + t) * a.rows + r0 + c;
+            if (a.rows % 4 == 0) __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(o));
+            else store4(o, v, a.rows - r0 - c);
         }
     }
 }
@@ -315,8 +319,7 @@ size_t blocks_of(int rows, int each) { return ((size_t)(rows + 15) / 16 + each -
 
 template <int RB, int TB, int W>
 void few(hipStream_t s, const Args &a) {
-    const size_t rbs = blocks_of(a.rows, RB), tbs = blocks_of(a.n, TB);
-    few_kernel<RB, TB, W, 5><<<(unsigned)((rbs + 7) / 8 * 8 * tbs), 64 * W, 0, s>>>(a);
+    few_kernel<RB, TB, W, 5><<<(unsigned)(blocks_of(a.rows, RB) * blocks_of(a.n, TB)), 64 * W, 0, s>>>(a);
 }
 
 template <class T>
@@ -330,23 +333,29 @@ void tiles(hipStream_t s, const Args &a) {
 }
 
 // About how long a launch takes, in us, from its shape alone. The constants
-// are fitted to back-to-back launches of every variant over 9 matrices (1024 x
-// 1024 to 4096 x 16384) and 14 counts of tokens (20 to 8192): the variant that
-// they choose is 1.01 times the fastest one's time in the geometric mean, 1.16
-// at most.
+// are fitted to back-to-back launches of every variant over 17 matrices (7 x
+// 3000 to 4096 x 16384) and 6 to 14 counts of tokens (20 to 8192): the variant
+// that they choose takes 1.02 times the fastest one's time in the geometric
+// mean, 1.42 times at most (1652 tokens x 51 x 6076; 1.18 for all others).
 constexpr double kLaunch = 2.4;
 constexpr int kCus = 256;
 
-// The work of the CUs and the matrices' way from and to HBM, which mostly overlap.
-double overlapped(const Args &a, double work) {
-    const double hbm = (1024.0 * blocks_of(a.rows, 1) * a.frags + 4.0 * a.n * a.rows) / 5.6e6;
-    return kLaunch + std::max(work, hbm) + 0.16 * std::min(work, hbm);
+// The work of the CUs and the matrices' way to and from them, which mostly overlap.
+double overlapped(double work, double bytes) {
+    const double way = bytes / 9.0e6;
+    return kLaunch + std::max(work, way) + 0.15 * std::min(work, way);
 }
 
-// Few tokens: what a CU takes in through its memory path, block after block.
+double weights_and_results(const Args &a) { return 1024.0 * blocks_of(a.rows, 1) * a.frags + 4.0 * a.n * a.rows; }
+double tokens(const Args &a) { return 1024.0 * blocks_of(a.n, 1) * a.frags; }
+
+// Few tokens: what a CU takes in through its memory path, block after block;
+// each group of row blocks reads the tokens again, mostly from L2.
 double few_us(const Args &a, int rb, int tb) {
-    const double rounds = std::ceil((double)(blocks_of(a.rows, rb) * blocks_of(a.n, tb)) / kCus);
-    return overlapped(a, rounds * (a.frags * (rb + tb) / 113.0 + 0.4 + 0.05 * rb * tb));
+    const double groups = (double)blocks_of(a.rows, rb), rounds = groups * blocks_of(a.n, tb) / kCus;
+    const double work = a.frags * (rb + tb) / 84.0 + 0.75 + 0.04 * rb * tb;
+    return overlapped((0.73 * std::ceil(rounds) + 0.27 * std::max(rounds, 1.0)) * work,
+                      weights_and_results(a) + tokens(a) * (1 + 0.11 * (groups - 1)));
 }
 
 struct TileVariant {
@@ -370,15 +379,16 @@ constexpr TileVariant kTiles[] = {
 };
 
 // Tiles: rounds of a tile a CU, each with its steps of K and its epilogue (the
-// variant of which a CU holds two: a round of both takes 1.37 times one tile's
+// variant of which a CU holds two: a round of both takes 1.29 times one tile's
 // time; with one it waits for its short ring). A split's sums go out and come
 // in again.
 double tile_us(const Args &a, const TileVariant &v, int ksplit) {
     const double count = (double)(blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn)) * ksplit;
     const double steps = std::ceil(a.frags / 2.0 / ksplit), rounds = std::ceil(count / (kCus * v.resident));
-    const double one = steps * (0.173 + 0.0262 * v.products) + 0.6 + 0.13 * v.products;
-    const double us = overlapped(a, rounds * one * (v.resident == 1 ? 1.0 : count > kCus ? 1.37 : 1.13));
-    return ksplit == 1 ? us : us + 3.4 + ksplit * 8.0 * a.n * a.rows / 3.9e6;
+    const double one = steps * (0.306 + 0.029 * v.products) + 0.6 + 0.15 * v.products;
+    const double us = overlapped(rounds * one * (v.resident == 1 ? 1.0 : count > kCus ? 1.29 : 1.08),
+                                 weights_and_results(a) + tokens(a));
+    return ksplit == 1 ? us : us + 3.8 + ksplit * 8.0 * a.n * a.rows / 3.9e6;
 }
 
 }  // namespace
@@ -399,11 +409,9 @@ hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_
     const TileVariant *tile = nullptr;
     int pick = 0, ksplit = 1;
     double best = 1e30;
-    if (a.n <= 512) {
-        const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}};
-        for (int i = 0; i < 4; ++i)
-            if (const double us = few_us(a, shapes[i][0], shapes[i][1]); us < best) best = us, pick = i;
-    }
+    const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}};
+    for (int i = 0; i < 4; ++i)
+        if (const double us = few_us(a, shapes[i][0], shapes[i][1]); us < best) best = us, pick = i;
     for (const TileVariant &v : kTiles) {
         const size_t count = blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn);
         if (const double us = tile_us(a, v, 1); us < best) best = us, tile = &v, ksplit = 1;
@@ -418,7 +426,7 @@ hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_
     } else if (pick == 0) {
         a.frags <= 24 ? few<1, 1, 4>(s, a) : few<1, 1, 8>(s, a);
     } else if (pick == 1) {
-        few<1, 2, 8>(s, a);
+        a.frags <= 24 ? few<1, 2, 4>(s, a) : few<1, 2, 8>(s, a);
     } else {
         pick == 2 ? few<2, 2, 8>(s, a) : few<2, 4, 8>(s, a);
     }
