@@ -456,12 +456,15 @@ void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
 // Rows that fit a block's registers: eight waves a row, more loads in flight
 // than four (us with 4 / 8 / 16 waves: silu 2048 x 9728 42 / 39 / 53, norm
 // 8192 x 2560 57 / 56 / 63, rows 8192 x 4096 34 / 31 / 42; one row: norm of
-// 2560 4.1 / 3.4 / 3.9).
+// 2560 4.1 / 3.4 / 3.9), and one wave for short ones (norm 8192 x 128 6.7
+// where four waves take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
     const size_t c = q.cols;
-    if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
+    if (c <= 256) launch_held<Source, 1, 1>(s, q, src);
+    else if (c <= 512) launch_held<Source, 1, 2>(s, q, src);
+    else if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
     else if (c <= 2048) launch_held<Source, 8, 1>(s, q, src);
     else if (c <= 4096) launch_held<Source, 8, 2>(s, q, src);
     else if (c <= 6144) launch_held<Source, 8, 3>(s, q, src);
