@@ -18,7 +18,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from titania_amd import InvalidArgument, Tensor, _lib
+from titania_amd import HipError, InvalidArgument, Tensor, _lib
 from titania_amd.synth import bf16_to_f32, f32_to_bf16
 
 EPS = 1e-6
@@ -48,7 +48,7 @@ def far_from_borders(v):
 
 def product32(wq, ws, xq, xs):
     """out[t][r] in the order of the definition: the exact sum to f32, times x's scale, times w's."""
-    total = xq.astype(np.int64) @ wq.astype(np.int64).T
+    total = xq.astype(np.float64) @ wq.astype(np.float64).T  # exact: every partial sum is below 2^53
     with np.errstate(all="ignore"):
         return total.astype(np.float32) * xs[:, None] * ws[None, :]
 
@@ -321,14 +321,20 @@ PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 17, 65), (2, 3, 127), (15, 15, 128), (16
             (33, 65, 320), (63, 127, 100), (65, 129, 1101), (50, 1003, 1101), (127, 255, 384), (129, 257, 640),
             (255, 130, 1000), (257, 300, 513), (300, 1000, 70), (513, 511, 260), (1, 1024, 2048), (1, 9728, 2560),
             (4, 2560, 9728), (11, 4096, 2560), (64, 2560, 9728), (512, 1030, 2560), (1, 5, 131071), (40, 20, 131071),
-            (1000, 16, 128), (3, 20000, 33), (700, 2050, 200)]
+            (1000, 16, 128), (3, 20000, 33), (700, 2050, 200),
+            # Each variant that a product can take, whole and with K split.
+            (17, 515, 2500), (17, 3001, 2500), (33, 3001, 60), (70, 3001, 60), (17, 3001, 60), (131, 3001, 60),
+            (50, 1037, 16000), (131, 7001, 60), (33, 3001, 16000), (700, 7001, 60), (2000, 1037, 60),
+            (70, 3001, 16000), (515, 7001, 60), (4100, 130, 9000), (700, 7001, 130), (131, 7001, 9000),
+            (8192, 1037, 60), (131, 7001, 16000), (1300, 7001, 60), (1550, 7001, 60), (1030, 12000, 600),
+            (6000, 3001, 60)]
 
 
 @gpu
 @pytest.mark.parametrize("n,rows,cols", PRODUCTS)
 def test_matmul(hip, n, rows, cols):
     r = np.random.default_rng(n + rows + cols)
-    xq, wq = (r.integers(-127, 128, (m, cols), dtype=np.int8) for m in (n, rows))
+    xq, wq = (r.integers(-128, 128, (m, cols), dtype=np.int8) for m in (n, rows))
     xs, ws = (r.random(m).astype(np.float32) + np.float32(0.01) for m in (n, rows))
     out = buf(hip, np.full(n * rows + 64, -5.0))  # the tail stays as it is
     hip.resize(out, n * rows)
@@ -545,6 +551,46 @@ def test_capture_refuses_copies_and_allocations(hip):
     hip.write_q8(q, np.ones((2, 64), np.int8), np.ones(2))
     assert hip.read_q8(q)[0].all()
     graph.free()
+
+
+@gpu
+def test_graphs_share_the_block_of_sums(hip):
+    """Two captured products that split K (their sums go through one block of
+    the device's), replayed in turn with an eager one between."""
+    r = np.random.default_rng(12)
+    runs = []
+    for n, rows, cols in ((70, 3001, 16000), (131, 2050, 16000)):
+        xq, wq = (r.integers(-127, 128, (m, cols), dtype=np.int8) for m in (n, rows))
+        xs, ws = (r.random(m).astype(np.float32) for m in (n, rows))
+        runs.append((hip.alloc(n * rows), q8(hip, wq, ws), q8(hip, xq, xs), product32(wq, ws, xq, xs).reshape(-1)))
+    graphs = []
+    for out, w, x, _ in runs:
+        hip.graph_begin()
+        try:
+            hip.matmul_q8(out, w, x)
+        finally:
+            graphs.append(hip.graph_end())
+    for replay in range(3):
+        for out, *_ in runs:
+            hip.write(out, np.zeros(len(out), np.float32))
+        for g in graphs:
+            g.launch()
+        assert all(np.array_equal(hip.read(out), want) for out, _, _, want in runs), f"replay {replay}"
+        hip.matmul_q8(*runs[replay % 2][:3])
+    for g in graphs:
+        g.free()
+
+
+@gpu
+def test_allocation_that_fails_leaves_no_error(hip):
+    """64 TB are not there; the next launch does not report it."""
+    with pytest.raises(HipError) as e:
+        hip.alloc_q8((1 << 29) + 5, 131071)
+    assert e.value.code == _lib.TH_ERR_NOMEM
+    x = np.arange(64, dtype=np.float32)
+    q = hip.alloc_q8(1, 64)
+    hip.quantize_q8(q, buf(hip, x))
+    assert np.array_equal(hip.read_q8(q)[0], rows64(x)[0])
 
 
 @gpu

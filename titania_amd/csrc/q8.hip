@@ -14,6 +14,25 @@ namespace {
 #define TH_Q8_HERE(dev, q) \
     TH_REQUIRE((q)->ordinal == (dev)->ordinal, "8-bit rows of GPU %d on GPU %d", (q)->ordinal, (dev)->ordinal)
 
+// The device made current, as allocations and launches want it, for a call.
+struct Current {
+    int before = 0;
+    bool changed = false;
+    hipError_t error;
+    explicit Current(const th_device *dev) : error(hipGetDevice(&before)) {
+        if (error == hipSuccess && before != dev->ordinal) {
+            error = hipSetDevice(dev->ordinal);
+            changed = error == hipSuccess;
+        }
+    }
+    ~Current() {
+        if (changed) (void)hipSetDevice(before);
+    }
+};
+#define TH_Q8_CURRENT(dev)   \
+    Current current_(dev);   \
+    TH_HIP(current_.error)
+
 // Bytes of the integers of `rows` rows.
 size_t value_bytes(size_t rows, size_t cols) { return th::q8_blocks(rows) * th::q8_frags(cols) * 1024; }
 
@@ -29,7 +48,7 @@ int th_q8_alloc(th_device *dev, size_t rows, size_t cols, th_q8 **out) {
     TH_NOT_CAPTURING(dev, "th_q8_alloc");
     TH_REQUIRE(cols > 0 && cols <= th::kQ8MaxCols, "8-bit rows of %zu columns: 1 to %zu", cols, th::kQ8MaxCols);
     TH_REQUIRE(rows < ((size_t)1 << 30), "%zu 8-bit rows: fewer than 2^30", rows);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     auto *q = new (std::nothrow) th_q8();
     if (!q) return fail(TH_ERR_NOMEM, "out of host memory");
     const size_t values = value_bytes(rows, cols), bytes = values + std::max<size_t>(th::q8_blocks(rows) * 64, 64);
@@ -37,6 +56,7 @@ int th_q8_alloc(th_device *dev, size_t rows, size_t cols, th_q8 **out) {
     if (e == hipSuccess) e = hipMemsetAsync(q->ptr, 0, bytes, dev->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(dev->stream);
     if (e != hipSuccess) {
+        (void)hipGetLastError();  // reported here, not by the next launch
         if (q->ptr) (void)hipFree(q->ptr);
         delete q;
         return fail(e == hipErrorOutOfMemory ? TH_ERR_NOMEM : TH_ERR_HIP, "alloc of %zu x %zu 8-bit rows failed: %s",
@@ -80,7 +100,7 @@ int th_q8_read(th_device *dev, const th_q8 *q, int8_t *values, float *scales) {
     TH_NOT_CAPTURING(dev, "th_q8_read");
     TH_REQUIRE(q->rows == 0 || (values && scales), "th_q8_read: null output");
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     // Through the device's block of partials, as many rows at a time as it holds.
     auto *plain = reinterpret_cast<int8_t *>(dev->part);
     const size_t most = kPartBytes / q->cols;
@@ -104,7 +124,7 @@ int th_q8_write(th_device *dev, th_q8 *q, const int8_t *values, const float *sca
     TH_NOT_CAPTURING(dev, "th_q8_write");
     TH_REQUIRE(q->rows == 0 || (values && scales), "th_q8_write: null data");
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     auto *plain = reinterpret_cast<int8_t *>(dev->part);
     const size_t most = kPartBytes / q->cols;
     hipError_t e = hipSuccess;
@@ -125,7 +145,7 @@ int th_quantize_q8(th_device *dev, th_q8 *q, const th_buffer *x) {
     TH_REQUIRE(dev && q && x, "th_quantize_q8: null argument");
     TH_REQUIRE(x->len == q->rows * q->cols, "x holds %zu activations, not %zu rows of %zu", x->len, q->rows, q->cols);
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_quantize_q8(dev->stream, *q, x->ptr));
     return TH_OK;
 }
@@ -135,7 +155,7 @@ int th_quantize_weight_q8(th_device *dev, th_q8 *q, const th_weight *w) {
     TH_REQUIRE(w->ndim == 2 && w->shape[0] == q->rows && w->shape[1] == q->cols,
                "the weight is not a matrix of %zu rows of %zu", q->rows, q->cols);
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_quantize_weight_q8(dev->stream, *q, w->ptr));
     return TH_OK;
 }
@@ -145,7 +165,7 @@ int th_dequantize_q8(th_device *dev, th_buffer *out, const th_q8 *q) {
     TH_REQUIRE(out->len == q->rows * q->cols, "out holds %zu activations, not %zu rows of %zu", out->len, q->rows,
                q->cols);
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_dequantize_q8(dev->stream, out->ptr, *q));
     return TH_OK;
 }
@@ -157,7 +177,7 @@ int th_add_rmsnorm_q8(th_device *dev, th_buffer *x, const th_buffer *y, th_q8 *q
     TH_REQUIRE(!y || y->len >= x->len, "y holds %zu activations, x %zu", y ? y->len : 0, x->len);
     TH_REQUIRE(!y || y->ptr != x->ptr, "y must not alias x");
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_add_rmsnorm_q8(dev->stream, x->ptr, y ? y->ptr : nullptr, *q, w->ptr, eps));
     return TH_OK;
 }
@@ -167,7 +187,7 @@ int th_silu_mul_q8(th_device *dev, th_q8 *q, const th_buffer *gate, const th_buf
     TH_REQUIRE(gate->len == q->rows * q->cols && up->len == gate->len,
                "gate and up hold %zu and %zu activations, not %zu rows of %zu", gate->len, up->len, q->rows, q->cols);
     TH_Q8_HERE(dev, q);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_silu_mul_q8(dev->stream, *q, gate->ptr, up->ptr));
     return TH_OK;
 }
@@ -179,7 +199,7 @@ int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x)
                w->rows);
     TH_Q8_HERE(dev, w);
     TH_Q8_HERE(dev, x);
-    TH_HIP(hipSetDevice(dev->ordinal));
+    TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_matmul_q8(dev->stream, out->ptr, *w, *x, reinterpret_cast<int *>(dev->part),
                                 kPartBytes / sizeof(int)));
     return TH_OK;

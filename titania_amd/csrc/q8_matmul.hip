@@ -374,7 +374,7 @@ constexpr TileVariant variant() {
 // 256, 1.25 rounds, 204 us; 224 x 256, 1.5 rounds, 188 us).
 constexpr TileVariant kTiles[] = {
     variant<2, 1, 4, 2, 4>(), variant<2, 2, 4, 2, 4>(), variant<4, 2, 2, 4, 2>(), variant<4, 2, 2, 4, 4>(),
-    variant<5, 2, 2, 4, 4>(), variant<6, 2, 2, 4, 3>(), variant<4, 4, 2, 4, 3>(), variant<5, 4, 2, 4, 3>(),
+    variant<5, 2, 2, 4, 4>(), variant<6, 2, 2, 4, 3>(), variant<5, 4, 2, 4, 3>(),
     variant<6, 4, 2, 4, 2>(), variant<7, 4, 2, 4, 2>(), variant<8, 4, 2, 4, 2>(), variant<10, 4, 2, 4, 2>(),
 };
 
@@ -391,45 +391,56 @@ double tile_us(const Args &a, const TileVariant &v, int ksplit) {
     return ksplit == 1 ? us : us + 3.8 + ksplit * 8.0 * a.n * a.rows / 3.9e6;
 }
 
+struct FewVariant {
+    int rb, tb;
+    void (*launch)(hipStream_t, const Args &);
+};
+// More waves where a block has much to read and the chip is not full, fewer
+// where there is little (one token, us with 4 / 8 / 16 waves: 1024 x 1024 2.4 /
+// 2.6 / 3.2, 2560 x 9728 7.2 / 6.1 / 5.7).
+constexpr FewVariant kFew[] = {
+    {1, 1, few<1, 1, 8>}, {1, 2, few<1, 2, 8>}, {2, 2, few<2, 2, 8>}, {2, 4, few<2, 4, 8>},  // as the estimate says
+    {1, 1, few<1, 1, 4>}, {1, 2, few<1, 2, 4>},                                              // for short rows
+    {1, 1, few<1, 1, 16>},                                                                   // for long ones
+};
+
+// What a product takes: a variant of kFew, or of kTiles with K in ksplit parts.
+struct Choice {
+    const FewVariant *few;
+    const TileVariant *tile;
+    int ksplit;
+};
+
+Choice choose(const Args &a, size_t part_len) {
+    const bool is_short = a.frags <= 24;
+    if (a.n <= 16) {
+        const bool is_long = a.frags >= 128 && blocks_of(a.rows, 1) <= (size_t)kCus;
+        return {&kFew[is_short ? 4 : is_long ? 6 : 0], nullptr, 1};
+    }
+    Choice best{};
+    double least = 1e30;
+    for (int i = 0; i < 4; ++i)
+        if (const double us = few_us(a, kFew[i].rb, kFew[i].tb); us < least)
+            least = us, best = {&kFew[is_short && i < 2 ? i + 4 : i], nullptr, 1};
+    for (const TileVariant &v : kTiles) {
+        if (const double us = tile_us(a, v, 1); us < least) least = us, best = {nullptr, &v, 1};
+        // As many parts as fill the chip, of two steps at least.
+        const size_t count = blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn);
+        const int z = (int)std::min<size_t>({kCus / count, (size_t)a.frags / 4, 16});
+        if (z < 2 || (size_t)z * a.n * a.rows > part_len) continue;
+        if (const double us = tile_us(a, v, z); us < least) least = us, best = {nullptr, &v, z};
+    }
+    return best;
+}
+
 }  // namespace
 
 hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len) {
     if (x.rows == 0 || w.rows == 0) return hipSuccess;
     Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols), part, 1};
-    const size_t rbs = blocks_of(a.rows, 1);
-    if (a.n <= 16) {
-        // More waves where a block has much to read and the chip is not full,
-        // fewer where there is little (one token, us with 4 / 8 / 16 waves:
-        // 1024 x 1024 2.4 / 2.6 / 3.2, 2560 x 9728 7.2 / 6.1 / 5.7).
-        if (a.frags <= 24) few<1, 1, 4>(s, a);
-        else if (a.frags >= 128 && rbs <= kCus) few<1, 1, 16>(s, a);
-        else few<1, 1, 8>(s, a);
-        return hipGetLastError();
-    }
-    const TileVariant *tile = nullptr;
-    int pick = 0, ksplit = 1;
-    double best = 1e30;
-    const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}};
-    for (int i = 0; i < 4; ++i)
-        if (const double us = few_us(a, shapes[i][0], shapes[i][1]); us < best) best = us, pick = i;
-    for (const TileVariant &v : kTiles) {
-        const size_t count = blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn);
-        if (const double us = tile_us(a, v, 1); us < best) best = us, tile = &v, ksplit = 1;
-        // As many parts as fill the chip, of two steps at least.
-        const int z = (int)std::min<size_t>({count ? kCus / count : 1, (size_t)a.frags / 4, 16});
-        if (z < 2 || (size_t)z * a.n * a.rows > part_len) continue;
-        if (const double us = tile_us(a, v, z); us < best) best = us, tile = &v, ksplit = z;
-    }
-    if (tile) {
-        a.ksplit = ksplit;
-        tile->launch(s, a);
-    } else if (pick == 0) {
-        a.frags <= 24 ? few<1, 1, 4>(s, a) : few<1, 1, 8>(s, a);
-    } else if (pick == 1) {
-        a.frags <= 24 ? few<1, 2, 4>(s, a) : few<1, 2, 8>(s, a);
-    } else {
-        pick == 2 ? few<2, 2, 8>(s, a) : few<2, 4, 8>(s, a);
-    }
+    const Choice c = choose(a, part_len);
+    a.ksplit = c.ksplit;
+    (c.tile ? c.tile->launch : c.few->launch)(s, a);
     return hipGetLastError();
 }
 
