@@ -169,17 +169,27 @@ __device__ __forceinline__ void wait_loads_and_lds() {
 // (1 KB each) that run NS - 1 steps ahead.
 //
 // A wave goes through a step row by row: FN products with one weight
-// fragment, the fragment of two rows on being read meanwhile, and one load
+// fragment, the fragment of kAhead rows on being read meanwhile, and one load
 // issued, so that neither LDS nor the memory path sees bursts. The barrier of a
-// step comes two rows before its end: by then everything of the stage is in
+// step comes kAhead rows before its end: by then everything of the stage is in
 // registers, its slot is free for new loads, and the first fragments of the
-// next stage are read under the last rows' products.
+// next stage are read under the last rows' products (1024 tokens x 2560 x
+// 9728, us, one row ahead / two / three: 39.6 / 38.9 / 36.8; with all of a
+// step's loads and reads at its start, 8192 tokens x 2560 x 9728: 155 -> 149).
+//
+// Bound by the clock the chip holds under it (about 2.0 GHz where all CUs
+// multiply), then by LDS: 8192 tokens x 2560 x 9728 in 149 us, 2740 TOPS,
+// 62% of the cycles with a matrix instruction, 84 MB of results at the end;
+// 512 x 9728 x 2560 in 18 us, of which 2.4 the launch, 1 the first loads, 4
+// the results' 20 MB. Measured and not kept: 32 x 32 x 32 products (8192 tokens
+// 161 us; 6% faster where few CUs work), K's halves on two groups of waves
+// (512 x 9728 x 2560 18.5 us), four waves of 128 x 128 (410 us).
 template <int FM_, int FN_, int WM_, int WN_, int NS_>
 struct Tile {
     static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, NS = NS_, BM = FM * WM, BN = FN * WN;
     static constexpr int kWaves = WM * WN, kFrags = 2 * (BM + BN);                         // of a stage
     static constexpr int kLoads = kFrags / kWaves, kMostLoads = (kFrags + kWaves - 1) / kWaves;  // a wave's
-    static constexpr int kRows = 2 * FM, kAhead = 2;
+    static constexpr int kRows = 2 * FM, kAhead = FM >= 4 ? 3 : 2;
     static constexpr int kLine = FM * 16 + 4;  // floats of a token in the epilogue, off the banks' period
     static_assert(kMostLoads <= kRows && kWaves * 16 * kLine * 4 <= NS * kFrags * 1024 && NS * kFrags <= 160, "");
     static_assert(kMostLoads >= kAhead, "the prologue issues kAhead loads of the last stage");
