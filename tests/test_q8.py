@@ -147,6 +147,19 @@ def test_quantize(hip, rows, cols):
     assert np.all(np.abs(got - x.astype(np.float64)) <= want_s[:, None] * (0.5 + 127 * 2.0**-23))
 
 
+@gpu
+def test_more_rows_than_a_launch_takes(hip):
+    rows, cols = (1 << 21) + 300, 3
+    x = np.random.default_rng(14).standard_normal((rows, cols)).astype(np.float32)
+    q, out = hip.alloc_q8(rows, cols), hip.alloc(rows * cols)
+    hip.quantize_q8(q, buf(hip, x))
+    want_q, want_s = rows64(x)
+    v, s = hip.read_q8(q)
+    assert np.array_equal(v, want_q) and np.array_equal(s, want_s)
+    hip.dequantize_q8(out, q)
+    assert np.array_equal(hip.read(out).reshape(rows, cols), want_q.astype(np.float32) * want_s[:, None])
+
+
 def special_rows(cols, seed=3):
     """Rows that the definition treats on their own, each beside ordinary ones."""
     x = np.random.default_rng(seed).standard_normal((14, cols)).astype(np.float32)
@@ -289,6 +302,22 @@ def test_silu_mul_special_rows(hip, cols):
     assert near(s, want_s)
     for i in range(len(g)):
         assert np.array_equal(v[i], want_q[i]), f"row {i}"
+
+
+@gpu
+@pytest.mark.parametrize("cols", [96, 1101, 9728])
+def test_silu_mul_of_subnormal_gates(hip, cols):
+    """Gates below f32's normal numbers with large ups: silu(gate) in f32 has few bits left, the product does not show it."""
+    r = np.random.default_rng(13)
+    g = (r.integers(1, 2000, (4, cols)) * 2.0**-149).astype(np.float32)
+    u = (r.standard_normal((4, cols)) * 1e37).astype(np.float32)
+    u[1], u[2] = u[1] * np.float32(1e-15), u[2] * np.float32(1e-30)
+    g[3, ::2] = r.standard_normal(g[3, ::2].shape)
+    q = hip.alloc_q8(4, cols)
+    hip.silu_mul_q8(q, buf(hip, g), buf(hip, u))
+    want_q, want_s = rows64(silu64(g, u))
+    v, s = hip.read_q8(q)
+    assert near(s, want_s) and np.array_equal(v, want_q)
 
 
 @gpu

@@ -3,10 +3,11 @@
 //
 // Of a row v with A = max |v|, the integers are those nearest to 127 v / A
 // (ties to even) and the scale is A / 127 in f32; where that rounds to zero, so
-// do the integers. The quotients are formed in
-// 64 bits, so that the integers are the definition's whatever the launch. For
-// rmsnorm, v_c = r x_c g_c with one positive r a row, which the quotients lose:
-// 127 x_c g_c / max |x g|, whose products are exact in 64 bits.
+// do the integers. The quotients are decided in 64 bits, so that the integers
+// are the definition's whatever the launch. For rmsnorm, v_c = r x_c g_c with
+// one positive r a row, which the quotients lose: 127 x_c g_c / max |x g|, whose
+// products are exact in 64 bits.
+#include <algorithm>
 #include <cfloat>
 
 #include "device_util.h"
@@ -88,7 +89,7 @@ struct SiluSource {
             load4(gate + row * cols, 4 * (threadIdx.x + T * k), cols, a[k]);
             load4(up + row * cols, 4 * (threadIdx.x + T * k), cols, b[k]);
         }
-        float least = 0;
+        float least = 0, most_up = 0;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
@@ -100,8 +101,11 @@ struct SiluSource {
                 const float e = __builtin_amdgcn_exp2f(t);
                 v[k][j] = g * __builtin_amdgcn_rcpf(1.f + fmaf(e, d * 0.693147182f, e)) * b[k][j];
                 least = fminf(least, g);
+                most_up = fmaxf(most_up, fabsf(b[k][j]));
             }
-        odd |= least < -80.f;
+        // exp(-g) past f32; or silu(g) below its normal numbers, off by 2^-150,
+        // times what makes that more than 2^-26 of the least maximum taken.
+        odd |= least < -80.f || most_up > 0x1p24f;
     }
 };
 
@@ -142,8 +146,8 @@ __device__ __forceinline__ void reduce(Reduced<W> &sh, double &most, double &sum
     }
 }
 
-// The scale of a row whose largest value is most (of the norm: times a factor),
-// and whether the row is marked instead.
+// The scale of a row whose largest value is most (the norm's: times r), or NaN,
+// with bad set, where the row is to be marked.
 template <class Source>
 __device__ __forceinline__ float scale_of(const Source &src, double most, double sum, int cols, int &bad) {
     double top = most;
@@ -154,7 +158,7 @@ __device__ __forceinline__ float scale_of(const Source &src, double most, double
 }
 
 // A row in 64 bits, read once for its maximum and again for its integers: any
-// row, by W waves.
+// row, by W waves. add: y is to be added first.
 template <class Source, int W>
 __device__ __forceinline__ void any_row(const Source &src, size_t row, int8_t *__restrict__ q,
                                         float *__restrict__ scale, int cols, int frags, bool add) {
@@ -182,10 +186,11 @@ __device__ __forceinline__ void any_row(const Source &src, size_t row, int8_t *_
     }
 }
 
+// Rows longer than registers hold, and weights (once a weight's life).
 template <class Source, int W>
 __global__ __launch_bounds__(64 * W) void any_row_kernel(Source src, int8_t *__restrict__ q, float *__restrict__ scale,
-                                                         int cols, int frags, bool add) {
-    any_row<Source, W>(src, blockIdx.x, q, scale, cols, frags, add);
+                                                         size_t row0, int cols, int frags) {
+    any_row<Source, W>(src, row0 + blockIdx.x, q, scale, cols, frags, true);
 }
 
 // Four f32 of a row, which starts at no more than 4-byte alignment.
@@ -285,22 +290,28 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // Rows of up to 256 W N columns, one block of W waves a row, N times four
 // columns a thread, held in registers, so that the row is read once.
 //
-// Bound by memory. What 64 bits decide is found in 32 first: a value's f32 is
-// off by at most Source::kOff of it and the quotient by 127 times that and four
-// roundings (the largest value's, its reciprocal's twice, the product's), so only values within twice that of the largest are compared
-// in 64 bits, and only quotients within 127 kNear of a border are formed again
-// (3 in 10000 for silu). Rows on which f32 does not hold what 64 bits do
-// (values past 1e38 or not finite, none as large as 1e-30, arguments whose
-// exponential overflows) are taken by any_row.
+// Bound by memory (norm 8192 x 2560 55.9 us, 4.9 TB/s; rows 8192 x 4096 31.3,
+// 5.4; silu 2048 x 9728 39.4, 4.6); one row by its chain of loads, maxima and
+// barriers on one CU (norm of 2560 3.5 us, silu of 9728 5.4). What 64 bits
+// decide is found in 32 first: a value's f32 is off by at most Source::kOff of
+// it, and the quotient by 127 times that and three roundings (the largest
+// value's, the factor's, the product's), so only values within twice kOff of
+// the largest are compared in 64 bits, and only quotients within 127 kNear of
+// a border are formed again (2 in 10000 for silu), from registers. With 64 bits
+// throughout and a second pass over memory the same took 90, 88 and 85 us.
+// Rows on which f32 does not hold what 64 bits do (values past 1e38 or not
+// finite, none as large as 1e-30, arguments at which silu leaves f32) are taken
+// by any_row.
 template <class Source, int W, int N>
 __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__restrict__ q, float *__restrict__ scale,
-                                                      size_t rows, int cols, int frags, bool grouped) {
+                                                      size_t row0, size_t rows, int cols, int frags,
+                                                      bool grouped) {
     constexpr int T = 64 * W;
     constexpr float kNear = Source::kOff + 5.0f / (1 << 24);
     __shared__ alignas(16) float red_max[W];
     __shared__ alignas(16) double red_sum[W];
     __shared__ alignas(16) unsigned long long red_exact[W];
-    const size_t row = row_of_block(blockIdx.x, grouped);
+    const size_t row = row0 + row_of_block(blockIdx.x, grouped);
     if (row >= rows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float v[N][4], a[N][4], b[N][4];
@@ -445,12 +456,25 @@ __global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, in
     }
 }
 
+// Rows a launch, whose threads are fewer than 2^32.
+constexpr size_t kRowsALaunch = (size_t)1 << 21;
+
 template <class Source, int W, int N>
 void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
-    const bool grouped = q.rows >= 128;
-    const size_t blocks = grouped ? (q.rows + 127) / 128 * 128 : q.rows;
-    rows_kernel<Source, W, N><<<(unsigned)blocks, 64 * W, 0, s>>>(src, q.ptr, q.scale, q.rows, (int)q.cols,
-                                                                  (int)q8_frags(q.cols), grouped);
+    for (size_t r = 0; r < q.rows; r += kRowsALaunch) {
+        const size_t rows = std::min(q.rows - r, kRowsALaunch);
+        const bool grouped = rows >= 128;
+        const size_t blocks = grouped ? (rows + 127) / 128 * 128 : rows;
+        rows_kernel<Source, W, N><<<(unsigned)blocks, 64 * W, 0, s>>>(src, q.ptr, q.scale, r, q.rows, (int)q.cols,
+                                                                      (int)q8_frags(q.cols), grouped);
+    }
+}
+
+template <class Source, int W>
+void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
+    for (size_t r = 0; r < q.rows; r += kRowsALaunch)
+        any_row_kernel<Source, W><<<(unsigned)std::min(q.rows - r, kRowsALaunch), 64 * W, 0, s>>>(
+            src, q.ptr, q.scale, r, (int)q.cols, (int)q8_frags(q.cols));
 }
 
 // Rows that fit a block's registers: eight waves a row, more loads in flight
@@ -470,9 +494,7 @@ hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     else if (c <= 6144) launch_held<Source, 8, 3>(s, q, src);
     else if (c <= 10240) launch_held<Source, 8, 5>(s, q, src);
     else if (c <= 20480) launch_held<Source, 16, 5>(s, q, src);
-    else
-        any_row_kernel<Source, 16><<<(unsigned)q.rows, 1024, 0, s>>>(src, q.ptr, q.scale, (int)q.cols,
-                                                                     (int)q8_frags(q.cols), true);
+    else launch_any<Source, 16>(s, q, src);
     return hipGetLastError();
 }
 
@@ -482,8 +504,7 @@ hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x) { r
 
 hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16_t *w) {
     if (q.rows == 0) return hipSuccess;
-    any_row_kernel<WeightSource, 4><<<(unsigned)q.rows, 256, 0, s>>>(WeightSource{w}, q.ptr, q.scale, (int)q.cols,
-                                                                     (int)q8_frags(q.cols), true);
+    launch_any<WeightSource, 4>(s, q, WeightSource{w});
     return hipGetLastError();
 }
 
