@@ -46,4 +46,22 @@ hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, 
 // splits K, the sums of the parts go to part (part_len long).
 hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len);
 
+// Four f32 at any multiple of 4 bytes: the memory path takes 16 bytes at any of
+// them, as one access where the type says so.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// Stores the first `left` of four values (all, if more are left). NT: past the
+// caches' normal order, for results larger than they are.
+template <bool NT = false>
+__device__ __forceinline__ void store4(float *o, f32x4_any v, int left) {
+    if (left >= 4) {
+        if (NT) __builtin_nontemporal_store(v, reinterpret_cast<f32x4_any *>(o));
+        else *reinterpret_cast<f32x4_any *>(o) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < left) o[i] = v[i];
+    }
+}
+
 }  // namespace th

@@ -64,22 +64,6 @@ __device__ __forceinline__ int xcd_range(int lin, int count) {
     return xcd * q + (xcd < rest ? xcd : rest) + (lin >> 3);
 }
 
-// Four values of a row of which `left` are left, at any multiple of 4 bytes
-// (rows of a number that 4 does not divide): the memory path takes 16 bytes at
-// any of them.
-__device__ __forceinline__ void store4(float *o, f32x4 v, int left) {
-    struct __attribute__((packed, aligned(4))) Loose {
-        f32x4 v;
-    };
-    if (left >= 4) {
-        reinterpret_cast<Loose *>(o)->v = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-            if (i < left) o[i] = v[i];
-    }
-}
-
 // Few tokens. A block takes RB row blocks and TB token blocks, its W waves the
 // fragments in turn (so that the block reads consecutive memory), U of them in
 // flight a wave; the waves' sums meet in LDS.
@@ -305,8 +289,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void tile_kernel(Args a, int gr, in
             const f32x4 v = *reinterpret_cast<const f32x4 *>(lines + t * T::kLine + c);
             if (t0 + j * 16 + t >= a.n || r0 + c >= a.rows) continue;
             float *o = out + (size_t)(t0 + j * 16 + t) * a.rows + r0 + c;
-            if (a.rows % 4 == 0) __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(o));
-            else store4(o, v, a.rows - r0 - c);
+            store4<true>(o, v, a.rows - r0 - c);
         }
     }
 }

@@ -24,7 +24,8 @@ __device__ __forceinline__ int nearest(double v, double most, double inv) {
     return (int)rint(t);
 }
 
-// Four values from column c of a row, zeros past its end.
+// Four values from column c of a row, which starts at any multiple of 4 bytes,
+// zeros past its end.
 __device__ __forceinline__ void load4(const float *row, int c, int cols, float (&v)[4]);
 
 // What a row is made of. value: the 64-bit value (of the norm without its
@@ -193,16 +194,15 @@ __global__ __launch_bounds__(64 * W) void any_row_kernel(Source src, int8_t *__r
     any_row<Source, W>(src, row0 + blockIdx.x, q, scale, cols, frags, true);
 }
 
-// Four f32 of a row, which starts at no more than 4-byte alignment.
-struct __attribute__((packed, aligned(4))) Loose4 {
-    float v[4];
-};
-
 __device__ __forceinline__ void load4(const float *row, int c, int cols, float (&v)[4]) {
     if (c + 4 <= cols) {
-        const Loose4 l = *reinterpret_cast<const Loose4 *>(row + c);
+        // In the caches' normal order: inputs larger than they are would gain
+        // from another (norm 8192 x 2560 48 us for 53), but what the product
+        // before has just left there is worth more (a gated MLP of 8192 tokens
+        // x 2560 x 9728 816 us, 916 with nontemporal loads).
+        const f32x4_any l = *reinterpret_cast<const f32x4_any *>(row + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = l.v[j];
+        for (int j = 0; j < 4; ++j) v[j] = l[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = c + j < cols ? row[c + j] : 0.f;
@@ -231,16 +231,9 @@ __device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], float (
     for (int k = 0; k < N; ++k) {
         const int c = 4 * (threadIdx.x + T * k);
         if (y) {
-            Loose4 l;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) l.v[j] = a[k][j] += u[k][j];
-            if (c + 4 <= cols) {
-                *reinterpret_cast<Loose4 *>(xr + c) = l;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < cols) xr[c + j] = l.v[j];
-            }
+            for (int j = 0; j < 4; ++j) a[k][j] += u[k][j];
+            store4(xr + c, f32x4_any{a[k][0], a[k][1], a[k][2], a[k][3]}, cols - c);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -424,14 +417,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(float *__restrict__ out
     for (int i = 0; i < 4; ++i) {
         if (row0 + i >= rows) return;
         float *o = out + (row0 + i) * cols + c;
-        const Loose4 l{{v[i].x * s[i], v[i].y * s[i], v[i].z * s[i], v[i].w * s[i]}};
-        if (c + 4 <= cols) {
-            *reinterpret_cast<Loose4 *>(o) = l;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c + j < cols) o[j] = l.v[j];
-        }
+        store4<true>(o, f32x4_any{v[i].x * s[i], v[i].y * s[i], v[i].z * s[i], v[i].w * s[i]}, cols - c);
     }
 }
 
@@ -477,23 +463,27 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
             src, q.ptr, q.scale, r, (int)q.cols, (int)q8_frags(q.cols));
 }
 
-// Rows that fit a block's registers: eight waves a row, more loads in flight
-// than four (us with 4 / 8 / 16 waves: silu 2048 x 9728 42 / 39 / 53, norm
-// 8192 x 2560 57 / 56 / 63, rows 8192 x 4096 34 / 31 / 42; one row: norm of
-// 2560 4.1 / 3.4 / 3.9), and one wave for short ones (norm 8192 x 128 6.7
-// where four waves take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6).
+// Rows that fit a block's registers, in the block that they fill best: up to
+// eight waves a row, with more loads in flight than four (us with 4 / 8 / 16
+// waves: silu 2048 x 9728 44 / 38 / 53, rows 8192 x 4096 33 / 31 / 42; norm
+// 8192 x 2560, which five fill, 49 / 52 / 60, five 48), and one wave for short
+// ones (norm 8192 x 128 6.7 where four waves take 14.8, 8192 x 512 11.7 / 16.1,
+// 8192 x 1024 21.0 / 19.6).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
-    const size_t c = q.cols;
-    if (c <= 256) launch_held<Source, 1, 1>(s, q, src);
-    else if (c <= 512) launch_held<Source, 1, 2>(s, q, src);
-    else if (c <= 1024) launch_held<Source, 4, 1>(s, q, src);
-    else if (c <= 2048) launch_held<Source, 8, 1>(s, q, src);
-    else if (c <= 4096) launch_held<Source, 8, 2>(s, q, src);
-    else if (c <= 6144) launch_held<Source, 8, 3>(s, q, src);
-    else if (c <= 10240) launch_held<Source, 8, 5>(s, q, src);
-    else if (c <= 20480) launch_held<Source, 16, 5>(s, q, src);
+    const size_t c = (q.cols + 255) / 256;
+    if (c <= 1) launch_held<Source, 1, 1>(s, q, src);
+    else if (c <= 2) launch_held<Source, 1, 2>(s, q, src);
+    else if (c <= 4) launch_held<Source, 4, 1>(s, q, src);
+    else if (c <= 6) launch_held<Source, 6, 1>(s, q, src);
+    else if (c <= 8) launch_held<Source, 8, 1>(s, q, src);
+    else if (c <= 10) launch_held<Source, 5, 2>(s, q, src);
+    else if (c <= 16) launch_held<Source, 8, 2>(s, q, src);
+    else if (c <= 24) launch_held<Source, 8, 3>(s, q, src);
+    else if (c <= 32) launch_held<Source, 8, 4>(s, q, src);
+    else if (c <= 40) launch_held<Source, 8, 5>(s, q, src);
+    else if (c <= 80) launch_held<Source, 16, 5>(s, q, src);
     else launch_any<Source, 16>(s, q, src);
     return hipGetLastError();
 }
