@@ -464,11 +464,15 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
 }
 
 // Rows that fit a block's registers, in the block that they fill best: up to
-// eight waves a row, with more loads in flight than four (us with 4 / 8 / 16
-// waves: silu 2048 x 9728 44 / 38 / 53, rows 8192 x 4096 33 / 31 / 42; norm
-// 8192 x 2560, which five fill, 49 / 52 / 60, five 48), and one wave for short
-// ones (norm 8192 x 128 6.7 where four waves take 14.8, 8192 x 512 11.7 / 16.1,
-// 8192 x 1024 21.0 / 19.6).
+// eight waves a row, with more loads in flight than four and more blocks a CU
+// than sixteen (us with 4 / 8 / 16 waves: silu 2048 x 9728 44 / 38 / 53, rows
+// 8192 x 4096 33 / 31 / 42; norm 8192 x 2560, which five fill, 49 / 52 / 60,
+// five 48), and one wave for short ones (norm 8192 x 128 6.7 where four waves
+// take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6). Sixteen hold
+// longer ones, with as few columns a thread as these need (silu 2048 x 12000
+// 52.7 with three times four, 63.4 with five). One row goes the same ways:
+// sixteen waves wait longer at their barriers than they save (norm of 4096
+// 3.9 with eight, 4.3; of 9728 5.4, 5.5).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
@@ -483,6 +487,8 @@ hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     else if (c <= 24) launch_held<Source, 8, 3>(s, q, src);
     else if (c <= 32) launch_held<Source, 8, 4>(s, q, src);
     else if (c <= 40) launch_held<Source, 8, 5>(s, q, src);
+    else if (c <= 48) launch_held<Source, 16, 3>(s, q, src);
+    else if (c <= 64) launch_held<Source, 16, 4>(s, q, src);
     else if (c <= 80) launch_held<Source, 16, 5>(s, q, src);
     else launch_any<Source, 16>(s, q, src);
     return hipGetLastError();
