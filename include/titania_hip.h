@@ -198,8 +198,9 @@ TH_API int th_sample(th_device *dev, const th_buffer *logits, float temperature,
  * The compute calls can be captured (th_graph_begin) at any size; alloc, free,
  * read and write are refused then. */
 typedef struct th_q8 th_q8;
-/* `rows` rows of `cols` (1 to 131071, the most whose sums of products fit 32
- * bits) zeros, of scale 0. Takes ceil(rows / 16) * ceil(cols / 128) * 2 KB. */
+/* `rows` rows (at most 2^25) of `cols` (1 to 131071, the most whose sums of
+ * products fit 32 bits) zeros, of scale 0. Takes ceil(rows / 16) *
+ * ceil(cols / 128) * 2 KB. */
 TH_API int th_q8_alloc(th_device *dev, size_t rows, size_t cols, th_q8 **out);
 TH_API void th_q8_free(th_device *dev, th_q8 *q);
 TH_API int th_q8_shape(const th_q8 *q, size_t *rows, size_t *cols);

@@ -613,9 +613,9 @@ def test_graphs_share_the_block_of_sums(hip):
 
 @gpu
 def test_allocation_that_fails_leaves_no_error(hip):
-    """64 TB are not there; the next launch does not report it."""
+    """4 TB are not there; the next launch does not report it."""
     with pytest.raises(HipError) as e:
-        hip.alloc_q8((1 << 29) + 5, 131071)
+        hip.alloc_q8(1 << 25, 131071)
     assert e.value.code == _lib.TH_ERR_NOMEM
     x = np.arange(64, dtype=np.float32)
     q = hip.alloc_q8(1, 64)
@@ -626,7 +626,8 @@ def test_allocation_that_fails_leaves_no_error(hip):
 @gpu
 def test_refusals_on_the_device(hip):
     q, x = hip.alloc_q8(2, 64), hip.alloc(128)
-    for call in (lambda: hip.alloc_q8(2, 0), lambda: hip.alloc_q8(1, 131072), lambda: hip.resize_q8(q, 3),
+    for call in (lambda: hip.alloc_q8(2, 0), lambda: hip.alloc_q8(1, 131072), lambda: hip.alloc_q8((1 << 25) + 1, 1),
+                 lambda: hip.resize_q8(q, 3),
                  lambda: hip.quantize_q8(q, hip.alloc(64)), lambda: hip.dequantize_q8(hip.alloc(64), q),
                  lambda: hip.silu_mul_q8(q, x, hip.alloc(64)), lambda: hip.matmul_q8(x, hip.alloc_q8(2, 65), q),
                  lambda: hip.add_rmsnorm_q8(x, x, q, hip.upload(Tensor((64,), np.zeros(64, np.uint16))), EPS)):
@@ -672,7 +673,8 @@ OUT = C.c_void_p()
 REFUSED = {
     "alloc: no columns": lambda l: l.th_q8_alloc(DEV, 4, 0, C.byref(OUT)),
     "alloc: sums past 32 bits": lambda l: l.th_q8_alloc(DEV, 4, 131072, C.byref(OUT)),
-    "alloc: too many rows": lambda l: l.th_q8_alloc(DEV, 1 << 62, 64, C.byref(OUT)),
+    "alloc: too many rows": lambda l: l.th_q8_alloc(DEV, (1 << 25) + 1, 64, C.byref(OUT)),
+    "alloc: rows past 64 bits": lambda l: l.th_q8_alloc(DEV, 1 << 62, 64, C.byref(OUT)),
     "alloc: no output": lambda l: l.th_q8_alloc(DEV, 4, 64, None),
     "alloc: no device": lambda l: l.th_q8_alloc(None, 4, 64, C.byref(OUT)),
     "shape: null": lambda l: l.th_q8_shape(None, None, None),

@@ -22,6 +22,8 @@ namespace th {
 
 // Sums of cols products of two 8-bit integers stay below 2^31.
 constexpr size_t kQ8MaxCols = 131071;
+// Of what fits 288 GB, every launch then has fewer than 2^32 threads.
+constexpr size_t kQ8MaxRows = (size_t)1 << 25;
 
 // Fragments of a row block: an even number, for kernels that step by 128 columns.
 constexpr size_t q8_frags(size_t cols) { return (cols + 127) / 128 * 2; }

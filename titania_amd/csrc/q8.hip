@@ -47,7 +47,7 @@ int th_q8_alloc(th_device *dev, size_t rows, size_t cols, th_q8 **out) {
     TH_REQUIRE(dev && out, "th_q8_alloc: null argument");
     TH_NOT_CAPTURING(dev, "th_q8_alloc");
     TH_REQUIRE(cols > 0 && cols <= th::kQ8MaxCols, "8-bit rows of %zu columns: 1 to %zu", cols, th::kQ8MaxCols);
-    TH_REQUIRE(rows < ((size_t)1 << 30), "%zu 8-bit rows: fewer than 2^30", rows);
+    TH_REQUIRE(rows <= th::kQ8MaxRows, "%zu 8-bit rows: at most %zu", rows, th::kQ8MaxRows);
     TH_Q8_CURRENT(dev);
     auto *q = new (std::nothrow) th_q8();
     if (!q) return fail(TH_ERR_NOMEM, "out of host memory");

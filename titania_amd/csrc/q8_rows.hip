@@ -283,9 +283,9 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // Rows of up to 256 W N columns, one block of W waves a row, N times four
 // columns a thread, held in registers, so that the row is read once.
 //
-// Bound by memory (norm 8192 x 2560 55.9 us, 4.9 TB/s; rows 8192 x 4096 31.3,
-// 5.4; silu 2048 x 9728 39.4, 4.6); one row by its chain of loads, maxima and
-// barriers on one CU (norm of 2560 3.5 us, silu of 9728 5.4). What 64 bits
+// Bound by memory (norm 8192 x 2560 52.2 us, 5.2 TB/s; rows 8192 x 4096 30.4,
+// 5.5; silu 2048 x 9728 39.3, 4.6); one row by its chain of loads, maxima and
+// barriers on one CU (norm of 2560 3.4 us, silu of 9728 5.5). What 64 bits
 // decide is found in 32 first: a value's f32 is off by at most Source::kOff of
 // it, and the quotient by 127 times that and three roundings (the largest
 // value's, the factor's, the product's), so only values within twice kOff of
@@ -398,7 +398,10 @@ __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__rest
         for (int c = 4 * threadIdx.x; c < cols; c += 4 * T) out[q8_at(row, c, frags) / 4] = make_char4(0, 0, 0, 0);
 }
 
-// A block a 16 rows x 256 columns: four rows of four columns a thread.
+// A block a 16 rows x 256 columns: four rows of four columns a thread. Stores
+// of 16 bytes past the caches' normal order (8192 x 4096 24.5 us; 46.7 with the
+// row ends' 4 and 8 bytes throughout, which the compiler makes of a packed
+// struct).
 __global__ __launch_bounds__(256) void dequantize_kernel(float *__restrict__ out, const int8_t *__restrict__ q,
                                                          const float *__restrict__ scale, size_t rows, int cols,
                                                          int frags, int parts) {
