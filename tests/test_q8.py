@@ -93,7 +93,7 @@ def near(got, want):
 
 # Columns about the 16, 64, 128 and 256 that kernels step by, and more than any holds of a row at once.
 COLS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 260, 512, 520, 1024, 1101, 1500, 2050, 2560, 4096,
-        4100, 6000, 6148, 8190, 9728, 10244, 12300, 16388, 20011, 28000, 40000, 41000, 131071]
+        4100, 5001, 6000, 6148, 8190, 9728, 10244, 12300, 16388, 20011, 20482, 24000, 28000, 28675, 33001, 40000, 41000, 131071]
 SIZES = [(3 if c < 20000 else 2, c) for c in COLS] + [(1, 2560), (1, 9728), (16, 512), (17, 512), (33, 130), (300, 96)]
 
 
@@ -233,7 +233,7 @@ def test_add_rmsnorm(hip, rows, cols, residual):
 
 
 @gpu
-@pytest.mark.parametrize("cols", [96, 1101, 2560, 12000])
+@pytest.mark.parametrize("cols", [96, 1101, 2560, 5001, 12000, 30000, 50000])
 def test_add_rmsnorm_special_rows(hip, cols):
     x = special_rows(cols)
     y = np.zeros((20, cols), np.float32)  # longer than x: the rest is not looked at
@@ -285,7 +285,7 @@ def test_silu_mul(hip, rows, cols):
 
 
 @gpu
-@pytest.mark.parametrize("cols", [96, 1101, 2560, 9728, 12000])
+@pytest.mark.parametrize("cols", [96, 1101, 2560, 5001, 9728, 12000, 30000, 50000])
 def test_silu_mul_special_rows(hip, cols):
     g = special_rows(cols)
     u = np.random.default_rng(6).standard_normal(g.shape).astype(np.float32)
@@ -306,7 +306,7 @@ def test_silu_mul_special_rows(hip, cols):
 
 
 @gpu
-@pytest.mark.parametrize("cols", [96, 1101, 9728])
+@pytest.mark.parametrize("cols", [96, 1101, 9728, 20011])
 def test_silu_mul_of_subnormal_gates(hip, cols):
     """Gates below f32's normal numbers with large ups: silu(gate) in f32 has few bits left, the product does not show it."""
     r = np.random.default_rng(13)
@@ -331,18 +331,23 @@ def test_silu_mul_of_one_buffer(hip):
 
 
 @gpu
-def test_values_next_to_borders(hip):
+@pytest.mark.parametrize("cols", [757, 1500, 2560, 4096, 5001, 6000, 8000, 9728, 12000, 16000, 20011, 24000, 28000, 32000, 40000])
+def test_values_next_to_borders(hip, cols):
     """Quotients of k + 1/2 exactly, and one f32 step to either side, with a
     largest value that 127 does not divide: 32 bits would not tell them apart."""
     top = np.float32(1.7)
     k = np.arange(-126, 126)
     mid = ((k + 0.5) * np.float64(top) / 127).astype(np.float32)
     x = np.concatenate([[top], mid, np.nextafter(mid, np.float32(9)), np.nextafter(mid, np.float32(-9))]).astype(np.float32)
+    x = np.resize(x, cols)
     b, q = buf(hip, x), hip.alloc_q8(1, x.size)
     hip.quantize_q8(q, b)
     assert np.array_equal(hip.read_q8(q)[0], rows64(x)[0])
     gain = np.full(x.size, 0x3f80, np.uint16)
     hip.add_rmsnorm_q8(b, None, q, hip.upload(Tensor((x.size,), gain)), EPS)
+    assert np.array_equal(hip.read_q8(q)[0], rows64(x)[0])
+    hip.write(b, x / 2)
+    hip.add_rmsnorm_q8(b, buf(hip, x / 2), q, hip.upload(Tensor((x.size,), gain)), EPS)
     assert np.array_equal(hip.read_q8(q)[0], rows64(x)[0])
 
 

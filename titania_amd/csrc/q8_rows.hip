@@ -29,9 +29,9 @@ __device__ __forceinline__ int nearest(double v, double most, double inv) {
 __device__ __forceinline__ void load4(const float *row, int c, int cols, float (&v)[4]);
 
 // What a row is made of. value: the 64-bit value (of the norm without its
-// factor r) at flat index i, column c. load: a thread's f32 values; kOff is how
-// far they may be off, relative to the value; a and b have what value64 makes
-// the 64-bit value of.
+// factor r) at flat index i, column c. load: a thread's f32 values, N times four
+// columns from column c0 + 4 threadIdx.x on; kOff is how far they may be off,
+// relative to the value; a and b have what value64 makes the 64-bit value of.
 struct RowsSource {
     static constexpr bool kNorm = false;
     static constexpr float kOff = 0;
@@ -39,11 +39,11 @@ struct RowsSource {
     static __device__ double value64(float a, float) { return (double)a; }
     __device__ double value(size_t i, size_t) const { return (double)x[i]; }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&)[N][4], double &,
+    __device__ void load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&)[N][4], double &,
                          int &) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            load4(x + row * cols, 4 * (threadIdx.x + T * k), cols, v[k]);
+            load4(x + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, v[k]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) a[k][j] = v[k][j];
         }
@@ -66,8 +66,8 @@ struct NormSource {
     static __device__ double value64(float a, float b) { return (double)a * (double)b; }
     __device__ double value(size_t i, size_t c) const { return value64(x[i], bf16_to_f32(g[c])); }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4], double &sum,
-                         int &odd) const;
+    __device__ void load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
+                         double &sum, int &odd) const;
 };
 
 struct SiluSource {
@@ -83,12 +83,12 @@ struct SiluSource {
     }
     __device__ double value(size_t i, size_t) const { return value64(gate[i], up[i]); }
     template <int N, int T>
-    __device__ void load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4], double &,
+    __device__ void load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4], double &,
                          int &odd) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            load4(gate + row * cols, 4 * (threadIdx.x + T * k), cols, a[k]);
-            load4(up + row * cols, 4 * (threadIdx.x + T * k), cols, b[k]);
+            load4(gate + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, a[k]);
+            load4(up + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, b[k]);
         }
         float least = 0, most_up = 0;
 #pragma unroll
@@ -210,14 +210,14 @@ __device__ __forceinline__ void load4(const float *row, int c, int cols, float (
 }
 
 template <int N, int T>
-__device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
+__device__ void NormSource::load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
                                  double &sum, int &odd) const {
     float u[N][4];
     alignas(8) uint16_t gain[N][4];
     float *xr = x + row * cols;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int c = 4 * (threadIdx.x + T * k);
+        const int c = c0 + 4 * (threadIdx.x + T * k);
         load4(xr, c, cols, a[k]);
         if (y) load4(y + row * cols, c, cols, u[k]);
         if (c + 4 <= cols) {
@@ -229,7 +229,7 @@ __device__ void NormSource::load(size_t row, int cols, float (&v)[N][4], float (
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int c = 4 * (threadIdx.x + T * k);
+        const int c = c0 + 4 * (threadIdx.x + T * k);
         if (y) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) a[k][j] += u[k][j];
@@ -280,8 +280,10 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return dpp_add_f64<0x143, 0xc>(v);
 }
 
-// Rows of up to 256 W N columns, one block of W waves a row, N times four
-// columns a thread, held in registers, so that the row is read once.
+// Rows of up to 256 W N G columns, one block of W waves a row, in G parts of N
+// times four columns a thread, whose values are held in registers, so that the
+// row is read once. Of a row in one part so is what they are formed from; of
+// one in several that is read again for the few values that need it.
 //
 // Bound by memory (norm 8192 x 2560 52.2 us, 5.2 TB/s; rows 8192 x 4096 30.4,
 // 5.5; silu 2048 x 9728 39.3, 4.6); one row by its chain of loads, maxima and
@@ -290,16 +292,16 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // it, and the quotient by 127 times that and three roundings (the largest
 // value's, the factor's, the product's), so only values within twice kOff of
 // the largest are compared in 64 bits, and only quotients within 127 kNear of
-// a border are formed again (2 in 10000 for silu), from registers. With 64 bits
+// a border are formed again (2 in 10000 for silu). With 64 bits
 // throughout and a second pass over memory the same took 90, 88 and 85 us.
 // Rows on which f32 does not hold what 64 bits do (values past 1e38 or not
 // finite, none as large as 1e-30, arguments at which silu leaves f32) are taken
 // by any_row.
-template <class Source, int W, int N>
-__global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__restrict__ q, float *__restrict__ scale,
+template <class Source, int W, int N, int G>
+__global__ __launch_bounds__(64 * W, G > 5 ? 4 : 1) void rows_kernel(Source src, int8_t *__restrict__ q, float *__restrict__ scale,
                                                       size_t row0, size_t rows, int cols, int frags,
                                                       bool grouped) {
-    constexpr int T = 64 * W;
+    constexpr int T = 64 * W, M = N * G;
     constexpr float kNear = Source::kOff + 5.0f / (1 << 24);
     __shared__ alignas(16) float red_max[W];
     __shared__ alignas(16) double red_sum[W];
@@ -307,15 +309,27 @@ __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__rest
     const size_t row = row0 + row_of_block(blockIdx.x, grouped);
     if (row >= rows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float v[N][4], a[N][4], b[N][4];
+    float v[M][4], a[N][4], b[N][4];
     double sum = 0;
     int odd = 0;
-    src.template load<N, T>(row, cols, v, a, b, sum, odd);
+    if constexpr (G == 1) {
+        src.template load<N, T>(row, 0, cols, v, a, b, sum, odd);
+    } else {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float(&part)[N][4] = *reinterpret_cast<float(*)[N][4]>(v[g * N]);
+            src.template load<N, T>(row, 4 * T * N * g, cols, part, a, b, sum, odd);
+            __builtin_amdgcn_sched_barrier(0);  // a part's inputs are gone before the next one's come
+        }
+    }
     auto column = [](int i) { return 4 * (int)(threadIdx.x + T * (i >> 2)) + (i & 3); };
-    auto value64 = [&](int i) { return Source::value64(pick(a, i), pick(b, i)); };
+    auto value64 = [&](int i) {
+        if constexpr (G == 1) return Source::value64(pick(a, i), pick(b, i));
+        else return src.value(row * cols + column(i), column(i));
+    };
     float m = 0, none = 0;  // 0 * v: NaN where v is not finite
 #pragma unroll
-    for (int k = 0; k < N; ++k)
+    for (int k = 0; k < M; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             none = fmaf(v[k][j], 0.f, none);
@@ -349,7 +363,7 @@ __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__rest
         if (own >= reach) {
             uint64_t near = 0;
 #pragma unroll
-            for (int i = 0; i < 4 * N; ++i) near |= (uint64_t)(fabsf(v[i / 4][i % 4]) >= reach) << i;
+            for (int i = 0; i < 4 * M; ++i) near |= (uint64_t)(fabsf(v[i / 4][i % 4]) >= reach) << i;
             for (; near; near &= near - 1) {
                 const double d = fabs(value64(__builtin_ctzll(near)));
                 atomicMax(&red_exact[wave], (unsigned long long)__double_as_longlong(d));
@@ -366,7 +380,7 @@ __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__rest
     constexpr float kBorder = 0.5f - 127 * kNear;
     float furthest = 0;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
+    for (int k = 0; k < M; ++k) {
         const int c = 4 * (threadIdx.x + T * k);
         if (c >= cols) break;
         int n[4];
@@ -381,7 +395,7 @@ __global__ __launch_bounds__(64 * W) void rows_kernel(Source src, int8_t *__rest
     if (furthest > kBorder) {
         uint64_t near = 0;
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i) {
+        for (int i = 0; i < 4 * M; ++i) {
             const float t = v[i / 4][i % 4] * inv32;
             near |= (uint64_t)(fabsf(t - rintf(t)) > kBorder && column(i) < cols) << i;
         }
@@ -448,14 +462,14 @@ __global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, in
 // Rows a launch, whose threads are fewer than 2^32.
 constexpr size_t kRowsALaunch = (size_t)1 << 21;
 
-template <class Source, int W, int N>
+template <class Source, int W, int N, int G = 1>
 void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
     for (size_t r = 0; r < q.rows; r += kRowsALaunch) {
         const size_t rows = std::min(q.rows - r, kRowsALaunch);
         const bool grouped = rows >= 128;
         const size_t blocks = grouped ? (rows + 127) / 128 * 128 : rows;
-        rows_kernel<Source, W, N><<<(unsigned)blocks, 64 * W, 0, s>>>(src, q.ptr, q.scale, r, q.rows, (int)q.cols,
-                                                                      (int)q8_frags(q.cols), grouped);
+        rows_kernel<Source, W, N, G><<<(unsigned)blocks, 64 * W, 0, s>>>(src, q.ptr, q.scale, r, q.rows, (int)q.cols,
+                                                                         (int)q8_frags(q.cols), grouped);
     }
 }
 
@@ -471,11 +485,13 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
 // than sixteen (us with 4 / 8 / 16 waves: silu 2048 x 9728 44 / 38 / 53, rows
 // 8192 x 4096 33 / 31 / 42; norm 8192 x 2560, which five fill, 49 / 52 / 60,
 // five 48), and one wave for short ones (norm 8192 x 128 6.7 where four waves
-// take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6). Sixteen hold
-// longer ones, with as few columns a thread as these need (silu 2048 x 12000
-// 52.7 with three times four, 63.4 with five). One row goes the same ways:
-// sixteen waves wait longer at their barriers than they save (norm of 4096
-// 3.9 with eight, 4.3; of 9728 5.4, 5.5).
+// take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6). Longer ones in
+// parts of which only the values stay (us whole / in parts: norm 2048 x 8192
+// 43.0 / 39.7, silu of it 31.7 / 30.9; silu 2048 x 12000 with sixteen waves
+// 62.6, eight in parts 46.0; 1024 x 28000 by any_row 132, in parts 58). One row
+// goes the same ways: sixteen waves wait longer at their barriers than they
+// save (norm of 4096 3.6 with eight, 4.3), and parts take their loads' time
+// one after the other (silu of 20000 8.6, with sixteen waves and no parts 7.6).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
@@ -487,12 +503,17 @@ hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     else if (c <= 8) launch_held<Source, 8, 1>(s, q, src);
     else if (c <= 10) launch_held<Source, 5, 2>(s, q, src);
     else if (c <= 16) launch_held<Source, 8, 2>(s, q, src);
+    else if (c <= 20) launch_held<Source, 5, 2, 2>(s, q, src);
     else if (c <= 24) launch_held<Source, 8, 3>(s, q, src);
-    else if (c <= 32) launch_held<Source, 8, 4>(s, q, src);
+    else if (c <= 32) launch_held<Source, 8, 2, 2>(s, q, src);
     else if (c <= 40) launch_held<Source, 8, 5>(s, q, src);
-    else if (c <= 48) launch_held<Source, 16, 3>(s, q, src);
-    else if (c <= 64) launch_held<Source, 16, 4>(s, q, src);
-    else if (c <= 80) launch_held<Source, 16, 5>(s, q, src);
+    else if (c <= 48) launch_held<Source, 8, 3, 2>(s, q, src);
+    else if (c <= 64) launch_held<Source, 8, 2, 4>(s, q, src);
+    else if (c <= 80) launch_held<Source, 8, 2, 5>(s, q, src);
+    else if (c <= 96) launch_held<Source, 8, 2, 6>(s, q, src);
+    else if (c <= 112) launch_held<Source, 8, 2, 7>(s, q, src);
+    else if (c <= 128) launch_held<Source, 16, 2, 4>(s, q, src);
+    else if (c <= 160) launch_held<Source, 16, 2, 5>(s, q, src);
     else launch_any<Source, 16>(s, q, src);
     return hipGetLastError();
 }
