@@ -492,9 +492,8 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
 // goes the same ways: sixteen waves wait longer at their barriers than they
 // save (norm of 4096 3.6 with eight, 4.3), and parts take their loads' time
 // one after the other (silu of 20000 8.6, with sixteen waves and no parts 7.6).
-// But 8193 to 10240 columns, which eight waves hold with many registers, take
-// ten while the chip holds all rows at once, two a CU (silu of 9728, us with
-// eight / ten: one row 5.9 / 5.1, 512 rows 12.5 / 12.2, 1024 20.3 / 21.3).
+// (Ten waves take silu of one row of 9728 after itself in 5.1 for eight's 5.9,
+// but a gated MLP of one token with them 33.0 for 32.3, of 300 72.1 for 71.6.)
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
@@ -509,7 +508,6 @@ hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     else if (c <= 20) launch_held<Source, 5, 2, 2>(s, q, src);
     else if (c <= 24) launch_held<Source, 8, 3>(s, q, src);
     else if (c <= 32) launch_held<Source, 8, 2, 2>(s, q, src);
-    else if (c <= 40 && q.rows <= 512) launch_held<Source, 10, 2, 2>(s, q, src);
     else if (c <= 40) launch_held<Source, 8, 5>(s, q, src);
     else if (c <= 48) launch_held<Source, 8, 3, 2>(s, q, src);
     else if (c <= 64) launch_held<Source, 8, 2, 4>(s, q, src);
