@@ -12,7 +12,8 @@
 // swizzle. Loads go through a buffer descriptor that ends with the matrix:
 // row blocks past its end read as zeros.
 #include <algorithm>
-#include <cmath>
+#include <iterator>
+#include <utility>
 
 #include "device_util.h"
 #include "q8.h"
@@ -79,7 +80,9 @@ template <int RB, int TB, int W, int U>
 __global__ __launch_bounds__(64 * W) void few_kernel(Args a) {
     __shared__ i32x4 red[W * RB * TB * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tbs = ((a.n + 15) / 16 + TB - 1) / TB, of_xcd = xcd_range(blockIdx.x, gridDim.x);
+    // (gridDim would add 0.3 us to a launch: an argument block of 256 more bytes.)
+    const int tbs = ((a.n + 15) / 16 + TB - 1) / TB, rbs = ((a.rows + 15) / 16 + RB - 1) / RB;
+    const int of_xcd = xcd_range(blockIdx.x, rbs * tbs);
     const int rb0 = of_xcd / tbs * RB, tb0 = of_xcd % tbs * TB;
     const unsigned block = (unsigned)a.frags * 1024;
     const __amdgpu_buffer_rsrc_t rw = blocks_from(a.w, a.rows, rb0, a.frags), rx = blocks_from(a.x, a.n, tb0, a.frags);
@@ -314,11 +317,12 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
     }
 }
 
-size_t blocks_of(int rows, int each) { return ((size_t)(rows + 15) / 16 + each - 1) / each; }
+unsigned ceil_div(unsigned a, unsigned b) { return (a + b - 1) / b; }
+unsigned blocks_of(int rows, unsigned each) { return ceil_div(ceil_div((unsigned)rows, 16), each); }
 
 template <int RB, int TB, int W>
 void few(hipStream_t s, const Args &a) {
-    few_kernel<RB, TB, W, 5><<<(unsigned)(blocks_of(a.rows, RB) * blocks_of(a.n, TB)), 64 * W, 0, s>>>(a);
+    few_kernel<RB, TB, W, 5><<<blocks_of(a.rows, RB) * blocks_of(a.n, TB), 64 * W, 0, s>>>(a);
 }
 
 template <class T>
@@ -337,7 +341,7 @@ void tiles(hipStream_t s, const Args &a) {
 // that they choose takes 1.02 times the fastest one's time in the geometric
 // mean, 1.42 times at most (1652 tokens x 51 x 6076; 1.18 for all others).
 constexpr double kLaunch = 2.4;
-constexpr int kCus = 256;
+constexpr unsigned kCus = 256;
 
 // The work of the CUs and the matrices' way to and from them, which mostly overlap.
 double overlapped(double work, double bytes) {
@@ -345,16 +349,25 @@ double overlapped(double work, double bytes) {
     return kLaunch + std::max(work, way) + 0.15 * std::min(work, way);
 }
 
-double weights_and_results(const Args &a) { return 1024.0 * blocks_of(a.rows, 1) * a.frags + 4.0 * a.n * a.rows; }
-double tokens(const Args &a) { return 1024.0 * blocks_of(a.n, 1) * a.frags; }
+// What the estimates look at.
+struct Shape {
+    unsigned rows, tokens, steps;       // row blocks of the weights and of the tokens, steps of 128 columns
+    double results;                     // values
+    double weights_and_results, token_bytes;
+    explicit Shape(const Args &a)
+        : rows(blocks_of(a.rows, 1)), tokens(blocks_of(a.n, 1)), steps(a.frags / 2), results((double)a.n * a.rows),
+          weights_and_results(1024.0 * rows * a.frags + 4 * results), token_bytes(1024.0 * tokens * a.frags) {}
+    size_t tiles(unsigned bm, unsigned bn) const { return (size_t)ceil_div(rows, bm) * ceil_div(tokens, bn); }
+};
 
 // Few tokens: what a CU takes in through its memory path, block after block;
 // each group of row blocks reads the tokens again, mostly from L2.
-double few_us(const Args &a, int rb, int tb) {
-    const double groups = (double)blocks_of(a.rows, rb), rounds = groups * blocks_of(a.n, tb) / kCus;
-    const double work = a.frags * (rb + tb) / 84.0 + 0.75 + 0.04 * rb * tb;
-    return overlapped((0.73 * std::ceil(rounds) + 0.27 * std::max(rounds, 1.0)) * work,
-                      weights_and_results(a) + tokens(a) * (1 + 0.11 * (groups - 1)));
+double few_us(const Shape &a, int rb, int tb) {
+    const size_t count = a.tiles(rb, tb);
+    const double groups = ceil_div(a.rows, rb), rounds = (double)count / kCus;
+    const double work = a.steps * (rb + tb) / 42.0 + 0.75 + 0.04 * rb * tb;
+    return overlapped((0.73 * ((count + kCus - 1) / kCus) + 0.27 * std::max(rounds, 1.0)) * work,
+                      a.weights_and_results + a.token_bytes * (1 + 0.11 * (groups - 1)));
 }
 
 struct TileVariant {
@@ -381,13 +394,13 @@ constexpr TileVariant kTiles[] = {
 // variant of which a CU holds two: a round of both takes 1.29 times one tile's
 // time; with one it waits for its short ring). A split's sums go out and come
 // in again.
-double tile_us(const Args &a, const TileVariant &v, int ksplit) {
-    const double count = (double)(blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn)) * ksplit;
-    const double steps = std::ceil(a.frags / 2.0 / ksplit), rounds = std::ceil(count / (kCus * v.resident));
+inline double tile_us(const Shape &a, const TileVariant &v, size_t tiles, unsigned ksplit) {
+    const size_t count = tiles * ksplit, at_once = (size_t)kCus * v.resident;
+    const double steps = ceil_div(a.steps, ksplit), rounds = (count + at_once - 1) / at_once;
     const double one = steps * (0.306 + 0.029 * v.products) + 0.6 + 0.15 * v.products;
     const double us = overlapped(rounds * one * (v.resident == 1 ? 1.0 : count > kCus ? 1.29 : 1.08),
-                                 weights_and_results(a) + tokens(a));
-    return ksplit == 1 ? us : us + 3.8 + ksplit * 8.0 * a.n * a.rows / 3.9e6;
+                                 a.weights_and_results + a.token_bytes);
+    return ksplit == 1 ? us : us + 3.8 + ksplit * 8.0 * a.results / 3.9e6;
 }
 
 struct FewVariant {
@@ -410,25 +423,37 @@ struct Choice {
     int ksplit;
 };
 
-Choice choose(const Args &a, size_t part_len) {
-    const bool is_short = a.frags <= 24;
-    if (a.n <= 16) {
-        const bool is_long = a.frags >= 128 && blocks_of(a.rows, 1) <= (size_t)kCus;
+// One instance a variant, so that their sizes are constants: the whole choice
+// takes a call about 75 ns, with a loop over the variants 210.
+template <size_t I>
+inline void consider_tile(const Shape &a, size_t part_len, Choice &best, double &least) {
+    constexpr TileVariant v = kTiles[I];
+    const size_t tiles = a.tiles(v.bm, v.bn);
+    if (const double us = tile_us(a, v, tiles, 1); us < least) least = us, best = {nullptr, &kTiles[I], 1};
+    // As many parts as fill the chip, of two steps at least.
+    if (tiles > kCus / 2) return;
+    const unsigned z = std::min({kCus / (unsigned)tiles, a.steps / 2, 16u});
+    if (z < 2 || z * a.results > (double)part_len) return;
+    if (const double us = tile_us(a, v, tiles, z); us < least) least = us, best = {nullptr, &kTiles[I], (int)z};
+}
+template <size_t... I>
+void consider_tiles(const Shape &a, size_t part_len, Choice &best, double &least, std::index_sequence<I...>) {
+    (consider_tile<I>(a, part_len, best, least), ...);
+}
+
+Choice choose(const Args &args, size_t part_len) {
+    const bool is_short = args.frags <= 24;
+    if (args.n <= 16) {
+        const bool is_long = args.frags >= 128 && blocks_of(args.rows, 1) <= kCus;
         return {&kFew[is_short ? 4 : is_long ? 6 : 0], nullptr, 1};
     }
+    const Shape a(args);
     Choice best{};
     double least = 1e30;
     for (int i = 0; i < 4; ++i)
         if (const double us = few_us(a, kFew[i].rb, kFew[i].tb); us < least)
             least = us, best = {&kFew[is_short && i < 2 ? i + 4 : i], nullptr, 1};
-    for (const TileVariant &v : kTiles) {
-        if (const double us = tile_us(a, v, 1); us < least) least = us, best = {nullptr, &v, 1};
-        // As many parts as fill the chip, of two steps at least.
-        const size_t count = blocks_of(a.rows, v.bm) * blocks_of(a.n, v.bn);
-        const int z = (int)std::min<size_t>({kCus / count, (size_t)a.frags / 4, 16});
-        if (z < 2 || (size_t)z * a.n * a.rows > part_len) continue;
-        if (const double us = tile_us(a, v, z); us < least) least = us, best = {nullptr, &v, z};
-    }
+    consider_tiles(a, part_len, best, least, std::make_index_sequence<std::size(kTiles)>());
     return best;
 }
 
