@@ -410,6 +410,57 @@ def test_matmul_of_special_scales(hip, n):
 
 
 @gpu
+def test_offsets_past_32_bits(hip):
+    """Rows of 4.4 GB, f32 values of 17.6: those behind 2^32 elements are as good as the first."""
+    rows, cols = 110000, 40000
+    look = [0, 1, 53687, 53688, 107374, 107375, rows - 1]  # about 2^31 and 2^32 values, and the last
+    r = np.random.default_rng(21)
+    aq, bq = (r.integers(-127, 128, (m, 128), dtype=np.int8) for m in (rows, cols))
+    sa, sb = (r.random(m).astype(np.float32) + np.float32(0.5) for m in (rows, cols))
+    a, b, x, one = q8(hip, aq, sa), q8(hip, bq, sb), hip.alloc(rows * cols), hip.alloc(cols)
+
+    def row(i):
+        hip.copy(one, 0, x, i * cols, cols)
+        return hip.read(one)
+
+    hip.matmul_q8(x, b, a)
+    v = product32(bq, sb, aq[look], sa[look])
+    assert np.array_equal(np.stack([row(i) for i in look]), v)
+
+    q = hip.alloc_q8(rows, cols)
+    hip.quantize_q8(q, x)
+    want_q, want_s = rows64(v)
+    for n in (3, 40, 200):  # columns of it, picked by tokens of one 1 each
+        at = r.permutation(cols)[:n]
+        at[:2] = 0, cols - 1
+        pick = np.zeros((n, cols), np.int8)
+        pick[np.arange(n), at] = 1
+        out = hip.alloc(n * rows)
+        hip.matmul_q8(out, q, q8(hip, pick, np.ones(n, np.float32)))
+        assert np.array_equal(hip.read(out).reshape(n, rows)[:, look], (want_q[:, at].astype(np.float32) * want_s[:, None]).T)
+        hip.matmul_q8(out, q8(hip, pick, np.ones(n, np.float32)), q)
+        assert np.array_equal(hip.read(out).reshape(rows, n)[look], want_q[:, at].astype(np.float32) * want_s[:, None])
+
+    gain = f32_to_bf16((1 + 0.1 * r.standard_normal(cols)).astype(np.float32))
+    for quantize, values in ((lambda: hip.silu_mul_q8(q, x, x), silu64(v, v)),
+                             (lambda: hip.add_rmsnorm_q8(x, None, q, hip.upload(Tensor((cols,), gain)), EPS), None)):
+        quantize()
+        if values is None:
+            assert np.array_equal(np.stack([row(i) for i in look]), v)
+            values, scales = norm64(v, gain)
+            want_q, scales = rows64(values, scales)
+        else:
+            want_q, scales = rows64(values)
+        assert far_from_borders(values)
+        hip.dequantize_q8(x, q)
+        got = np.stack([row(i) for i in look])
+        s = np.abs(got).max(axis=1) / np.float32(127)  # 127 is among a row's integers: two roundings, and the norm's step
+        assert np.all(np.abs(s - scales) <= 2.0**-22 * scales)
+        assert np.array_equal(np.rint(got / s[:, None]).astype(np.int8), want_q)
+        hip.matmul_q8(x, b, a)
+
+
+@gpu
 def test_rows_with_themselves(hip):
     v = np.random.default_rng(8).integers(-127, 128, (40, 200), dtype=np.int8)
     s = np.linspace(0.1, 2, 40).astype(np.float32)
