@@ -92,7 +92,7 @@ def near(got, want):
 
 
 # Columns about the 16, 64, 128 and 256 that kernels step by, and more than any holds of a row at once.
-COLS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 260, 512, 520, 1024, 1101, 1500, 2050, 2560, 4096,
+COLS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 260, 512, 520, 1024, 1101, 1500, 2000, 2050, 2560, 4096,
         4100, 5001, 6000, 6148, 8190, 9728, 10244, 12300, 16388, 20011, 20482, 24000, 28000, 28675, 33001, 40000, 41000, 131071]
 SIZES = [(3 if c < 20000 else 2, c) for c in COLS] + [(1, 2560), (1, 9728), (16, 512), (17, 512), (33, 130), (300, 96), (520, 8200)]
 
