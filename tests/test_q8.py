@@ -94,7 +94,8 @@ def near(got, want):
 # Columns about the 16, 64, 128 and 256 that kernels step by, and more than any holds of a row at once.
 COLS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 260, 512, 520, 1024, 1101, 1500, 2000, 2050, 2560, 4096,
         4100, 5001, 6000, 6148, 8190, 9728, 10244, 12300, 16388, 20011, 20482, 24000, 28000, 28675, 33001, 40000, 41000, 131071]
-SIZES = [(3 if c < 20000 else 2, c) for c in COLS] + [(1, 2560), (1, 9728), (16, 512), (17, 512), (33, 130), (300, 96), (520, 8200)]
+SIZES = [(3 if c < 20000 else 2, c) for c in COLS] + [(1, 2560), (1, 9728), (16, 512), (17, 512), (33, 130), (300, 96), (520, 8200),
+    (260, 13000), (260, 18000)]
 
 
 @gpu
@@ -319,6 +320,50 @@ def test_silu_mul_of_subnormal_gates(hip, cols):
     want_q, want_s = rows64(silu64(g, u))
     v, s = hip.read_q8(q)
     assert near(s, want_s) and np.array_equal(v, want_q)
+
+
+def repeated(hip, a, rows):
+    """A buffer of `rows` rows, those of a again and again."""
+    b, have, total = hip.alloc(rows * a.shape[1]), a.size, rows * a.shape[1]
+    first = buf(hip, a)
+    hip.copy(b, 0, first, 0, have)
+    while have < total:
+        n = min(have, total - have)
+        hip.copy(b, have, b, 0, n)
+        have += n
+    return b
+
+
+@gpu
+@pytest.mark.parametrize("cols", [200, 512, 1000, 1500, 2000, 2560, 4096, 5001, 6000, 8190, 9728, 12000, 16000, 20011, 24000, 28000,
+                                  32000, 40000, 50000])
+def test_more_than_the_caches_hold(hip, cols):
+    """Inputs of 128 MB and more are read another way."""
+    r = np.random.default_rng(cols)
+    x, y = (r.standard_normal((19, cols)).astype(np.float32) for _ in range(2))
+    gain = f32_to_bf16((1 + 0.1 * r.standard_normal(cols)).astype(np.float32))
+    rows = (1 << 25) // cols + 1
+    half = rows // 2 + 1  # of two inputs each
+
+    def check(q, v, scale64=None):
+        want_q, want_s = rows64(v, scale64)
+        got, s = hip.read_q8(q)
+        again = np.arange(len(s)) % 19
+        assert np.array_equal(got, want_q[again]) and near(s, want_s[again])
+
+    q, x0 = hip.alloc_q8(rows, cols), repeated(hip, x, rows)
+    hip.quantize_q8(q, x0)
+    check(q, x)
+    hip.add_rmsnorm_q8(x0, None, q, hip.upload(Tensor((cols,), gain)), EPS)
+    check(q, *norm64(x, gain))
+    hip.resize_q8(q, half)
+    x1, y1 = repeated(hip, x, half), repeated(hip, y, half)
+    hip.silu_mul_q8(q, x1, y1)
+    assert far_from_borders(silu64(x, y))  # the others' values are exact, ties among them
+    check(q, silu64(x, y))
+    hip.add_rmsnorm_q8(x1, y1, q, hip.upload(Tensor((cols,), gain)), EPS)
+    check(q, *norm64(x + y, gain))
+    assert np.array_equal(hip.read(x1).reshape(half, cols), (x + y)[np.arange(half) % 19])
 
 
 @gpu

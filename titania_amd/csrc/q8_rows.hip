@@ -25,15 +25,17 @@ __device__ __forceinline__ int nearest(double v, double most, double inv) {
 }
 
 // Four values from column c of a row, which starts at any multiple of 4 bytes,
-// zeros past its end.
+// zeros past its end. NT: past the caches' normal order.
+template <bool NT>
 __device__ __forceinline__ void load4(const float *row, int c, int cols, float (&v)[4]);
 
 // What a row is made of. value: the 64-bit value (of the norm without its
 // factor r) at flat index i, column c. load: a thread's f32 values, N times four
 // columns from column c0 + 4 threadIdx.x on; kOff is how far they may be off,
 // relative to the value; a and b have what value64 makes the 64-bit value of.
+template <bool NT>
 struct RowsSource {
-    static constexpr bool kNorm = false;
+    static constexpr bool kNorm = false, kNt = NT;
     static constexpr float kOff = 0;
     const float *x;
     static __device__ double value64(float a, float) { return (double)a; }
@@ -43,7 +45,7 @@ struct RowsSource {
                          int &) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            load4(x + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, v[k]);
+            load4<NT>(x + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, v[k]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) a[k][j] = v[k][j];
         }
@@ -56,8 +58,9 @@ struct WeightSource {
     __device__ double value(size_t i, size_t) const { return (double)bf16_to_f32(w[i]); }
 };
 
+template <bool NT>
 struct NormSource {
-    static constexpr bool kNorm = true;
+    static constexpr bool kNorm = true, kNt = NT;
     static constexpr float kOff = 1.0f / (1 << 24);
     float *x;
     const float *y;
@@ -70,8 +73,9 @@ struct NormSource {
                          double &sum, int &odd) const;
 };
 
+template <bool NT>
 struct SiluSource {
-    static constexpr bool kNorm = false;
+    static constexpr bool kNorm = false, kNt = NT;
     // The exponential and the reciprocal within 2^-23, the exponential's
     // correction, its product, the sum and the two products within 2^-24: 4.5
     // 2^-23 and a little for their products.
@@ -87,8 +91,8 @@ struct SiluSource {
                          int &odd) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            load4(gate + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, a[k]);
-            load4(up + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, b[k]);
+            load4<NT>(gate + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, a[k]);
+            load4<NT>(up + row * cols, c0 + 4 * (threadIdx.x + T * k), cols, b[k]);
         }
         float least = 0, most_up = 0;
 #pragma unroll
@@ -194,13 +198,11 @@ __global__ __launch_bounds__(64 * W) void any_row_kernel(Source src, int8_t *__r
     any_row<Source, W>(src, row0 + blockIdx.x, q, scale, cols, frags, true);
 }
 
+template <bool NT>
 __device__ __forceinline__ void load4(const float *row, int c, int cols, float (&v)[4]) {
     if (c + 4 <= cols) {
-        // In the caches' normal order: inputs larger than they are would gain
-        // from another (norm 8192 x 2560 48 us for 53), but what the product
-        // before has just left there is worth more (a gated MLP of 8192 tokens
-        // x 2560 x 9728 816 us, 916 with nontemporal loads).
-        const f32x4_any l = *reinterpret_cast<const f32x4_any *>(row + c);
+        const auto *at = reinterpret_cast<const f32x4_any *>(row + c);
+        const f32x4_any l = NT ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = l[j];
     } else {
@@ -209,8 +211,9 @@ __device__ __forceinline__ void load4(const float *row, int c, int cols, float (
     }
 }
 
+template <bool NT>
 template <int N, int T>
-__device__ void NormSource::load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
+__device__ void NormSource<NT>::load(size_t row, int c0, int cols, float (&v)[N][4], float (&a)[N][4], float (&b)[N][4],
                                  double &sum, int &odd) const {
     float u[N][4];
     alignas(8) uint16_t gain[N][4];
@@ -218,8 +221,8 @@ __device__ void NormSource::load(size_t row, int c0, int cols, float (&v)[N][4],
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int c = c0 + 4 * (threadIdx.x + T * k);
-        load4(xr, c, cols, a[k]);
-        if (y) load4(y + row * cols, c, cols, u[k]);
+        load4<NT>(xr, c, cols, a[k]);
+        if (y) load4<NT>(y + row * cols, c, cols, u[k]);
         if (c + 4 <= cols) {
             *reinterpret_cast<uint2 *>(gain[k]) = *reinterpret_cast<const uint2 *>(g + c);
         } else {
@@ -459,6 +462,13 @@ __global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, in
     }
 }
 
+// Inputs of half the 256 MB of the memory-side cache are read past the caches'
+// normal order (norm 8192 x 2560 from memory 53 -> 48 us; a gated MLP of 8192
+// tokens x 2560 x 9728 733 -> 695, of 4096 388 -> 376, of 2048 208 -> 205);
+// smaller ones not: they may still be there (84 MB quantized again and again
+// 16.7 us, 20.9 so read; the MLP of 64 tokens 38.2 / 38.6).
+constexpr size_t kPastCaches = (size_t)128 << 20;
+
 // Rows a launch, whose threads are fewer than 2^32.
 constexpr size_t kRowsALaunch = (size_t)1 << 21;
 
@@ -488,16 +498,23 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
 // take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6). Longer ones in
 // parts of which only the values stay (us whole / in parts: norm 2048 x 8192
 // 43.0 / 39.7, silu of it 31.7 / 30.9; silu 2048 x 12000 with sixteen waves
-// 62.6, eight in parts 46.0; 1024 x 28000 by any_row 132, in parts 58). One row
-// goes the same ways: sixteen waves wait longer at their barriers than they
-// save (norm of 4096 3.6 with eight, 4.3), and parts take their loads' time
-// one after the other (silu of 20000 8.6, with sixteen waves and no parts 7.6).
-// (Ten waves take silu of one row of 9728 after itself in 5.1 for eight's 5.9,
-// but a gated MLP of one token with them 33.0 for 32.3, of 300 72.1 for 71.6.)
+// 62.6, eight in parts 46.0; 1024 x 28000 by any_row 132, in parts 58). Rows
+// that have a CU each go the same ways (sixteen waves wait longer at their
+// barriers than they save: norm of 4096 3.6 with eight, 4.3), but for lengths
+// that eight waves hold with many registers or in many parts, whose loads come
+// one after the other: ten or sixteen waves (a gated MLP of 64 tokens, 9728
+// between, 38.2 -> 37.8; 20000, 57.4 -> 56.7; of one token 40.7 -> 39.9).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
     const size_t c = (q.cols + 255) / 256;
+    if constexpr (!Source::kNt) {
+        if (q.rows <= 256) {
+            if (c > 32 && c <= 40) return launch_held<Source, 10, 2, 2>(s, q, src), hipGetLastError();
+            if (c > 48 && c <= 64) return launch_held<Source, 16, 4>(s, q, src), hipGetLastError();
+            if (c > 64 && c <= 80) return launch_held<Source, 16, 5>(s, q, src), hipGetLastError();
+        }
+    }
     if (c <= 1) launch_held<Source, 1, 1>(s, q, src);
     else if (c <= 2) launch_held<Source, 1, 2>(s, q, src);
     else if (c <= 4) launch_held<Source, 4, 1>(s, q, src);
@@ -520,9 +537,14 @@ hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     return hipGetLastError();
 }
 
+// Whether n inputs of q's shape are read past the caches' normal order.
+bool past_caches(const th_q8 &q, size_t n) { return n * q.rows * q.cols * sizeof(float) >= kPastCaches; }
+
 }  // namespace
 
-hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x) { return launch_rows(s, q, RowsSource{x}); }
+hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x) {
+    return past_caches(q, 1) ? launch_rows(s, q, RowsSource<true>{x}) : launch_rows(s, q, RowsSource<false>{x});
+}
 
 hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16_t *w) {
     if (q.rows == 0) return hipSuccess;
@@ -531,11 +553,13 @@ hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16
 }
 
 hipError_t launch_add_rmsnorm_q8(hipStream_t s, float *x, const float *y, const th_q8 &q, const uint16_t *w, float eps) {
-    return launch_rows(s, q, NormSource{x, y, w, eps});
+    return past_caches(q, y ? 2 : 1) ? launch_rows(s, q, NormSource<true>{x, y, w, eps})
+                                     : launch_rows(s, q, NormSource<false>{x, y, w, eps});
 }
 
 hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, const float *up) {
-    return launch_rows(s, q, SiluSource{gate, up});
+    return past_caches(q, 2) ? launch_rows(s, q, SiluSource<true>{gate, up})
+                             : launch_rows(s, q, SiluSource<false>{gate, up});
 }
 
 hipError_t launch_reorder_q8(hipStream_t s, const th_q8 &q, int8_t *plain, size_t row0, size_t rows, bool in) {
