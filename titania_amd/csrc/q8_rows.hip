@@ -288,8 +288,8 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // row is read once. Of a row in one part so is what they are formed from; of
 // one in several that is read again for the few values that need it.
 //
-// Bound by memory (norm 8192 x 2560 52.2 us, 5.2 TB/s; rows 8192 x 4096 30.4,
-// 5.5; silu 2048 x 9728 39.3, 4.6); one row by its chain of loads, maxima and
+// Bound by memory (norm 8192 x 2560 48.4 us, 5.6 TB/s; rows 8192 x 4096 30.9,
+// 5.4; silu 2048 x 9728 37.8, 4.7); one row by its chain of loads, maxima and
 // barriers on one CU (norm of 2560 3.4 us, silu of 9728 5.5). What 64 bits
 // decide is found in 32 first: a value's f32 is off by at most Source::kOff of
 // it, and the quotient by 127 times that and three roundings (the largest
