@@ -32,6 +32,7 @@ struct Args {
     // A split of K (ksplit > 1): part z's sums go to part[z][n][rows].
     int *part;
     int ksplit;
+    int keep;  // results stay in the caches (tiles)
 };
 
 constexpr unsigned kMostBytes = 0x40000000u;  // a descriptor's range: more than any block's row blocks take
@@ -292,7 +293,8 @@ __global__ __launch_bounds__(64 * T::kWaves) void tile_kernel(Args a, int gr, in
             const f32x4 v = *reinterpret_cast<const f32x4 *>(lines + t * T::kLine + c);
             if (t0 + j * 16 + t >= a.n || r0 + c >= a.rows) continue;
             float *o = out + (size_t)(t0 + j * 16 + t) * a.rows + r0 + c;
-            store4<true>(o, v, a.rows - r0 - c);
+            if (a.keep) store4(o, v, a.rows - r0 - c);
+            else store4<true>(o, v, a.rows - r0 - c);
         }
     }
 }
@@ -457,13 +459,24 @@ Choice choose(const Args &args, size_t part_len) {
     return best;
 }
 
+// Results that a tile stores in the caches' normal order: those that the L2s do
+// not hold (which would write them back all at once at the kernel's end), and
+// of which two and their operands find room in the 256 MB of the memory-side
+// cache until they are read (a gated MLP of 2560 columns, us so / with
+// nontemporal stores: 1024 tokens x 9728, 40 MB each, 120 / 125; 2048 x 4096,
+// 34 MB, 108 / 111; 4096 x 4096, 67 MB, 173 / 177; but 768 x 9728, 30 MB, 98 /
+// 96; 2048 x 9728, 80 MB, 202 / 201; 8192 x 9728 702 / 695).
+constexpr size_t kKeepFrom = (size_t)32 << 20, kKeepTo = (size_t)64 << 20;
+
 }  // namespace
 
 hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len) {
     if (x.rows == 0 || w.rows == 0) return hipSuccess;
-    Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols), part, 1};
+    Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols), part, 1, 0};
     const Choice c = choose(a, part_len);
     a.ksplit = c.ksplit;
+    const size_t bytes = x.rows * w.rows * sizeof(float);
+    a.keep = c.ksplit == 1 && bytes >= kKeepFrom && bytes <= kKeepTo;
     (c.tile ? c.tile->launch : c.few->launch)(s, a);
     return hipGetLastError();
 }
