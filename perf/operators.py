@@ -11,6 +11,12 @@ even) to 127 v / max |v|, s the 32-bit max |v| / 127. Four operators:
 
 What is held in 8 bits is returned as the values it stands for. Shapes are the
 Qwen3-4B layer's, and odd ones.
+
+The framework's calls go to its device's own stream, which neither waits for
+torch's streams nor is waited for by them. What `prepare` writes with torch is
+there when it returns; a pass of the framework's calls is over, and its outputs
+may be read, once the whole device has been waited for
+(`torch.cuda.synchronize()`): an event on a torch stream does not see it.
 """
 
 from __future__ import annotations
@@ -135,6 +141,7 @@ def _view(buf, *shape) -> torch.Tensor:
 def _buffer(values: torch.Tensor):
     b = _hip().alloc(values.numel())
     _view(b, values.numel()).copy_(values.reshape(-1))
+    torch.cuda.current_stream().synchronize()  # the device's own stream does not wait for torch's
     return b
 
 
