@@ -182,6 +182,7 @@ def _view(buf, *shape) -> torch.Tensor:
 def _buffer(values: torch.Tensor):
     b = _hip().alloc(values.numel())
     _view(b, values.numel()).copy_(values.reshape(-1))
+    torch.cuda.current_stream().synchronize()  # the device's own stream does not wait for torch's
     return b
 
 

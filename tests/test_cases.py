@@ -36,15 +36,20 @@ def module(name):
         sys.path.remove(str(PERF))
 
 
-@pytest.mark.parametrize("name,kind", [("operators", "norm"), ("operators", "silu"), ("operators", "rows")])
+@pytest.mark.parametrize("name,kind", [("operators", "norm"), ("operators", "silu"), ("operators", "rows"),
+                                       ("cases", "matmul"), ("cases", "attention"), ("cases", "norm")])
 def test_prepared_buffers_are_waited_for(name, kind, monkeypatch):
     """Every copy that torch queues into a buffer has been waited for when
     prepare() returns: the framework's first call would not wait for it."""
     m, log = module(name), Log()
     inputs = tuple(torch.zeros(2, 4) for _ in range(2)) + (torch.zeros(4, dtype=torch.bfloat16),)
-    if kind == "rows":
+    if kind == "matmul":
+        inputs = torch.zeros((3, 4), dtype=torch.bfloat16), torch.zeros(2, 4)
+    elif kind == "attention":
+        inputs = torch.zeros(2, 4), torch.zeros(2, 4), torch.zeros(2, 4)
+    elif kind == "rows":
         inputs = inputs[0], None, inputs[2]
-    for f in ("_row_inputs",):
+    for f in ("_row_inputs", "_matmul_inputs", "_attention_inputs", "_norm_inputs"):
         monkeypatch.setattr(m, f, lambda case, seed: inputs, raising=False)
     monkeypatch.setattr(m, "own", True, raising=False)
     monkeypatch.setattr(m, "_hip", lambda: log)
