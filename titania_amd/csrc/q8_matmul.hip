@@ -148,6 +148,14 @@ __device__ __forceinline__ void stage_barrier() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// What this wave's lanes have done to LDS comes before what they do next. (The
+// hardware keeps a wave's LDS operations in order; this keeps the compiler to it.)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Waits until at most VM loads and no LDS reads are outstanding.
 template <int VM>
 __device__ __forceinline__ void wait_loads_and_lds() {
@@ -283,10 +291,12 @@ __global__ __launch_bounds__(64 * T::kWaves) void tile_kernel(Args a, int gr, in
     float *out = a.ksplit > 1 ? reinterpret_cast<float *>(a.part + (size_t)z * a.n * a.rows) : a.out;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
+        if (j) wave_lds_order();  // the lines have been read
 #pragma unroll
         for (int i = 0; i < FM; ++i)
             *reinterpret_cast<f32x4 *>(lines + lt * T::kLine + i * 16 + lr) =
                 a.ksplit > 1 ? __builtin_bit_cast(f32x4, acc[i][j]) : scaled(acc[i][j], xs[j], ws[i]);
+        wave_lds_order();  // other lanes read them
 #pragma unroll
         for (int q = 0; q < FM; ++q) {
             const int e = q * 64 + lane, t = e / (FM * 4), c = e % (FM * 4) * 4;
