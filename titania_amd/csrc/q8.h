@@ -22,7 +22,7 @@ namespace th {
 
 // Sums of cols products of two 8-bit integers stay below 2^31.
 constexpr size_t kQ8MaxCols = 131071;
-// Of what fits 288 GB, every launch then has fewer than 2^32 threads.
+// Of what fits 288 GB, a product's launch then has fewer than 2^32 threads.
 constexpr size_t kQ8MaxRows = (size_t)1 << 25;
 
 // Fragments of a row block: an even number, for kernels that step by 128 columns.
@@ -40,6 +40,8 @@ hipError_t launch_quantize_q8(hipStream_t s, const th_q8 &q, const float *x);
 hipError_t launch_quantize_weight_q8(hipStream_t s, const th_q8 &q, const uint16_t *w);
 // out [rows][cols] = the values that q stands for.
 hipError_t launch_dequantize_q8(hipStream_t s, float *out, const th_q8 &q);
+// The rows that one launch of it takes, a multiple of 16.
+size_t dequantize_rows_a_launch(size_t cols);
 // x += y (unless y is null), q = 8-bit rows of rmsnorm(x).
 hipError_t launch_add_rmsnorm_q8(hipStream_t s, float *x, const float *y, const th_q8 &q, const uint16_t *w, float eps);
 // q = 8-bit rows of silu(gate) * up.

@@ -469,8 +469,11 @@ __global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, in
 // 16.7 us, 20.9 so read; the MLP of 64 tokens 38.2 / 38.6).
 constexpr size_t kPastCaches = (size_t)128 << 20;
 
-// Rows a launch, whose threads are fewer than 2^32.
-constexpr size_t kRowsALaunch = (size_t)1 << 21;
+// Rows a launch of up to 1024 threads a row, and blocks of one of 256 threads a
+// block: fewer than 2^32 threads. (2^25 rows of 1793 values, which 288 GB hold,
+// would be 2^24 of those blocks.)
+constexpr size_t kRowsALaunch = (size_t)1 << 21, kBlocksALaunch = (size_t)1 << 22;
+static_assert(kRowsALaunch * 1024 < (size_t)1 << 32 && kBlocksALaunch * 256 < (size_t)1 << 32, "");
 
 template <class Source, int W, int N, int G = 1>
 void launch_held(hipStream_t s, const th_q8 &q, const Source &src) {
@@ -571,11 +574,15 @@ hipError_t launch_reorder_q8(hipStream_t s, const th_q8 &q, int8_t *plain, size_
     return hipGetLastError();
 }
 
+size_t dequantize_rows_a_launch(size_t cols) { return kBlocksALaunch / ((cols + 255) / 256) * 16; }
+
 hipError_t launch_dequantize_q8(hipStream_t s, float *out, const th_q8 &q) {
-    if (q.rows == 0) return hipSuccess;
-    const size_t parts = (q.cols + 255) / 256;
-    dequantize_kernel<<<(unsigned)(q8_blocks(q.rows) * parts), 256, 0, s>>>(out, q.ptr, q.scale, q.rows, (int)q.cols,
-                                                                            (int)q8_frags(q.cols), (int)parts);
+    const size_t parts = (q.cols + 255) / 256, most = dequantize_rows_a_launch(q.cols), frags = q8_frags(q.cols);
+    for (size_t r = 0; r < q.rows; r += most) {
+        const size_t rows = std::min(q.rows - r, most);
+        dequantize_kernel<<<(unsigned)(q8_blocks(rows) * parts), 256, 0, s>>>(
+            out + r * q.cols, q.ptr + r / 16 * frags * 1024, q.scale + r, rows, (int)q.cols, (int)frags, (int)parts);
+    }
     return hipGetLastError();
 }
 

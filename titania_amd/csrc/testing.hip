@@ -11,10 +11,12 @@
 #include <vector>
 
 #include "../../include/titania_hip_test.h"
+#include "../../include/titania_hip_test_q8.h"
 #include "common.h"
 #include "few.h"
 #include "fused.h"
 #include "gemm.h"
+#include "q8.h"
 #include "step.h"
 
 namespace {
@@ -443,6 +445,13 @@ int th_test_gemm_ragged(th_device *dev, const th_weight *w, const th_buffer *x, 
     TH_HIP(th::launch_gemm_ragged(dev->stream, x->ptr, n, cols, w->ptr, rows, out->ptr, dev->part, ksplit));
     if (ksplit > 1) TH_HIP(th::launch_splitk_sum(dev->stream, dev->part, out->ptr, n * rows, ksplit));
     TH_HIP(hipStreamSynchronize(dev->stream));
+    return TH_OK;
+}
+
+int th_test_dequantize_q8_threads(size_t rows, size_t cols, size_t *threads) {
+    TH_REQUIRE(rows <= th::kQ8MaxRows && cols > 0 && cols <= th::kQ8MaxCols && threads,
+               "th_test_dequantize_q8_threads: no 8-bit rows' size, or a null argument");
+    *threads = th::q8_blocks(std::min(rows, th::dequantize_rows_a_launch(cols))) * ((cols + 255) / 256) * 256;
     return TH_OK;
 }
 
