@@ -15,6 +15,11 @@ extern "C" {
 /* The threads of the largest launch of th_dequantize_q8. */
 TH_API int th_test_dequantize_q8_threads(size_t rows, size_t cols, size_t *threads);
 
+/* What th_matmul_q8 takes for n tokens: *variant, the few-token kernel's seven
+ * first, then the tiles' eleven, in the order of their tables, and *ksplit, the
+ * parts of K. */
+TH_API int th_test_matmul_q8_variant(size_t n, size_t rows, size_t cols, int *variant, int *ksplit);
+
 #ifdef __cplusplus
 }
 #endif

@@ -403,6 +403,7 @@ PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 17, 65), (2, 3, 127), (15, 15, 128), (16
             (4, 2560, 9728), (11, 4096, 2560), (64, 2560, 9728), (512, 1030, 2560), (1, 5, 131071), (40, 20, 131071),
             (1000, 16, 128), (3, 20000, 33), (700, 2050, 200),
             # Each variant that a product can take, whole and with K split.
+            # (Four tall tiles with K split have theirs beside the list of variants.)
             (17, 515, 2500), (17, 3001, 2500), (33, 3001, 60), (70, 3001, 60), (17, 3001, 60), (131, 3001, 60),
             (50, 1037, 16000), (131, 7001, 60), (33, 3001, 16000), (700, 7001, 60), (2000, 1037, 60),
             (70, 3001, 16000), (515, 7001, 60), (4100, 130, 9000), (700, 7001, 130), (131, 7001, 9000),

@@ -1,7 +1,10 @@
 // 8-bit rows (th_q8): their layout, and the launchers of their kernels.
 #pragma once
 
+#include <algorithm>
+
 #include "common.h"
+#include "gemm.h"
 
 // Rows of 8-bit integers with an f32 scale each. A wave's matrix-core operand
 // of 16 rows x 64 columns (a fragment) is 1 KB of consecutive memory, lane
@@ -24,6 +27,9 @@ namespace th {
 constexpr size_t kQ8MaxCols = 131071;
 // Of what fits 288 GB, a product's launch then has fewer than 2^32 threads.
 constexpr size_t kQ8MaxRows = (size_t)1 << 25;
+
+// The device's block of partials, which calls use in the stream's order.
+constexpr size_t kQ8PartBytes = std::max(kPartFloats, kAttnRoundFloats) * sizeof(float);
 
 // Fragments of a row block: an even number, for kernels that step by 128 columns.
 constexpr size_t q8_frags(size_t cols) { return (cols + 127) / 128 * 2; }
@@ -49,6 +55,9 @@ hipError_t launch_silu_mul_q8(hipStream_t s, const th_q8 &q, const float *gate, 
 // out[t * w.rows + r] = x.scale[t] w.scale[r] sum_k x[t][k] w[r][k]. Where it
 // splits K, the sums of the parts go to part (part_len long).
 hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len);
+// Which of its variants it takes (the few-token kernel's, then the tiles'), and
+// the parts of K.
+int matmul_q8_variant(size_t n, size_t rows, size_t cols, size_t part_len, int *ksplit);
 
 // Four f32 at any multiple of 4 bytes: the memory path takes 16 bytes at any of
 // them, as one access where the type says so.

@@ -3,7 +3,6 @@
 #include <new>
 
 #include "common.h"
-#include "gemm.h"
 #include "q8.h"
 
 using th::fail;
@@ -35,9 +34,6 @@ struct Current {
 
 // Bytes of the integers of `rows` rows.
 size_t value_bytes(size_t rows, size_t cols) { return th::q8_blocks(rows) * th::q8_frags(cols) * 1024; }
-
-// The device's block of partials, which calls use in the stream's order.
-constexpr size_t kPartBytes = std::max(th::kPartFloats, th::kAttnRoundFloats) * sizeof(float);
 
 }  // namespace
 
@@ -103,7 +99,7 @@ int th_q8_read(th_device *dev, const th_q8 *q, int8_t *values, float *scales) {
     TH_Q8_CURRENT(dev);
     // Through the device's block of partials, as many rows at a time as it holds.
     auto *plain = reinterpret_cast<int8_t *>(dev->part);
-    const size_t most = kPartBytes / q->cols;
+    const size_t most = th::kQ8PartBytes / q->cols;
     hipError_t e = hipSuccess;
     for (size_t r = 0; r < q->rows && e == hipSuccess; r += most) {
         const size_t n = std::min(most, q->rows - r);
@@ -126,7 +122,7 @@ int th_q8_write(th_device *dev, th_q8 *q, const int8_t *values, const float *sca
     TH_Q8_HERE(dev, q);
     TH_Q8_CURRENT(dev);
     auto *plain = reinterpret_cast<int8_t *>(dev->part);
-    const size_t most = kPartBytes / q->cols;
+    const size_t most = th::kQ8PartBytes / q->cols;
     hipError_t e = hipSuccess;
     for (size_t r = 0; r < q->rows && e == hipSuccess; r += most) {
         const size_t n = std::min(most, q->rows - r);
@@ -201,7 +197,7 @@ int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x)
     TH_Q8_HERE(dev, x);
     TH_Q8_CURRENT(dev);
     TH_HIP(th::launch_matmul_q8(dev->stream, out->ptr, *w, *x, reinterpret_cast<int *>(dev->part),
-                                kPartBytes / sizeof(int)));
+                                th::kQ8PartBytes / sizeof(int)));
     return TH_OK;
 }
 

@@ -480,6 +480,14 @@ constexpr size_t kKeepFrom = (size_t)32 << 20, kKeepTo = (size_t)64 << 20;
 
 }  // namespace
 
+int matmul_q8_variant(size_t n, size_t rows, size_t cols, size_t part_len, int *ksplit) {
+    Args a{};
+    a.n = (int)n, a.rows = (int)rows, a.frags = (int)q8_frags(cols);
+    const Choice c = choose(a, part_len);
+    *ksplit = c.ksplit;
+    return c.few ? (int)(c.few - kFew) : (int)(std::size(kFew) + (c.tile - kTiles));
+}
+
 hipError_t launch_matmul_q8(hipStream_t s, float *out, const th_q8 &w, const th_q8 &x, int *part, size_t part_len) {
     if (x.rows == 0 || w.rows == 0) return hipSuccess;
     Args a{w.ptr, x.ptr, w.scale, x.scale, out, (int)x.rows, (int)w.rows, (int)q8_frags(w.cols), part, 1, 0};

@@ -455,4 +455,12 @@ int th_test_dequantize_q8_threads(size_t rows, size_t cols, size_t *threads) {
     return TH_OK;
 }
 
+int th_test_matmul_q8_variant(size_t n, size_t rows, size_t cols, int *variant, int *ksplit) {
+    TH_REQUIRE(n > 0 && n <= th::kQ8MaxRows && rows > 0 && rows <= th::kQ8MaxRows && cols > 0 && cols <= th::kQ8MaxCols &&
+                   variant && ksplit,
+               "th_test_matmul_q8_variant: no product's size, or a null argument");
+    *variant = th::matmul_q8_variant(n, rows, cols, th::kQ8PartBytes / sizeof(int), ksplit);
+    return TH_OK;
+}
+
 }  // extern "C"
