@@ -31,11 +31,12 @@ struct th_device {
     // The device address of the no-alloc entry points' fixed array (looked up
     // once, at th_device_create, with this device current).
     void *noalloc_scratch = nullptr;
-    // Split-K partials of a matmul (th::kPartFloats) and partials of an
-    // attention split by rounds (th::kAttnRoundFloats), for the device's life:
-    // calls that allocate nothing (a matmul of fewer than 16 tokens, so that
-    // it can be captured; th_attention_noalloc) then split like any other, and
-    // an allocation costs more than most matmuls.
+    // Split-K partials of a matmul (th::kPartFloats, or of 8-bit rows) and
+    // partials of an attention split by rounds (th::kAttnRoundFloats), and what
+    // 8-bit rows pass through from and to the host, for the device's life:
+    // calls that allocate nothing (a matmul of fewer than 16 tokens, so that it
+    // can be captured; th_attention_noalloc) then split like any other, and an
+    // allocation costs more than most matmuls.
     float *part = nullptr;
     // One u32 the argmax kernels leave their result in.
     uint32_t *token_out = nullptr;

@@ -67,16 +67,21 @@ __device__ __forceinline__ int xcd_range(int lin, int count) {
 }
 
 // Few tokens. A block takes RB row blocks and TB token blocks, its W waves the
-// fragments in turn (so that the block reads consecutive memory), U of them in
-// flight a wave; the waves' sums meet in LDS.
+// fragments in turn (so that the block reads consecutive memory), U a wave in
+// each round of its loop; the waves' sums meet in LDS.
 //
-// Bound by the weights' bytes, each read once (one token x 9728 x 2560: 5.4 us
-// back to back, of which a launch is 2.4), and with more tokens by what a CU
-// takes in, about 115 KB a us (64 tokens x 2560 x 9728: 9.1 us, 608 KB a CU).
-// 16 tokens' products take a twentieth of the matrix cores' time in which HBM
-// delivers their weights, so that one token is no other case than 16. Measured
-// and not kept: K split over blocks, the last to arrive adding the parts (64
-// tokens 9.6 to 14 us).
+// What bounds it is loads in flight: the compiler puts a round's loads between
+// its products as registers come free, and each round ends with none. Of a
+// round's U (RB + TB) fragments a wave has at first 7 of 10 in flight (one row
+// block, one token block), 8 of 15 (one, two), 5 of 20 (two, two) or 6 of 30
+// (two, four). One token x 9728 x 2560, captured, takes 3.6 us where the caches
+// hold the weights (6.9 TB/s) and 7.1 where 49 such matrices take turns (3.5);
+// 151936 x 2560, which no cache holds, 63.5 (6.1); 64 tokens x 2560 x 9728 6.9
+// and 13.9. 16 tokens' products take a twentieth of the matrix cores' time in
+// which HBM delivers their weights, so that one token is no other case than 16
+// (9728 x 2560 from memory 7.1 and 7.7 us). Measured and not kept: K split over
+// blocks, the last to arrive adding the parts (64 tokens x 2560 x 9728 back to
+// back 9.1 us whole, 9.6 to 14 so).
 template <int RB, int TB, int W, int U>
 __global__ __launch_bounds__(64 * W) void few_kernel(Args a) {
     __shared__ i32x4 red[W * RB * TB * 64];
@@ -177,13 +182,17 @@ __device__ __forceinline__ void wait_loads_and_lds() {
 // 9728, us, one row ahead / two / three: 39.6 / 38.9 / 36.8; with all of a
 // step's loads and reads at its start, 8192 tokens x 2560 x 9728: 155 -> 149).
 //
-// Bound by the clock the chip holds under it (about 2.0 GHz where all CUs
-// multiply), then by LDS: 8192 tokens x 2560 x 9728 in 149 us, 2740 TOPS,
-// 62% of the cycles with a matrix instruction, 84 MB of results at the end;
-// 512 x 9728 x 2560 in 18 us, of which 2.4 the launch, 1 the first loads, 4
-// the results' 20 MB. Measured and not kept: 32 x 32 x 32 products (8192 tokens
-// 161 us; 6% faster where few CUs work), K's halves on two groups of waves
-// (512 x 9728 x 2560 18.5 us), four waves of 128 x 128 (410 us).
+// Bound by what LDS moves, at the clock that the chip holds under it: a step of
+// 160 x 128 takes 1160 cycles, 640 of them with a matrix instruction, whether 61
+// CUs work (2.3 GHz, 0.50 us) or 244 (1.85 GHz, 0.62 us), and its 112 KB of
+// reads and 36 KB of loads into LDS are 1184 at 128 bytes a cycle. 512 x 9728 x
+// 2560 takes 18 us: 20 such steps, the launch (2.4), the first loads, 20 MB of
+// results. 8192 tokens x 2560 x 9728 in 320 x 256 tiles back to back 155 us,
+// 2630 TOPS, 61% of the cycles with a matrix instruction, 84 MB of results at
+// the end. Measured and not kept (before the reads ran three rows ahead): 32 x
+// 32 x 32 products (8192 tokens 149 -> 161 us; 6% faster where few CUs work),
+// K's halves on two groups of waves (512 x 9728 x 2560 18.5 us), four waves of
+// 128 x 128 (410 us).
 template <int FM_, int FN_, int WM_, int WN_, int NS_>
 struct Tile {
     static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, NS = NS_, BM = FM * WM, BN = FN * WN;
@@ -348,10 +357,12 @@ void tiles(hipStream_t s, const Args &a) {
 }
 
 // About how long a launch takes, in us, from its shape alone. The constants
-// are fitted to back-to-back launches of every variant over 17 matrices (7 x
-// 3000 to 4096 x 16384) and 6 to 14 counts of tokens (20 to 8192): the variant
-// that they choose takes 1.02 times the fastest one's time in the geometric
-// mean, 1.42 times at most (1652 tokens x 51 x 6076; 1.18 for all others).
+// are fitted to back-to-back launches of every variant. Over 17 matrices (7 x
+// 3000 to 16384 x 2048) and up to 15 counts of tokens (20 to 8192), 254 products,
+// the variant that they choose takes 1.02 times the fastest one's time in the
+// geometric mean and 1.64 times at most (2048 tokens x 51 x 6076 9.6 us for 5.9;
+// 1500 x 300 x 16000 30.7 for 21.0, 1024 x 1024 x 9728 25.3 for 18.3, all others
+// within 1.31).
 constexpr double kLaunch = 2.4;
 constexpr unsigned kCus = 256;
 
@@ -472,10 +483,12 @@ Choice choose(const Args &args, size_t part_len) {
 // Results that a tile stores in the caches' normal order: those that the L2s do
 // not hold (which would write them back all at once at the kernel's end), and
 // of which two and their operands find room in the 256 MB of the memory-side
-// cache until they are read (a gated MLP of 2560 columns, us so / with
-// nontemporal stores: 1024 tokens x 9728, 40 MB each, 120 / 125; 2048 x 4096,
-// 34 MB, 108 / 111; 4096 x 4096, 67 MB, 173 / 177; but 768 x 9728, 30 MB, 98 /
-// 96; 2048 x 9728, 80 MB, 202 / 201; 8192 x 9728 702 / 695).
+// cache until they are read. (Three gated MLPs of 2560 columns in turn, us each
+// so / with nontemporal stores. 9728 between, results of 23.8 MB 94.6 / 93.4,
+// 31.5 119.5 / 121.8, 33.4 120.7 / 122.9, 38.0 128.0 / 131.4, 48.2 151.8 /
+// 154.5, 55.7 161.6 / 167.9, 63.1 182.3 / 187.0, 66.8 192.2 / 192.3, 76.0 206.6 /
+// 204.3; 4096 between, 28.1 101.5 / 100.9, 32.0 107.7 / 111.8, 46.9 147.2 /
+// 153.4, 62.5 175.3 / 180.6, 65.6 194.1 / 193.5, 78.1 239.0 / 235.5.)
 constexpr size_t kKeepFrom = (size_t)32 << 20, kKeepTo = (size_t)64 << 20;
 
 }  // namespace

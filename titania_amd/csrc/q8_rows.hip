@@ -78,7 +78,8 @@ struct SiluSource {
     static constexpr bool kNorm = false, kNt = NT;
     // The exponential and the reciprocal within 2^-23, the exponential's
     // correction, its product, the sum and the two products within 2^-24: 4.5
-    // 2^-23 and a little for their products.
+    // 2^-23 and a little for their products. (silu alone, over every f32 gate
+    // from -80 up: 2.13 2^-23 at most, where this allows 4.)
     static constexpr float kOff = 5.0f / (1 << 23);
     const float *gate, *up;
     static __device__ double value64(float a, float b) {
@@ -466,7 +467,12 @@ __global__ __launch_bounds__(256) void reorder_kernel(int8_t *__restrict__ q, in
 // normal order (norm 8192 x 2560 from memory 53 -> 48 us; a gated MLP of 8192
 // tokens x 2560 x 9728 733 -> 695, of 4096 388 -> 376, of 2048 208 -> 205);
 // smaller ones not: they may still be there (84 MB quantized again and again
-// 16.7 us, 20.9 so read; the MLP of 64 tokens 38.2 / 38.6).
+// 16.7 us, 20.7 so read). At the limit (us in the normal order / past it): from
+// memory norm of 98 MB 34.7 / 32.4, 117 40.1 / 37.3, 128 42.9 / 40.3, silu of
+// 128 33.8 / 33.1; again and again, norm 28.3 / 32.4, 32.8 / 37.3, 35.4 / 40.2,
+// silu 28.9 / 31.5; three MLPs in turn, of which the silu reads 111 MB 162.7 /
+// 162.5, 126 182.3 / 183.4, 134 195.2 / 191.9, 152 207.6 / 204.8. Rows alone
+// gain nothing by it (129 MB 31.9 / 33.2 from memory, 24.6 / 32.6 again).
 constexpr size_t kPastCaches = (size_t)128 << 20;
 
 // Rows a launch of up to 1024 threads a row, and blocks of one of 256 threads a
@@ -501,12 +507,27 @@ void launch_any(hipStream_t s, const th_q8 &q, const Source &src) {
 // take 14.8, 8192 x 512 11.7 / 16.1, 8192 x 1024 21.0 / 19.6). Longer ones in
 // parts of which only the values stay (us whole / in parts: norm 2048 x 8192
 // 43.0 / 39.7, silu of it 31.7 / 30.9; silu 2048 x 12000 with sixteen waves
-// 62.6, eight in parts 46.0; 1024 x 28000 by any_row 132, in parts 58). Rows
-// that have a CU each go the same ways (sixteen waves wait longer at their
-// barriers than they save: norm of 4096 3.6 with eight, 4.3), but for lengths
-// that eight waves hold with many registers or in many parts, whose loads come
-// one after the other: ten or sixteen waves (a gated MLP of 64 tokens, 9728
-// between, 38.2 -> 37.8; 20000, 57.4 -> 56.7; of one token 40.7 -> 39.9).
+// 62.6, eight in parts 46.0; 1024 x 28000 by any_row 132, in parts 58).
+//
+// Each of the others against the next longer rows' block (us of the norm, and
+// of silu, of 1024 rows; of 64 where it says so): <6, 1> 1536 columns 5.6 / 6.4,
+// 6.0 / 6.5; <5, 2, 2> 5120 8.4 / 9.7, 11.7 / 13.2; <8, 3> 6144 of 64 rows 5.1 /
+// 5.6, 5.7 / 6.1 (1024 rows 10.2 / 10.5, 13.8 both); <8, 3, 2> 12288 16.6 /
+// 19.2, 24.2 / 26.2; <8, 2, 6> 24576 29.2 / 31.0, 48.2 / 49.9; <8, 2, 7> 28672
+// 33.4 / 43.2, 56.3 / 66.3; <16, 2, 4> 32768 51.1 / 54.7, 71.8 / 77.5; <16, 2,
+// 5> 40960 against any_row 61.8 / 86.1, 89.6 / 187. <8, 1> 2048 of 64 rows 4.05
+// / 4.26, 4.2 / 4.5, but of 1024 rows 6.5 / 5.9, 7.0 / 6.9 with <5, 2>.
+//
+// Rows that have a CU each (up to 256) go the same ways (sixteen waves wait
+// longer at their barriers than they save: norm of 4096 3.6 with eight, 4.3),
+// but for 8193 to 10240 columns and 12289 to 20480: ten or sixteen waves take
+// 1.05 to 1.2 times less for rows and 1.03 to 1.13 for silu, and the norm is up to 7%
+// either way (64 rows, us eight waves / so: of 9728 4.2 / 3.9, silu 6.9 / 6.4,
+// norm 5.9 both; of 20000 6.2 / 5.5, 10.2 / 9.5, 8.5 both; one row of 9728 2.75
+// / 2.80, 4.7 / 4.9, 4.4 / 4.75). In a gated MLP of 1 to 128 tokens that is 0.1
+// to 0.8 us a layer, with its weights from the caches or from memory (64 tokens
+// of eight layers in turn, 9728 between, 51.1 / 50.6; 14336, 59.8 / 59.0; 20000,
+// 70.4 / 69.6).
 template <class Source>
 hipError_t launch_rows(hipStream_t s, const th_q8 &q, const Source &src) {
     if (q.rows == 0) return hipSuccess;
