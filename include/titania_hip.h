@@ -119,7 +119,7 @@ TH_API int th_timer_end(th_device *dev, float *ms);
  * extension of the Device boundary). th_graph_begin starts capturing the
  * stream in thread-local mode: the compute calls that follow (copy, matmul of
  * fewer than 16 tokens, add, rmsnorm, rope, attention, silu_mul, the fused
- * extensions) are recorded, not run. th_graph_end stops the capture and
+ * extensions, the paged append and attention) are recorded, not run. th_graph_end stops the capture and
  * instantiates it; th_graph_launch queues one replay on the stream, reading
  * and writing the buffers named at capture time. While capturing, the calls
  * that allocate, move data to or from the host, wait or free (upload, alloc,
@@ -230,6 +230,94 @@ TH_API int th_silu_mul_q8(th_device *dev, th_q8 *q, const th_buffer *gate, const
  * rows, the sum exact, converted to f32 and multiplied by x.s[t], then w.s[r].
  * w.cols == x.cols, out.len == x.rows * w.rows. */
 TH_API int th_matmul_q8(th_device *dev, th_buffer *out, const th_q8 *w, const th_q8 *x);
+
+/* ---- paged caches (no counterpart in model/device.rs) ---- */
+
+/* The keys and values of one layer for many sequences: `pages` pages of
+ * `page_len` positions, which sequences take in any order. Position p of a
+ * sequence is row p % page_len of its page p / page_len. With a step's batch
+ * (th_batch) below, a layer's attention block (model/model.rs:108-130) for
+ * several sequences, or for tokens drafted ahead, is th_matmul x 3,
+ * th_paged_append, th_paged_attention. */
+typedef struct th_paged th_paged;
+/* Zeroed pages. page_len: 16, 32, 64, 128 or 256; pages * page_len < 2^31;
+ * n_kv_heads: 1 to 1024; head_dim: 64, 128 or 256; kv_dtype: TH_KV_F32 or
+ * TH_KV_BF16 (keys and values rounded to the nearest, ties to even). Takes
+ * pages * page_len * n_kv_heads * head_dim * 2 values. */
+TH_API int th_paged_alloc(th_device *dev, size_t pages, size_t page_len, size_t n_kv_heads, size_t head_dim, int kv_dtype,
+                          th_paged **out);
+TH_API void th_paged_free(th_device *dev, th_paged *cache);
+TH_API int th_paged_shape(const th_paged *cache, size_t *pages, size_t *page_len, size_t *n_kv_heads, size_t *head_dim,
+                          int *kv_dtype);
+/* Copies one page out, or in (blocking): keys and values, each
+ * [page_len][n_kv_heads][head_dim] in f32. */
+TH_API int th_paged_read(th_device *dev, const th_paged *cache, size_t page, float *k, float *v);
+TH_API int th_paged_write(th_device *dev, th_paged *cache, size_t page, const float *k, const float *v);
+
+/* A step's sequences and their new tokens, for the calls of all layers (whose
+ * caches have one shape). A token's activations lie at its place in the batch:
+ * first the tokens of sequence 0, then those of sequence 1, and so on. */
+typedef struct th_batch th_batch;
+/* Room for max_seqs sequences (at most 65536) with max_tokens new tokens in
+ * all (max_tokens * n_heads <= 2^24) and max_pages entries of pages (at most
+ * 2^26), over caches of the shape of `cache`; n_heads: query heads, 1 to 16 for
+ * each KV head. Nothing is set. A batch belongs to `dev`: calls with another
+ * device refuse it. */
+TH_API int th_batch_alloc(th_device *dev, const th_paged *cache, size_t n_heads, size_t max_seqs, size_t max_tokens,
+                          size_t max_pages, th_batch **out);
+TH_API void th_batch_free(th_device *dev, th_batch *batch);
+/* Once a step: sequence s has context[s] positions in the caches and n_new[s]
+ * new tokens (possibly none) behind them. `pages`: the pages of sequence 0, of
+ * sequence 1, ..., ceil((context[s] + n_new[s]) / page_len) each, n_pages in
+ * all. Sequences may share pages of their contexts; a page that gets new rows
+ * may be nobody else's. parents: NULL, or for each token the one of its own
+ * sequence that it follows, by its place there, lower than its own, or -1 for
+ * the context. Tokens that each follow the one before (always so with NULL)
+ * are a chain; other sequences are trees, of at most 256 tokens. Token i is
+ * written to position context[s] + i; it is rotated by context[s] plus its
+ * depth, i in a chain, and sees the context, itself and what it follows, up to
+ * the root. The arrays are copied before the call returns, to the device in
+ * its stream's order; a failed call changes nothing.
+ *
+ * Captured calls (th_graph_begin) read what is set when they run, so that one
+ * graph serves any step: from then on th_batch_set refuses more tokens than
+ * were set at the capture. Rows of activations behind the last token stay as
+ * they are. */
+TH_API int th_batch_set(th_device *dev, th_batch *batch, size_t n_seqs, const uint32_t *context, const uint32_t *n_new,
+                        const uint32_t *pages, size_t n_pages, const int32_t *parents);
+/* For each token of the batch: q_out = q RMSNorm'd per head by q_norm and
+ * rotated with the rope table; k, RMSNorm'd by k_norm and rotated, and v to
+ * their rows of the cache. Either norm may be NULL. q and q_out (which may be
+ * q) hold n_heads * head_dim activations a token, k and v n_kv_heads *
+ * head_dim. Equals rmsnorm x 2, rope x 2 and copy x 2 (model/model.rs:111-120)
+ * within rounding. */
+TH_API int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q, const th_buffer *k, const th_buffer *v,
+                           const th_weight *q_norm, const th_weight *k_norm, const th_buffer *rope, th_paged *cache,
+                           const th_batch *batch, float eps);
+/* For each token of the batch: attention of its n_heads queries over what it
+ * sees, whose rows th_paged_append has written (th_attention over a paged
+ * cache; a sequence alone and in a chain gives its result within rounding).
+ * What a token does not see does not reach its result, NaN and infinities
+ * included. */
+TH_API int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const th_paged *cache,
+                              const th_batch *batch);
+/* The greedy verification of drafted tokens. logits: a row for each token of
+ * the batch; tokens: the tokens themselves. picks[t] is the index of the
+ * largest logit of row t, as th_argmax finds it. Of sequence s the first
+ * token is kept, and then, as long as there is one, the first token that
+ * follows the last one kept and is what that one picked: n_kept[s] in all,
+ * their places in the sequence from kept[first token of s] on, -1 behind them.
+ * picks and kept have an element for each token of the batch. The pick of the
+ * last one kept is the next token. Blocking, and refused while capturing. */
+TH_API int th_batch_accept(th_device *dev, const th_batch *batch, const th_buffer *logits, const uint32_t *tokens,
+                           uint32_t *picks, uint32_t *n_kept, int32_t *kept);
+/* The keys and values of the tokens kept (rising places, as th_batch_accept
+ * gives them, or any other verification), moved up behind the context in each
+ * of the caches, different ones of one type: that of the j-th goes from
+ * position context[s] + kept[..] to context[s] + j. The context of the next
+ * step is then context[s] + n_kept[s]. Refused while capturing. */
+TH_API int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, const th_batch *batch,
+                         const uint32_t *n_kept, const int32_t *kept);
 
 /* ---- the forward pass (model/model.rs) ---- */
 

@@ -96,6 +96,18 @@ SIGNATURES: dict[str, tuple] = {
     "th_add_rmsnorm_q8": (_I, [_P, _P, _P, _P, _P, C.c_float]),
     "th_silu_mul_q8": (_I, [_P, _P, _P, _P]),
     "th_matmul_q8": (_I, [_P, _P, _P, _P]),
+    "th_paged_alloc": (_I, [_P, _SZ, _SZ, _SZ, _SZ, _I, C.POINTER(_P)]),
+    "th_paged_free": (None, [_P, _P]),
+    "th_paged_shape": (_I, [_P, *[C.POINTER(_SZ)] * 4, C.POINTER(_I)]),
+    "th_paged_read": (_I, [_P, _P, _SZ, _P, _P]),
+    "th_paged_write": (_I, [_P, _P, _SZ, _P, _P]),
+    "th_batch_alloc": (_I, [_P, _P, _SZ, _SZ, _SZ, _SZ, C.POINTER(_P)]),
+    "th_batch_free": (None, [_P, _P]),
+    "th_batch_set": (_I, [_P, _P, _SZ, _P, _P, _P, _SZ, _P]),
+    "th_paged_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_float]),
+    "th_paged_attention": (_I, [_P, _P, _P, _P, _P]),
+    "th_batch_accept": (_I, [_P, _P, _P, _P, _P, _P, _P]),
+    "th_paged_keep": (_I, [_P, _P, _SZ, _P, _P, _P]),
     "th_model_create": (_I, [_P, C.POINTER(ThConfig), C.POINTER(_P), _SZ, C.POINTER(_P)]),
     "th_model_destroy": (None, [_P]),
     "th_config_load": (_I, [C.c_char_p, C.POINTER(ThConfig)]),

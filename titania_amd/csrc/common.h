@@ -83,6 +83,22 @@ int read_back(th_device *dev, const float *src, size_t len, float *out, const un
 // Makes sure the device scratch holds at least `bytes`; returns its pointer or null.
 void *scratch(th_device *dev, size_t bytes);
 
+// The device made current, as allocations and launches want it, for a call.
+struct Current {
+    int before = 0;
+    bool changed = false;
+    hipError_t error;
+    explicit Current(const th_device *dev) : error(hipGetDevice(&before)) {
+        if (error == hipSuccess && before != dev->ordinal) {
+            error = hipSetDevice(dev->ordinal);
+            changed = error == hipSuccess;
+        }
+    }
+    ~Current() {
+        if (changed) (void)hipSetDevice(before);
+    }
+};
+
 // The fixed array of the no-alloc entry points: its size, and its address on
 // the current device.
 size_t noalloc_scratch_bytes();

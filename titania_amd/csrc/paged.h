@@ -1,0 +1,101 @@
+// Paged caches (th_paged) and the batches that use them (th_batch): their
+// layout in memory, and the launchers of their kernels.
+#pragma once
+
+#include "common.h"
+
+// One layer's keys and values of many sequences, in pages of `page_len`
+// positions: [page][keys, values][kv head][row][head_dim], f32 or bf16, so that
+// what an attention of one KV head reads of a page is consecutive memory.
+struct th_paged {
+    void *ptr = nullptr;
+    size_t pages = 0, page_len = 0, n_kv_heads = 0, head_dim = 0;
+    int kv_dtype = TH_KV_F32;
+    int ordinal = 0;  // the GPU that holds it
+};
+
+namespace th {
+
+constexpr size_t kTreeTokens = 256;  // drafted tokens of one sequence's tree
+constexpr int kTreeWords = (int)kTreeTokens / 64;
+constexpr size_t kPagedMaxGroup = 16;  // query heads per KV head
+
+// What the kernels read of a batch. A token: the row of the cache that it is
+// written to (page * page_len + row), the position of its rotation, its
+// sequence and its place among that sequence's tokens.
+struct TokenAt {
+    uint32_t slot, pos, seq, index;
+};
+// A sequence: its first token, its tokens, the positions before them, where
+// its pages begin in the list of pages, and whether its tokens form a tree
+// (they see what `tree` says) or a chain.
+struct SeqAt {
+    uint32_t token0, n_new, context, page0, is_tree;
+};
+// The counts that a captured launch, whose grid is fixed, reads.
+struct BatchHead {
+    uint32_t n_seqs, n_tokens;
+};
+// A batch's arrays in device memory.
+struct BatchView {
+    const BatchHead *head;
+    const SeqAt *seqs;
+    const TokenAt *tokens;
+    const uint32_t *pages;
+    const uint64_t *tree;  // [token][kTreeWords]: which of its sequence's tokens it sees
+    int page_shift;
+};
+
+// q_out = q normalized and rotated; keys (normalized and rotated) and values to
+// the cache. `n` tokens are launched for, those of the head are done.
+struct PagedAppendArgs {
+    BatchView b;
+    float *q_out;
+    const float *q, *k, *v;
+    const uint16_t *q_norm, *k_norm;  // may be null
+    const float *rope;
+    void *cache;
+    int n_heads, n_kv_heads;
+    float eps;
+};
+hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs &a, size_t n, size_t head_dim, bool bf16);
+
+struct PagedAttnArgs {
+    BatchView b;
+    float *out;
+    const float *q;
+    const void *cache;
+    int n_heads, n_kv_heads, group;
+    float scale;
+};
+hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, size_t n, size_t head_dim, bool bf16);
+
+// picks[row * splits + split] = the packed argmax of a part of a row.
+hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, int splits, uint64_t *picks);
+
+// Rows to move in every layer's cache, as kernel arguments: of segment i (a
+// sequence) moves [start[i], start[i + 1]), in order.
+struct PagedMove {
+    uint32_t from, to;
+};
+constexpr int kMoves = 256, kMoveSegments = 64, kMoveLayers = 64;
+struct PagedMoves {
+    int n_segments, n_layers;
+    int page_shift, n_kv_heads, row_bytes;  // row_bytes: of one head's row
+    uint32_t start[kMoveSegments + 1];
+    PagedMove move[kMoves];
+    void *cache[kMoveLayers];
+};
+static_assert(sizeof(PagedMoves) <= 4096, "kernel arguments");
+hipError_t launch_paged_moves(hipStream_t s, const PagedMoves &m);
+
+// Copies of up to six arrays from pinned host memory in one launch (16-byte
+// units; the addresses are multiples of 16).
+struct Upload {
+    const void *from[6];
+    void *to[6];
+    uint32_t units[6];
+};
+hipError_t launch_upload(hipStream_t s, const Upload &u);
+
+}  // namespace th

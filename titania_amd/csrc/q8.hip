@@ -13,23 +13,8 @@ namespace {
 #define TH_Q8_HERE(dev, q) \
     TH_REQUIRE((q)->ordinal == (dev)->ordinal, "8-bit rows of GPU %d on GPU %d", (q)->ordinal, (dev)->ordinal)
 
-// The device made current, as allocations and launches want it, for a call.
-struct Current {
-    int before = 0;
-    bool changed = false;
-    hipError_t error;
-    explicit Current(const th_device *dev) : error(hipGetDevice(&before)) {
-        if (error == hipSuccess && before != dev->ordinal) {
-            error = hipSetDevice(dev->ordinal);
-            changed = error == hipSuccess;
-        }
-    }
-    ~Current() {
-        if (changed) (void)hipSetDevice(before);
-    }
-};
-#define TH_Q8_CURRENT(dev)   \
-    Current current_(dev);   \
+#define TH_Q8_CURRENT(dev)     \
+    th::Current current_(dev); \
     TH_HIP(current_.error)
 
 // Bytes of the integers of `rows` rows.

@@ -130,6 +130,67 @@ class Q8:
             pass
 
 
+class Paged:
+    """One layer's keys and values in pages in device memory (th_paged)."""
+
+    def __init__(self, dev: "Hip", handle: int):
+        self._dev = dev
+        self.handle = handle
+
+    @property
+    def shape(self) -> tuple:
+        """(pages, page_len, n_kv_heads, head_dim, kv_dtype)"""
+        n, kv = [C.c_size_t() for _ in range(4)], C.c_int()
+        check(lib().th_paged_shape(self.handle, *map(C.byref, n), C.byref(kv)))
+        return (*(int(x.value) for x in n), int(kv.value))
+
+    def free(self) -> None:
+        if self.handle:
+            self._dev._refuse_while_capturing("free a paged cache")
+            lib().th_paged_free(self._dev.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self._dev.handle:
+                self.free()
+        except Exception:
+            pass
+
+
+class Batch:
+    """A step's sequences and their new tokens (th_batch): n_seqs and n_tokens of what is set."""
+
+    def __init__(self, dev: "Hip", handle: int):
+        self._dev = dev
+        self.handle = handle
+        self.n_seqs = self.n_tokens = 0
+
+    def free(self) -> None:
+        if self.handle:
+            self._dev._refuse_while_capturing("free a batch")
+            lib().th_batch_free(self._dev.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self._dev.handle:
+                self.free()
+        except Exception:
+            pass
+
+
+def _ints(a, dtype) -> np.ndarray:
+    """Whole numbers as `dtype`, those that it does not hold refused."""
+    a = np.asarray(a)
+    if a.size and not np.issubdtype(a.dtype, np.integer):
+        raise TypeError(f"whole numbers, not {a.dtype}")
+    info = np.iinfo(dtype)
+    if a.size and (int(a.min()) < info.min or int(a.max()) > info.max):
+        raise ValueError(f"numbers past {np.dtype(dtype).name}")
+    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32).reshape(-1)
 
@@ -314,6 +375,83 @@ class Hip:
         """matmul() over 8-bit rows: sums of integer products, times both scales."""
         check(lib().th_matmul_q8(self.handle, out.handle, w.handle, x.handle))
 
+    # ---- paged caches ----
+
+    def alloc_paged(self, pages: int, page_len: int, n_kv_heads: int, head_dim: int,
+                    kv_dtype: int = _lib.TH_KV_F32) -> Paged:
+        """A layer's cache of zeroed pages of page_len positions."""
+        out = C.c_void_p()
+        check(lib().th_paged_alloc(self.handle, int(pages), int(page_len), int(n_kv_heads), int(head_dim), int(kv_dtype),
+                                   C.byref(out)))
+        return Paged(self, out.value)
+
+    def read_paged(self, cache: Paged, page: int) -> tuple[np.ndarray, np.ndarray]:
+        """A page's keys and values [page_len, n_kv_heads, head_dim]."""
+        k, v = (np.empty(cache.shape[1:4], dtype=np.float32) for _ in range(2))
+        check(lib().th_paged_read(self.handle, cache.handle, int(page), k.ctypes.data, v.ctypes.data))
+        return k, v
+
+    def write_paged(self, cache: Paged, page: int, k, v) -> None:
+        k, v = _f32(k), _f32(v)
+        if not k.size == v.size == int(np.prod(cache.shape[1:4])):
+            raise ValueError(f"{k.size} keys and {v.size} values for a page of shape {cache.shape[1:4]}")
+        check(lib().th_paged_write(self.handle, cache.handle, int(page), k.ctypes.data, v.ctypes.data))
+
+    def alloc_batch(self, cache: Paged, n_heads: int, max_seqs: int, max_tokens: int, max_pages: int) -> Batch:
+        """Room for a step's sequences, new tokens and pages, over caches of this one's shape."""
+        out = C.c_void_p()
+        check(lib().th_batch_alloc(self.handle, cache.handle, int(n_heads), int(max_seqs), int(max_tokens),
+                                   int(max_pages), C.byref(out)))
+        return Batch(self, out.value)
+
+    def set_batch(self, batch: Batch, context, new, pages, parents=None) -> None:
+        """Once a step: sequence s has context[s] positions in the caches and
+        new[s] tokens behind them, in its pages (those of all sequences one
+        after another); parents: of each token the one of its sequence that it
+        follows, -1 for the context (None: each follows the one before)."""
+        c, n, p = _ints(context, np.uint32), _ints(new, np.uint32), _ints(pages, np.uint32)
+        if c.size != n.size:
+            raise ValueError(f"{c.size} contexts of {n.size} sequences")
+        t = None if parents is None else _ints(parents, np.int32)
+        tokens = int(n.sum(dtype=np.int64))
+        if t is not None and t.size != tokens:
+            raise ValueError(f"{t.size} parents of {tokens} tokens")
+        check(lib().th_batch_set(self.handle, batch.handle, n.size, c.ctypes.data, n.ctypes.data, p.ctypes.data, p.size,
+                                 None if t is None else t.ctypes.data))
+        batch.n_seqs, batch.n_tokens = n.size, tokens
+
+    def paged_append(self, q_out: Buffer, q: Buffer, k: Buffer, v: Buffer, q_norm: Weight | None, k_norm: Weight | None,
+                     rope: Buffer, cache: Paged, batch: Batch, eps: float) -> None:
+        """q_out = q, normed and rotated; k, normed and rotated, and v to the batch's rows of the cache."""
+        check(lib().th_paged_append(self.handle, q_out.handle, q.handle, k.handle, v.handle,
+                                    q_norm.handle if q_norm is not None else None,
+                                    k_norm.handle if k_norm is not None else None, rope.handle, cache.handle,
+                                    batch.handle, float(eps)))
+
+    def paged_attention(self, out: Buffer, q: Buffer, cache: Paged, batch: Batch) -> None:
+        """attention() of the batch's tokens over what each of them sees."""
+        check(lib().th_paged_attention(self.handle, out.handle, q.handle, cache.handle, batch.handle))
+
+    def accept(self, batch: Batch, logits: Buffer, tokens) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+        """The greedy verification of the batch's drafted tokens: each row's
+        largest logit, how many tokens of each sequence are kept, and their
+        places in it, from its first token's element on (-1 behind them)."""
+        t = _ints(tokens, np.uint32)
+        if t.size != batch.n_tokens:
+            raise ValueError(f"{t.size} tokens of a batch of {batch.n_tokens}")
+        picks, n_kept, kept = np.empty(t.size, np.uint32), np.empty(batch.n_seqs, np.uint32), np.empty(t.size, np.int32)
+        check(lib().th_batch_accept(self.handle, batch.handle, logits.handle, t.ctypes.data, picks.ctypes.data,
+                                    n_kept.ctypes.data, kept.ctypes.data))
+        return picks, n_kept, kept
+
+    def paged_keep(self, caches, batch: Batch, n_kept, kept) -> None:
+        """The rows of the tokens kept (as accept() gives them), moved up behind the context in each cache."""
+        n, k = _ints(n_kept, np.uint32), _ints(kept, np.int32)
+        if n.size != batch.n_seqs or k.size != batch.n_tokens:
+            raise ValueError(f"{n.size} counts and {k.size} places for {batch.n_seqs} sequences of {batch.n_tokens} tokens")
+        handles = (C.c_void_p * len(caches))(*(c.handle for c in caches))
+        check(lib().th_paged_keep(self.handle, handles, len(caches), batch.handle, n.ctypes.data, k.ctypes.data))
+
     # ---- the next token ----
 
     def argmax(self, logits: Buffer) -> int:
@@ -332,4 +470,4 @@ class Hip:
         return int(tok.value)
 
 
-__all__ = ["Hip", "Tensor", "Weight", "Buffer", "Q8", "_lib"]
+__all__ = ["Hip", "Tensor", "Weight", "Buffer", "Q8", "Paged", "Batch", "_lib"]

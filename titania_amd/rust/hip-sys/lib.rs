@@ -34,6 +34,14 @@ pub struct th_graph {
 pub struct th_q8 {
     _p: [u8; 0],
 }
+#[repr(C)]
+pub struct th_paged {
+    _p: [u8; 0],
+}
+#[repr(C)]
+pub struct th_batch {
+    _p: [u8; 0],
+}
 
 /// model/config.rs:9-36 with head_dim resolved.
 #[repr(C)]
@@ -135,6 +143,27 @@ unsafe extern "C" {
     pub fn th_matmul_q8(dev: *mut th_device, out: *mut th_buffer, w: *const th_q8, x: *const th_q8) -> c_int;
 
     // The forward pass (model/model.rs) and the decode loops on the device.
+    pub fn th_paged_alloc(dev: *mut th_device, pages: usize, page_len: usize, n_kv_heads: usize, head_dim: usize,
+                          kv_dtype: c_int, out: *mut *mut th_paged) -> c_int;
+    pub fn th_paged_free(dev: *mut th_device, cache: *mut th_paged);
+    pub fn th_paged_shape(cache: *const th_paged, pages: *mut usize, page_len: *mut usize, n_kv_heads: *mut usize,
+                          head_dim: *mut usize, kv_dtype: *mut c_int) -> c_int;
+    pub fn th_paged_read(dev: *mut th_device, cache: *const th_paged, page: usize, k: *mut f32, v: *mut f32) -> c_int;
+    pub fn th_paged_write(dev: *mut th_device, cache: *mut th_paged, page: usize, k: *const f32, v: *const f32) -> c_int;
+    pub fn th_batch_alloc(dev: *mut th_device, cache: *const th_paged, n_heads: usize, max_seqs: usize,
+                          max_tokens: usize, max_pages: usize, out: *mut *mut th_batch) -> c_int;
+    pub fn th_batch_free(dev: *mut th_device, batch: *mut th_batch);
+    pub fn th_batch_set(dev: *mut th_device, batch: *mut th_batch, n_seqs: usize, context: *const u32,
+                        n_new: *const u32, pages: *const u32, n_pages: usize, parents: *const i32) -> c_int;
+    pub fn th_paged_append(dev: *mut th_device, q_out: *mut th_buffer, q: *const th_buffer, k: *const th_buffer,
+                           v: *const th_buffer, q_norm: *const th_weight, k_norm: *const th_weight,
+                           rope: *const th_buffer, cache: *mut th_paged, batch: *const th_batch, eps: f32) -> c_int;
+    pub fn th_paged_attention(dev: *mut th_device, out: *mut th_buffer, q: *const th_buffer, cache: *const th_paged,
+                              batch: *const th_batch) -> c_int;
+    pub fn th_batch_accept(dev: *mut th_device, batch: *const th_batch, logits: *const th_buffer, tokens: *const u32,
+                           picks: *mut u32, n_kept: *mut u32, kept: *mut i32) -> c_int;
+    pub fn th_paged_keep(dev: *mut th_device, caches: *const *mut th_paged, n_caches: usize, batch: *const th_batch,
+                         n_kept: *const u32, kept: *const i32) -> c_int;
     pub fn th_model_create(dev: *mut th_device, config: *const th_config, weights: *const *const th_weight,
                            n_weights: usize, out: *mut *mut th_model) -> c_int;
     pub fn th_model_destroy(model: *mut th_model);
