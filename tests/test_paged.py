@@ -481,17 +481,19 @@ def test_keep(hip, layers, kvh, hd, page, context, new, kv):
 
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
-def test_captured_calls_take_any_step(hip, kv):
-    """One graph of an append and an attention, over steps of other lengths,
-    pages and trees, with the same calls run eagerly between the replays."""
+@pytest.mark.parametrize("at", [([100, 7], [60, 13]), ([2] * 73, [1] * 73)])
+def test_captured_calls_take_any_step(hip, at, kv):
+    """One graph of an append and an attention, captured with two trees or with
+    73 single tokens, over steps of other lengths, pages and trees, with the same
+    calls run eagerly between the replays."""
     r = np.random.default_rng(8)
     heads, kvh, hd, page = 16, 8, 128, 16
-    lens = [([100, 7], [60, 13]), ([3, 900], [1, 2]), ([500], [70]), ([0, 0, 0], [20, 1, 1]), ([64], [1]), ([], []), ([1200, 40], [5, 66])]
-    steps = [Step(r, c, n, page, [some_tree(r, x) for x in n] if i % 2 else None, spare=0) for i, (c, n) in enumerate(lens)]
+    lens = [at, ([3, 900], [1, 2]), ([500], [70]), ([0, 0, 0], [20, 1, 1]), ([64], [1]), ([], []), ([1200, 40], [5, 66])]
+    steps = [Step(r, c, n, page, [some_tree(r, x) for x in n] if i % 2 == 0 else None, spare=0) for i, (c, n) in enumerate(lens)]
     most, tokens = max(s.pages for s in steps), 73
     pool = pool_of(r, most, page, kvh, hd, kv)
     cache = cache_of(hip, pool, kv)
-    batch = hip.alloc_batch(cache, heads, 3, tokens + 1, most)
+    batch = hip.alloc_batch(cache, heads, 73, tokens + 1, most)
     q, k, v = (r.standard_normal((tokens, h, hd), dtype=np.float32) for h in (heads, kvh, kvh))
     bq, bk, bv = buf(hip, q), buf(hip, k), buf(hip, v)
     gain = hip.upload(Tensor((hd,), f32_to_bf16(1 + 0.1 * r.standard_normal(hd).astype(np.float32))))

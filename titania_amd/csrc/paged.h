@@ -32,9 +32,29 @@ struct TokenAt {
 struct SeqAt {
     uint32_t token0, n_new, context, page0, is_tree;
 };
+// The attention's work, planned once a step for all layers: rows (token, query
+// head of the group) [row0, row0 + the class's tile) of a sequence over its
+// positions [k0, k1), for each KV head. Where a tile's positions are split,
+// `part` is the first slab of its partials (kNoPart: none).
+constexpr int kClasses = 3;
+constexpr int kClassRows[kClasses] = {16, 32, 64};
+constexpr uint32_t kNoPart = 0xffffffffu;
+struct ItemAt {
+    uint32_t seq, row0, k0, k1, part;
+};
+// A split tile: `n_parts` items, each with `slabs` slabs for each KV head.
+struct JoinAt {
+    uint32_t seq, row0, part, n_parts, slabs;
+};
+// A slab: the unnormalized results of 16 rows, then their maxima and sums.
+constexpr size_t slab_floats(size_t head_dim) { return 16 * (head_dim + 2); }
+constexpr size_t slabs_of(size_t head_dim) { return kAttnRoundFloats / slab_floats(head_dim); }
+
 // The counts that a captured launch, whose grid is fixed, reads.
 struct BatchHead {
     uint32_t n_seqs, n_tokens;
+    uint32_t n_joins, join_rows;  // the most rows of a split tile
+    uint32_t first[kClasses + 1];  // a class's items: [first[c], first[c + 1])
 };
 // A batch's arrays in device memory.
 struct BatchView {
@@ -43,8 +63,21 @@ struct BatchView {
     const TokenAt *tokens;
     const uint32_t *pages;
     const uint64_t *tree;  // [token][kTreeWords]: which of its sequence's tokens it sees
+    const ItemAt *items;
+    const JoinAt *joins;
     int page_shift;
 };
+
+// What a plan may hold, and what it is made for.
+struct PlanShape {
+    size_t n_kv_heads, head_dim, group, max_items, max_joins;
+    unsigned classes;  // a bit for each class that may be used: the first always
+};
+// The most items and split tiles of a batch.
+size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens);
+size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens);
+// Plans the attention of the head's sequences.
+void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins);
 
 // q_out = q normalized and rotated; keys (normalized and rotated) and values to
 // the cache. `n` tokens are launched for, those of the head are done.
@@ -67,8 +100,12 @@ struct PagedAttnArgs {
     const void *cache;
     int n_heads, n_kv_heads, group;
     float scale;
+    float *part;  // slabs
 };
-hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, size_t n, size_t head_dim, bool bf16);
+// `count`: what is set now, to be launched for. `captured`: what is set later is
+// launched for too, by the classes that are set now and the first.
+hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, size_t head_dim, bool bf16,
+                                  bool captured);
 
 // picks[row * splits + split] = the packed argmax of a part of a row.
 hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, int splits, uint64_t *picks);
@@ -89,12 +126,12 @@ struct PagedMoves {
 static_assert(sizeof(PagedMoves) <= 4096, "kernel arguments");
 hipError_t launch_paged_moves(hipStream_t s, const PagedMoves &m);
 
-// Copies of up to six arrays from pinned host memory in one launch (16-byte
+// Copies of up to eight arrays from pinned host memory in one launch (16-byte
 // units; the addresses are multiples of 16).
 struct Upload {
-    const void *from[6];
-    void *to[6];
-    uint32_t units[6];
+    const void *from[8];
+    void *to[8];
+    uint32_t units[8];
 };
 hipError_t launch_upload(hipStream_t s, const Upload &u);
 

@@ -25,21 +25,31 @@ struct th_batch {
     size_t n_seqs = 0, n_tokens = 0, n_pages = 0, positions = 0;
     // The fewest tokens that a captured call was launched for.
     size_t captured_tokens = SIZE_MAX;
+    // The classes of the attention's items that every captured call launches.
+    unsigned classes = (1u << th::kClasses) - 1;
     char *device = nullptr, *pinned = nullptr;
-    size_t at_seqs = 0, at_tokens = 0, at_pages = 0, at_tree = 0;  // offsets, the same in both
+    // Offsets, the same in both.
+    size_t at_seqs = 0, at_tokens = 0, at_pages = 0, at_tree = 0, at_items = 0, at_joins = 0;
     hipEvent_t copied = nullptr;  // the pinned memory has been read
     int32_t *parents = nullptr;   // [max_tokens], -1: the context
     uint32_t *stamp = nullptr;    // [pages]: the last set() that wrote to a page
     uint32_t epoch = 0;
 
+    th::BatchHead *head() const { return reinterpret_cast<th::BatchHead *>(pinned); }
     th::SeqAt *seqs() const { return reinterpret_cast<th::SeqAt *>(pinned + at_seqs); }
     uint32_t *page_list() const { return reinterpret_cast<uint32_t *>(pinned + at_pages); }
+    th::PlanShape plan_shape() const {
+        return {n_kv_heads, head_dim, n_heads / n_kv_heads, th::most_items(n_heads, n_kv_heads, max_seqs, max_tokens),
+                th::most_joins(n_heads, n_kv_heads, max_seqs, max_tokens), classes};
+    }
     th::BatchView view() const {
         return {reinterpret_cast<const th::BatchHead *>(device),
                 reinterpret_cast<const th::SeqAt *>(device + at_seqs),
                 reinterpret_cast<const th::TokenAt *>(device + at_tokens),
                 reinterpret_cast<const uint32_t *>(device + at_pages),
                 reinterpret_cast<const uint64_t *>(device + at_tree),
+                reinterpret_cast<const th::ItemAt *>(device + at_items),
+                reinterpret_cast<const th::JoinAt *>(device + at_joins),
                 page_shift};
     }
 };
@@ -255,6 +265,8 @@ int th_batch_alloc(th_device *dev, const th_paged *c, size_t n_heads, size_t max
     b->at_tokens = place(max_tokens * sizeof(th::TokenAt));
     b->at_pages = place(max_pages * sizeof(uint32_t));
     b->at_tree = place(max_tokens * th::kTreeWords * sizeof(uint64_t));
+    b->at_items = place(th::most_items(n_heads, c->n_kv_heads, max_seqs, max_tokens) * sizeof(th::ItemAt));
+    b->at_joins = place(th::most_joins(n_heads, c->n_kv_heads, max_seqs, max_tokens) * sizeof(th::JoinAt));
     b->parents = static_cast<int32_t *>(malloc(max_tokens * sizeof(int32_t)));
     b->stamp = static_cast<uint32_t *>(calloc(c->pages, sizeof(uint32_t)));
     if (!b->parents || !b->stamp) {
@@ -331,7 +343,7 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     }
     TH_PAGED_CURRENT(dev);
     TH_HIP(hipEventSynchronize(b->copied));  // the copy before has read the pinned memory
-    auto *head = reinterpret_cast<th::BatchHead *>(b->pinned);
+    auto *head = b->head();
     auto *seqs = b->seqs();
     auto *toks = reinterpret_cast<th::TokenAt *>(b->pinned + b->at_tokens);
     auto *tree = reinterpret_cast<uint64_t *>(b->pinned + b->at_tree);
@@ -369,6 +381,9 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     b->n_tokens = tokens;
     b->n_pages = n_pages;
     b->positions = positions;
+    auto *items = reinterpret_cast<th::ItemAt *>(b->pinned + b->at_items);
+    auto *joins = reinterpret_cast<th::JoinAt *>(b->pinned + b->at_joins);
+    th::plan_attention(b->plan_shape(), seqs, head, items, joins);
     th::Upload u{};
     int k = 0;
     auto add = [&](size_t at, size_t bytes) {
@@ -381,6 +396,8 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     add(b->at_tokens, tokens * sizeof(th::TokenAt));
     add(b->at_pages, n_pages * sizeof(uint32_t));
     add(b->at_tree, trees * th::kTreeWords * sizeof(uint64_t));
+    add(b->at_items, head->first[th::kClasses] * sizeof(th::ItemAt));
+    add(b->at_joins, head->n_joins * sizeof(th::JoinAt));
     TH_HIP(th::launch_upload(dev->stream, u));
     TH_HIP(hipEventRecord(b->copied, dev->stream));
     return TH_OK;
@@ -416,9 +433,14 @@ int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const
     TH_REQUIRE(n == 0 || out->ptr != q->ptr, "attention cannot write its queries");
     TH_PAGED_CURRENT(dev);
     th::PagedAttnArgs a{b->view(), out->ptr, q->ptr, c->ptr, (int)b->n_heads, (int)b->n_kv_heads,
-                        (int)(b->n_heads / b->n_kv_heads), 1.0f / sqrtf((float)hd)};
-    TH_HIP(th::launch_paged_attention(dev->stream, a, n, hd, c->kv_dtype == TH_KV_BF16));
+                        (int)(b->n_heads / b->n_kv_heads), 1.0f / sqrtf((float)hd), dev->part};
+    TH_HIP(th::launch_paged_attention(dev->stream, a, *b->head(), hd, c->kv_dtype == TH_KV_BF16, dev->capturing));
     note_capture(dev, b);
+    if (dev->capturing) {
+        unsigned launched = 1;
+        for (int i = 0; i < th::kClasses; ++i) launched |= (b->head()->first[i + 1] > b->head()->first[i]) << i;
+        const_cast<th_batch *>(b)->classes &= launched;
+    }
     return TH_OK;
 }
 

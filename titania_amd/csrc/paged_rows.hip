@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void argmax_rows_kernel(const float *x, size_t
 
 __global__ __launch_bounds__(256) void upload_kernel(Upload u) {
 #pragma unroll
-    for (int k = 0; k < 6; ++k)
+    for (int k = 0; k < 8; ++k)
         for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < u.units[k]; i += gridDim.x * 256)
             static_cast<uint4 *>(u.to[k])[i] = static_cast<const uint4 *>(u.from[k])[i];
 }
