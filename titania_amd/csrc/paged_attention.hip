@@ -309,6 +309,511 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
     }
 }
 
+// ---- tiles of many rows ----
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kManyThreads = 512, kManyKeys = 64;
+
+// Two f32 as f16 terms hi + lo, each to the nearest: 22 bits of a value within
+// 2^16 below the largest that f16 holds, 2^-25 below that of any.
+template <bool LO>
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const f16x2 h = __builtin_convertvector((f32x2){a, b}, f16x2);
+    hi = __builtin_bit_cast(uint32_t, h);
+    if constexpr (LO)
+        lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a - (float)h[0], b - (float)h[1]}, f16x2));
+}
+
+__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+// The exponent that brings values of at most this magnitude below 2^15.
+__device__ __forceinline__ int shift_of(uint32_t most) { return 14 + 127 - (int)(most >> 23); }
+
+// The maximum over aligned groups of `LANES` lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// Which of the 64 positions from c on a sequence's token sees.
+__device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tree, uint32_t token, uint32_t c) {
+    const int d = (int)(c - seq.context);
+    const int before = d >= 0 ? 0 : d <= -64 ? 64 : -d;
+    if (!seq.is_tree) {
+        const int n = (int)token + 1 - d;
+        return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+    }
+    const uint64_t *words = tree + (size_t)(seq.token0 + token) * kTreeWords;
+    const int at = d < 0 ? 0 : d, word = at >> 6, shift = at & 63;
+    const uint64_t low = words[word] >> shift, high = words[word + 1 < kTreeWords ? word + 1 : word];
+    const uint64_t bits = low | (shift && word + 1 < kTreeWords ? high << (64 - shift) : 0ull);
+    return before == 64 ? ~0ull : (bits << before) | ((1ull << before) - 1);
+}
+
+// Tiles of up to 128 SETS rows: eight waves of SETS sets of 16, positions 64 at
+// a time through LDS, in two buffers: while a tile's products run, the next
+// one's keys and values, already in registers, are converted and stored, and
+// the one after it is requested. One barrier a tile.
+//
+// Products on v_mfma_f32_16x16x32_f16, every f32 as two f16 terms and a product
+// as hi hi + hi lo + lo hi (values of a bf16 cache are one f16 term, exactly,
+// and two products). What f16 lacks in range powers of two make up: of each
+// key and each query row its own, of a tile's values one, the smallest so far
+// in the tile's order, to which a row's sums are brought along when it changes;
+// the weights are of exp2(x - max + 14). Results are those of f32 but for
+// 2^-21 of a product, and for what lies 2^38 below the largest value that a
+// row sees.
+//
+// S^T = K Q^T leaves a lane four neighbouring positions of its row in each of
+// the tile's four sixteens, which with V^T's columns in that order are the
+// operand of O^T = V^T P^T.
+//
+// A tile with an infinity or a NaN, or where rows do not see all positions and
+// the positions' values differ by more than 2^12, and the ones after it, are
+// summed from memory in f32, a position at a time, by each row for itself:
+// what it does not see does not reach it.
+template <int HD, int SETS, typename KV>
+__global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnArgs a, int cls) {
+    constexpr bool F32 = sizeof(KV) == 4;
+    constexpr int KT = kManyKeys, RW = 16 * SETS;
+    constexpr int KS = HD + 8, VS = KT + 8;    // f16 between rows in LDS: fragment reads meet no bank twice
+    constexpr int LPK = HD / 8;                // lanes a key
+    constexpr int KU = KT * LPK / kManyThreads;  // keys' units (8 values) of a thread
+    constexpr int VD = HD / 64;                // neighbouring dimensions of a thread, of 8 positions
+    // A buffer's parts, in bytes: keys hi, lo, values hi, lo.
+    constexpr uint32_t kKL = KT * KS * 2, kVH = (F32 ? 2 : 1) * kKL, kVL = kVH + HD * VS * 2, kBuf = F32 ? kVL + HD * VS * 2 : kVL;
+    __shared__ __align__(16) char lds[2 * kBuf];
+    __shared__ __align__(16) float kscale[2][KT];
+    __shared__ uint32_t top_of[2][8], least_of[2][8];
+    __shared__ uint32_t odd_of[4];
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t first = a.b.head->first[cls], n = (a.b.head->first[cls + 1] - first) * a.n_kv_heads;
+    const float c2 = a.scale * kLog2e;
+    for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
+        const ItemAt it = a.b.items[first + at / a.n_kv_heads];
+        const int kvh = at % a.n_kv_heads;
+        const SeqAt seq = a.b.seqs[it.seq];
+        const uint32_t rows = min((uint32_t)(8 * RW), seq.n_new * a.group - it.row0);
+        const size_t qbase = ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
+        auto row_at = [&](uint32_t row) { return qbase + ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
+        uint32_t token[SETS];
+        uint4 qh[SETS][HD / 32], ql[SETS][HD / 32];
+        float qf[SETS];  // the scale of a row's scores, c2 in it
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+            const uint32_t row = it.row0 + min((uint32_t)(RW * wave + 16 * s + li), rows - 1);  // past the last: it again
+            token[s] = row / a.group;
+            const float *const src = a.q + row_at(row) + 8 * lg;
+            float f[HD / 32][8];
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                const float4 x = *reinterpret_cast<const float4 *>(src + 32 * c);
+                const float4 y = *reinterpret_cast<const float4 *>(src + 32 * c + 4);
+                const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[c][e] = v[e];
+                    most = max(most, magnitude(v[e]));
+                }
+            }
+            most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+            const int sh = shift_of(most);
+            qf[s] = ldexpf(c2, -sh);
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_f16<true>(ldexpf(f[c][2 * e], sh), ldexpf(f[c][2 * e + 1], sh), h[e], l[e]);
+                qh[s][c] = make_uint4(h[0], h[1], h[2], h[3]);
+                ql[s][c] = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        }
+        // The first and the last position that not every row of the wave sees.
+        const uint32_t w0 = min((uint32_t)(RW * wave), rows - 1), w1 = min((uint32_t)(RW * wave + RW - 1), rows - 1);
+        const uint32_t all_see = seq.context + (seq.is_tree ? 0 : (it.row0 + w0) / a.group + 1);
+        const uint32_t none_sees = seq.context + (it.row0 + w1) / a.group + 1;
+        const bool idle = (uint32_t)(RW * wave) >= rows;
+        f32x4 o[SETS][HD / 16];
+        float mx[SETS], l[SETS];
+        int units[SETS];  // o is of values times 2^units
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+            mx[s] = -INFINITY;
+            l[s] = 0.f;
+            units[s] = 0;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) o[s][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const uint32_t *const pages = a.b.pages + seq.page0;
+        const uint32_t mask = (1u << a.b.page_shift) - 1;
+        const size_t to_v = ((size_t)a.n_kv_heads << a.b.page_shift) * HD;
+        // A key's row, with its sixteen's page: positions past the last repeat its page.
+        auto row_of = [&](uint32_t pos) {
+            const size_t page = pages[min(pos, it.k1 - 1) >> a.b.page_shift];
+            return static_cast<const KV *>(a.cache) +
+                   ((((page * 2 * a.n_kv_heads + kvh)) << a.b.page_shift) + (pos & mask)) * HD;
+        };
+        // What a thread stages: keys kkey + KT / KU i, 8 values from 8 kch;
+        // values of dimensions VD lane + {0, ..}, of the 8 positions that are
+        // operand group `wave`: sixteens 2 sigma and 2 sigma + 1, four of each.
+        // (Formed from the thread's number where they are used: with all of them
+        // kept, the registers do not suffice.)
+        const int wkey = wave * (64 / LPK);  // the wave's first
+        const int vkey = 32 * (wave >> 2) + 4 * (wave & 3);
+        auto thread = [] {
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));
+            return t;
+        };
+        auto at_lds = [&](uint32_t o) -> uint4 & { return *reinterpret_cast<uint4 *>(lds + o); };
+        float kraw[KU][8], vraw[8][VD];
+        auto fetch = [&](uint32_t c0) {
+            const int tid = thread();
+            const uint32_t klane = ((tid / LPK - (wkey & ~15)) * HD + 8 * (tid % LPK)) * sizeof(KV);
+            const uint32_t vlane = VD * (tid & 63) * sizeof(KV);
+#pragma unroll
+            for (int i = 0; i < KU; ++i) {
+                const KV *src = reinterpret_cast<const KV *>(
+                    reinterpret_cast<const char *>(row_of(c0 + (wkey & ~15) + KT / KU * i)) + klane);
+                if constexpr (F32) {
+                    const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
+                    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) kraw[i][e] = v[e];
+                } else {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(src);
+                    kraw[i][0] = __uint_as_float(w.x); kraw[i][1] = __uint_as_float(w.y);
+                    kraw[i][2] = __uint_as_float(w.z); kraw[i][3] = __uint_as_float(w.w);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const KV *src = reinterpret_cast<const KV *>(
+                    reinterpret_cast<const char *>(row_of(c0 + 32 * (wave >> 2) + 16 * h) + to_v + 4 * (wave & 3) * HD) + vlane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (F32 && VD == 2) {
+                        const float2 x = *reinterpret_cast<const float2 *>(src + j * HD);
+                        vraw[4 * h + j][0] = x.x;
+                        vraw[4 * h + j][1] = x.y;
+                    } else if constexpr (F32) {
+                        vraw[4 * h + j][0] = src[j * HD];
+                    } else if constexpr (VD == 2) {
+                        vraw[4 * h + j][0] = __uint_as_float(*reinterpret_cast<const uint32_t *>(src + j * HD));
+                    } else {
+                        vraw[4 * h + j][0] = __uint_as_float((uint32_t)src[j * HD]);
+                    }
+                }
+            }
+        };
+        // Values as f32 from what is in registers, zero past the last position.
+        auto value = [&](uint32_t c0, int j, int d) {
+            float f;
+            if constexpr (F32) f = vraw[j][d];
+            else f = d ? bf16_hi(__float_as_uint(vraw[j][0])) : bf16_lo(__float_as_uint(vraw[j][0]));
+            return c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? f : 0.f;
+        };
+        // The largest magnitude of the wave's values, and, where some row does
+        // not see some position, the smallest of a position's largest.
+        auto look = [&](uint32_t c0, uint32_t tile) {
+            uint32_t most = 0, least = 0x7f000000u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int d = 0; d < VD; ++d) most = max(most, magnitude(value(c0, j, d)));
+            most = lanes_max<64>(most);
+            if (c0 + KT > seq.context) {
+#pragma unroll 1
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t own = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+#pragma unroll
+                        for (int d = 0; d < VD; ++d) own = k == j ? max(own, magnitude(value(c0, k, d))) : own;
+                    own = lanes_max<64>(own);
+                    least = own ? min(least, own) : least;
+                }
+            }
+            if (lane == 0) {
+                top_of[tile & 1][wave] = most;
+                least_of[tile & 1][wave] = least;
+            }
+        };
+        int shift = 1 << 20;  // of the last tile's values; at first more than any
+        // The tile in registers to LDS. Returns its values' shift.
+        auto store = [&](uint32_t c0, uint32_t tile) {
+            uint32_t most = 0, least = 0x7f000000u;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                most = max(most, top_of[tile & 1][w]);
+                least = min(least, least_of[tile & 1][w]);
+            }
+            // Infinities and NaN; positions 2^12 apart that not all rows see.
+            bool odd = most >= 0x7f800000u || (least < most && (most >> 23) - (least >> 23) > 12);
+            if (!odd) shift = min(shift, shift_of(most));
+            const uint32_t buf = (tile & 1) * kBuf;
+            const int tid = thread(), kkey = tid / LPK, kch = tid % LPK;
+            const uint32_t kput = buf + (kkey * KS + 8 * kch) * 2, vput = buf + kVH + (VD * (tid & 63) * VS + 8 * wave) * 2;
+#pragma unroll
+            for (int i = 0; i < KU; ++i) {
+                float f[8];
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = kraw[i][e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f[2 * e] = bf16_lo(__float_as_uint(kraw[i][e]));
+                        f[2 * e + 1] = bf16_hi(__float_as_uint(kraw[i][e]));
+                    }
+                }
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, magnitude(f[e]));
+                top = lanes_max<LPK>(top);
+                const int key = kkey + KT / KU * i, sh = shift_of(top);
+                if (top >= 0x7f800000u && c0 + key < it.k1) odd = true;
+                uint32_t h[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_f16<F32>(ldexpf(f[2 * e], sh), ldexpf(f[2 * e + 1], sh), h[e], lo[e]);
+                const uint32_t to = kput + KT / KU * i * KS * 2;
+                at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (F32) at_lds(to + kKL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                if (kch == 0) kscale[tile & 1][key] = ldexpf(1.f, -sh);
+            }
+#pragma unroll
+            for (int d = 0; d < VD; ++d) {
+                uint32_t h[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    split_f16<F32>(ldexpf(value(c0, 2 * e, d), shift), ldexpf(value(c0, 2 * e + 1, d), shift), h[e], lo[e]);
+                const uint32_t to = vput + d * VS * 2;
+                at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (F32) at_lds(to + kVL - kVH) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            if (odd) odd_of[tile & 3] = 1;
+        };
+        // A row's maximum moves to `top`: what to multiply its sums by.
+        auto moved = [&](int s, float top) {
+            const float alpha = mx[s] == -INFINITY ? (l[s] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mx[s] - top);
+            mx[s] = top;
+            return alpha;
+        };
+        // Scores, weights and sums of 32 positions at a time (of 64: 16 more
+        // registers for scores and 16 for weights than there are).
+        auto products = [&](uint32_t c0, uint32_t tile, int tile_shift) {
+            auto mfma = [](const uint4 &x, const uint4 &y, const f32x4 &z) {
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
+            };
+            const bool masked = c0 + KT > all_see || c0 + KT > it.k1;
+            const int tid = thread(), li = tid & 15, lg = tid >> 4 & 3;
+            const uint32_t buf = (tile & 1) * kBuf, kget = buf + (li * KS + 8 * lg) * 2, vget = buf + kVH + (li * VS + 8 * lg) * 2;
+#pragma unroll 1
+            for (int h = 0; h < KT / 32; ++h) {
+                f32x4 st[SETS][2];
+#pragma unroll
+                for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) st[s][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                const uint32_t kb = kget + 32 * h * KS * 2, vb = vget + 32 * h * 2;
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    __builtin_amdgcn_sched_barrier(0);  // one step's fragments in registers
+                    uint4 x[2], y[F32 ? 2 : 1];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) x[j] = at_lds(kb + (16 * j * KS + 32 * c) * 2);
+                    if constexpr (F32)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) y[j] = at_lds(kb + kKL + (16 * j * KS + 32 * c) * 2);
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[j], qh[s][c], st[s][j]);
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[j], ql[s][c], st[s][j]);
+                    if constexpr (F32)
+#pragma unroll
+                        for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) st[s][j] = mfma(y[j], qh[s][c], st[s][j]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                uint4 ph[SETS], pl[SETS];
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float4 kf = *reinterpret_cast<const float4 *>(&kscale[tile & 1][32 * h + 16 * j + 4 * lg]);
+                        const float f[4] = {kf.x, kf.y, kf.z, kf.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) st[s][j][e] *= f[e] * qf[s];
+                    }
+                    if (masked) {
+                        uint32_t own = token[s];
+                        asm volatile("" : "+v"(own));  // (as in one_by_one)
+                        uint64_t all = seen64(seq, a.b.tree, own, c0);
+                        if (it.k1 - c0 < 64) all &= (1ull << (it.k1 - c0)) - 1;
+                        const uint32_t seen = (uint32_t)(all >> 32 * h) >> 4 * lg;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st[s][j][e] = seen >> (16 * j + e) & 1 ? st[s][j][e] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = max_nn(top, st[s][j][e]);
+                    top = rows_max_nn(top);
+                    const bool any = top != -INFINITY;  // the row sees some
+                    top = max_nn(mx[s], top);
+                    if (__any(top != mx[s] || (any && units[s] != tile_shift))) {
+                        const float alpha = moved(s, top);
+                        l[s] *= alpha;
+                        const int by = any ? tile_shift - units[s] : 0;
+                        units[s] += by;
+                        const float f = ldexpf(alpha, by);
+#pragma unroll
+                        for (int d = 0; d < HD / 16; ++d) o[s][d] *= f;
+                    }
+                    const float base = top == -INFINITY ? 0.f : top - 14.f;
+                    uint32_t x[4], y[4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            st[s][j][e] = __builtin_amdgcn_exp2f(st[s][j][e] - base);
+                            l[s] += st[s][j][e];
+                        }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        split_f16<true>(st[s][e / 2][2 * (e & 1)], st[s][e / 2][2 * (e & 1) + 1], x[e], y[e]);
+                    ph[s] = make_uint4(x[0], x[1], x[2], x[3]);
+                    pl[s] = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+#pragma unroll
+                for (int d0 = 0; d0 < HD / 16; d0 += 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    uint4 x[2], y[F32 ? 2 : 1];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) x[i] = at_lds(vb + 16 * (d0 + i) * VS * 2);
+                    if constexpr (F32)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) y[i] = at_lds(vb + kVL - kVH + 16 * (d0 + i) * VS * 2);
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(x[i], ph[s], o[s][d0 + i]);
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(x[i], pl[s], o[s][d0 + i]);
+                    if constexpr (F32)
+#pragma unroll
+                        for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(y[i], ph[s], o[s][d0 + i]);
+                }
+            }
+        };
+        // A row set's results, or partial ones: x[d][e] 2^-by is dimension
+        // 16 d + 4 lg + e of the lane's row, of weights exp2(. - top).
+        auto put = [&](int s, const f32x4 (&x)[HD / 16], float top, float sum, int by) {
+            const int tid = thread(), li = tid & 15, g4 = 4 * (tid >> 4 & 3);
+            const uint32_t r = RW * wave + 16 * s + li;
+            if (r >= rows) return;
+            float *dst;
+            float f;
+            if (it.part == kNoPart) {
+                dst = a.out + row_at(it.row0 + r);
+                f = 1.f / sum;
+            } else {
+                dst = a.part + (size_t)(it.part + kvh * 8 * SETS + r / 16) * slab_floats(HD);
+                f = 1.f;
+                if (g4 == 0) *reinterpret_cast<float2 *>(dst + 16 * HD + 2 * li) = make_float2(top, sum);
+                dst += li * HD;
+            }
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+                *reinterpret_cast<float4 *>(dst + 16 * d + g4) = make_float4(ldexpf(x[d][0] * f, -by), ldexpf(x[d][1] * f, -by),
+                                                                            ldexpf(x[d][2] * f, -by), ldexpf(x[d][3] * f, -by));
+        };
+        // A row set from memory, from the first position on, one at a time.
+        auto one_by_one = [&](int s) {
+            auto as_f32 = [](KV w) { return F32 ? (float)w : bf16_to_f32((uint16_t)w); };
+            const int own = thread() & 63, g4 = 4 * (own >> 4);
+            const uint32_t row = it.row0 + min((uint32_t)(RW * wave + 16 * s + (own & 15)), rows - 1);
+            const float *const qr = a.q + row_at(row) + g4;
+            f32x4 x[HD / 16];
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) x[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (uint32_t key = it.k0; key < it.k1; ++key) {
+                const KV *const kr = row_of(key) + g4, *const vr = kr + to_v;
+                float y = 0.f;
+#pragma unroll 1
+                for (int i = 0; i < HD / 4; ++i) y = fmaf(qr[16 * (i / 4) + i % 4], as_f32(kr[16 * (i / 4) + i % 4]), y);
+                y = rows_sum(y) * c2;
+                const bool sees = seen64(seq, a.b.tree, row / a.group, key) & 1;
+                y = sees ? y : -INFINITY;
+                const float next = max_nn(top, y), base = next == -INFINITY ? 0.f : next;
+                const float alpha = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top - base);
+                const float p = __builtin_amdgcn_exp2f(y - base);
+                top = next;
+                sum = sum * alpha + p;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float more = fmaf(p, as_f32(vr[16 * d + e]), x[d][e] * alpha);
+                        x[d][e] = sees ? more : x[d][e];
+                    }
+            }
+            put(s, x, top, sum, 0);
+        };
+        const uint32_t tiles = (it.k1 - it.k0 + KT - 1) / KT;
+        if (threadIdx.x < 4) odd_of[threadIdx.x] = 0;
+        fetch(it.k0);
+        look(it.k0, 0);
+        __syncthreads();
+        store(it.k0, 0);
+        int now = shift;
+        if (tiles > 1) fetch(it.k0 + KT);
+        uint32_t t = 0;
+        for (; t < tiles; ++t) {
+            const uint32_t c0 = it.k0 + t * KT;
+            if (t + 1 < tiles) look(c0 + KT, t + 1);
+            __syncthreads();  // tile t is stored, the other buffer free, the next one looked at
+            if (odd_of[t & 3]) break;
+            if (threadIdx.x == 0) odd_of[(t + 3) & 3] = 0;  // tile t - 1's, for tile t + 3
+            if (t + 1 < tiles) store(c0 + KT, t + 1);
+            if (t + 2 < tiles) fetch(c0 + 2 * KT);
+            if (!idle && c0 < none_sees) products(c0, t, now);
+            now = shift;
+        }
+        if (!idle) {
+            if (__builtin_expect(t < tiles, 0)) {
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) one_by_one(s);
+            } else {
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) put(s, o[s], mx[s] - 14.f, rows_sum(l[s]), units[s]);
+            }
+        }
+        __syncthreads();  // LDS is written again
+    }
+}
+
 // Joins a split tile's parts: a block a row, its waves over the parts.
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
@@ -377,6 +882,13 @@ hipError_t few(hipStream_t s, const PagedAttnArgs &a, int cls, unsigned grid, bo
     return hipGetLastError();
 }
 
+template <int HD, int SETS>
+hipError_t many(hipStream_t s, const PagedAttnArgs &a, int cls, unsigned grid, bool bf16) {
+    if (bf16) paged_many_kernel<HD, SETS, uint16_t><<<grid, kManyThreads, 0, s>>>(a, cls);
+    else paged_many_kernel<HD, SETS, float><<<grid, kManyThreads, 0, s>>>(a, cls);
+    return hipGetLastError();
+}
+
 template <int HD>
 hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, bool bf16, bool captured) {
     for (int c = 0; c < kClasses; ++c) {
@@ -388,6 +900,8 @@ hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &cou
         if constexpr (HD < 256) {
             if (c == 1) e = few<HD, 2>(s, a, c, grid, bf16);
             if (c == 2) e = few<HD, 4>(s, a, c, grid, bf16);
+            if (c == 3) e = many<HD, 1>(s, a, c, grid, bf16);
+            if (c == 4) e = many<HD, 2>(s, a, c, grid, bf16);
         }
         if (e != hipSuccess) return e;
     }
