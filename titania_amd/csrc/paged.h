@@ -36,8 +36,8 @@ struct SeqAt {
 // head of the group) [row0, row0 + the class's tile) of a sequence over its
 // positions [k0, k1), for each KV head. Where a tile's positions are split,
 // `part` is the first slab of its partials (kNoPart: none).
-constexpr int kClasses = 5;
-constexpr int kClassRows[kClasses] = {16, 32, 64, 128, 256};
+constexpr int kClasses = 4;
+constexpr int kClassRows[kClasses] = {16, 64, 128, 256};
 constexpr uint32_t kNoPart = 0xffffffffu;
 struct ItemAt {
     uint32_t seq, row0, k0, k1, part;

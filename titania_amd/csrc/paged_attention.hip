@@ -39,6 +39,18 @@ __device__ __forceinline__ void widen(const u32x2 &w, float (&f)[4]) {  // four 
     }
 }
 
+// What an earlier launch left and this one only reads, through the scalar cache.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T *p, size_t i) {
+    T v;
+    const auto *w = (const __attribute__((address_space(4))) uint32_t *)(uintptr_t)(p + i);
+    uint32_t u[sizeof(T) / 4];
+#pragma unroll
+    for (size_t k = 0; k < sizeof(T) / 4; ++k) u[k] = w[k];
+    __builtin_memcpy(&v, u, sizeof(T));
+    return v;
+}
+
 __device__ __forceinline__ bool finite(float f) { return (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u; }
 
 // Which of the 16 positions from c on a sequence's token sees, a bit each.
@@ -89,12 +101,12 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
     __shared__ float stat[4][16 * R][2];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t first = a.b.head->first[cls], n = (a.b.head->first[cls + 1] - first) * a.n_kv_heads;
+    const uint32_t first = scalar_load(a.b.head->first, cls), n = (scalar_load(a.b.head->first, cls + 1) - first) * a.n_kv_heads;
     const float c2 = a.scale * kLog2e;
     for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
-        const ItemAt it = a.b.items[first + at / a.n_kv_heads];
+        const ItemAt it = scalar_load(a.b.items, first + at / a.n_kv_heads);
         const int kvh = at % a.n_kv_heads;
-        const SeqAt seq = a.b.seqs[it.seq];
+        const SeqAt seq = scalar_load(a.b.seqs, it.seq);
         const uint32_t rows = min((uint32_t)(16 * R), seq.n_new * a.group - it.row0);
         const float *const qb = a.q + ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
         // Row `row` of the sequence, in q and out.
@@ -131,7 +143,7 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
         const uint32_t *const pages = a.b.pages + seq.page0;
         const uint32_t mask = (1u << a.b.page_shift) - 1;
         // 16 positions from c on, a multiple of 16, lie in one page.
-        auto page_of = [&](uint32_t c) { return pages[min(c, it.k1 - 1) >> a.b.page_shift]; };
+        auto page_of = [&](uint32_t c) { return scalar_load(pages, min(c, it.k1 - 1) >> a.b.page_shift); };
         auto rows_of = [&](uint32_t page, uint32_t c) {
             return static_cast<const KV *>(a.cache) +
                    ((((size_t)page * 2 * a.n_kv_heads + kvh) << a.b.page_shift) + (c & mask)) * HD;
@@ -187,6 +199,7 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                if (16u * r >= rows) break;
                 // One row set's operands and scores at a time.
                 if constexpr (R > 1) asm volatile("" ::: "memory");
                 f32x4 s{0.f, 0.f, 0.f, 0.f};
@@ -323,20 +336,37 @@ template <bool LO>
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo) {
     const f16x2 h = __builtin_convertvector((f32x2){a, b}, f16x2);
     hi = __builtin_bit_cast(uint32_t, h);
-    if constexpr (LO)
-        lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a - (float)h[0], b - (float)h[1]}, f16x2));
+    if constexpr (LO) {  // what is left, exactly, in an instruction that takes the f16 as it is
+        float c, d;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(c) : "v"(hi), "v"(a));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(hi), "v"(b));
+        lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){c, d}, f16x2));
+    }
 }
 
+// The larger; NaN if one is (three of them are one instruction).
+__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 // The exponent that brings values of at most this magnitude below 2^15.
 __device__ __forceinline__ int shift_of(uint32_t most) { return 14 + 127 - (int)(most >> 23); }
 
-// The maximum over aligned groups of `LANES` lanes, in each of them.
-template <int LANES>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
+}
+// The maximum over each 16 lanes, in each of them.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = dpp_max<0xB1>(v);          // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);          // quad_perm [2,3,0,1]
+    v = dpp_max<0x124>(v);         // row_ror:4
+    return dpp_max<0x128>(v);      // row_ror:8
+}
+// Over the lanes that are a multiple of 16 apart, in each of them.
+__device__ __forceinline__ uint32_t across_max(uint32_t v) {
+    auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+    auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(q[0], q[1]);
 }
 
 // Which of the 64 positions from c on a sequence's token sees.
@@ -362,9 +392,10 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // Products on v_mfma_f32_16x16x32_f16, every f32 as two f16 terms and a product
 // as hi hi + hi lo + lo hi (values of a bf16 cache are one f16 term, exactly,
 // and two products). What f16 lacks in range powers of two make up: of each
-// key and each query row its own, of a tile's values one, the smallest so far
-// in the tile's order, to which a row's sums are brought along when it changes;
-// the weights are of exp2(x - max + 14). Results are those of f32 but for
+// query row its own, of a tile's keys one, and of its values one, the smallest
+// so far, to which a row's sums are brought along when it changes;
+// the weights are of exp2(x - r + 10), r the row's maximum, or within
+// 2^5 of it. Results are those of f32 but for
 // 2^-21 of a product, and for what lies 2^38 below the largest value that a
 // row sees.
 //
@@ -380,24 +411,24 @@ template <int HD, int SETS, typename KV>
 __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnArgs a, int cls) {
     constexpr bool F32 = sizeof(KV) == 4;
     constexpr int KT = kManyKeys, RW = 16 * SETS;
-    constexpr int KS = HD + 8, VS = KT + 8;    // f16 between rows in LDS: fragment reads meet no bank twice
+    constexpr float kGrow = 5.f, kBase = 10.f;  // weights below 2^15
+    constexpr uint32_t KB = 2 * HD, VB = 2 * KT;  // bytes of a key, and of a dimension's positions
     constexpr int LPK = HD / 8;                // lanes a key
     constexpr int KU = KT * LPK / kManyThreads;  // keys' units (8 values) of a thread
     constexpr int VD = HD / 64;                // neighbouring dimensions of a thread, of 8 positions
     // A buffer's parts, in bytes: keys hi, lo, values hi, lo.
-    constexpr uint32_t kKL = KT * KS * 2, kVH = (F32 ? 2 : 1) * kKL, kVL = kVH + HD * VS * 2, kBuf = F32 ? kVL + HD * VS * 2 : kVL;
+    constexpr uint32_t kKL = KT * KB, kVH = (F32 ? 2 : 1) * kKL, kVL = kVH + HD * VB, kBuf = F32 ? kVL + HD * VB : kVL;
     __shared__ __align__(16) char lds[2 * kBuf];
-    __shared__ __align__(16) float kscale[2][KT];
-    __shared__ uint32_t top_of[2][8], least_of[2][8];
+    __shared__ __align__(16) uint4 looked[2][8];  // of a wave's part of a tile: magnitudes, as below
     __shared__ uint32_t odd_of[4];
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t first = a.b.head->first[cls], n = (a.b.head->first[cls + 1] - first) * a.n_kv_heads;
+    const uint32_t first = scalar_load(a.b.head->first, cls), n = (scalar_load(a.b.head->first, cls + 1) - first) * a.n_kv_heads;
     const float c2 = a.scale * kLog2e;
     for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
-        const ItemAt it = a.b.items[first + at / a.n_kv_heads];
+        const ItemAt it = scalar_load(a.b.items, first + at / a.n_kv_heads);
         const int kvh = at % a.n_kv_heads;
-        const SeqAt seq = a.b.seqs[it.seq];
+        const SeqAt seq = scalar_load(a.b.seqs, it.seq);
         const uint32_t rows = min((uint32_t)(8 * RW), seq.n_new * a.group - it.row0);
         const size_t qbase = ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
         auto row_at = [&](uint32_t row) { return qbase + ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
@@ -422,8 +453,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
                     most = max(most, magnitude(v[e]));
                 }
             }
-            most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-            most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+            most = across_max(most);
             const int sh = shift_of(most);
             qf[s] = ldexpf(c2, -sh);
 #pragma unroll
@@ -435,11 +465,11 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
                 ql[s][c] = make_uint4(l[0], l[1], l[2], l[3]);
             }
         }
-        // The first and the last position that not every row of the wave sees.
-        const uint32_t w0 = min((uint32_t)(RW * wave), rows - 1), w1 = min((uint32_t)(RW * wave + RW - 1), rows - 1);
-        const uint32_t all_see = seq.context + (seq.is_tree ? 0 : (it.row0 + w0) / a.group + 1);
-        const uint32_t none_sees = seq.context + (it.row0 + w1) / a.group + 1;
-        const bool idle = (uint32_t)(RW * wave) >= rows;
+        // Of the wave's rows: the first position that one does not see, and the
+        // first that none sees (zero: there are no such rows).
+        const uint32_t w0 = RW * wave, w1 = min(w0 + RW, rows) - 1;
+        const uint32_t all_see = seq.context + (seq.is_tree ? 0 : (it.row0 + min(w0, rows - 1)) / a.group + 1);
+        const uint32_t none_sees = w0 >= rows ? 0 : seq.context + (it.row0 + w1) / a.group + 1;
         f32x4 o[SETS][HD / 16];
         float mx[SETS], l[SETS];
         int units[SETS];  // o is of values times 2^units
@@ -456,7 +486,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
         const size_t to_v = ((size_t)a.n_kv_heads << a.b.page_shift) * HD;
         // A key's row, with its sixteen's page: positions past the last repeat its page.
         auto row_of = [&](uint32_t pos) {
-            const size_t page = pages[min(pos, it.k1 - 1) >> a.b.page_shift];
+            const size_t page = scalar_load(pages, min(pos, it.k1 - 1) >> a.b.page_shift);
             return static_cast<const KV *>(a.cache) +
                    ((((page * 2 * a.n_kv_heads + kvh)) << a.b.page_shift) + (pos & mask)) * HD;
         };
@@ -471,6 +501,12 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
             int t = threadIdx.x;
             asm volatile("" : "+v"(t));
             return t;
+        };
+        // Where 16 bytes of a row lie: rows of 256 bytes cover the banks, two of
+        // 128 do. What the lanes of a fragment's read take, and neighbouring
+        // lanes write, is in as many banks.
+        auto swizzled = [](uint32_t bytes, uint32_t row, uint32_t chunk) {
+            return row * bytes + 16 * (chunk ^ (bytes == 256 ? row & 15 : row >> 1 & 7));
         };
         auto at_lds = [&](uint32_t o) -> uint4 & { return *reinterpret_cast<uint4 *>(lds + o); };
         float kraw[KU][8], vraw[8][VD];
@@ -513,108 +549,117 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
                 }
             }
         };
-        // Values as f32 from what is in registers, zero past the last position.
-        auto value = [&](uint32_t c0, int j, int d) {
-            float f;
-            if constexpr (F32) f = vraw[j][d];
-            else f = d ? bf16_hi(__float_as_uint(vraw[j][0])) : bf16_lo(__float_as_uint(vraw[j][0]));
-            return c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? f : 0.f;
+        // As f32 from what is in registers.
+        auto value = [&](int j, int d) {
+            if constexpr (F32) return vraw[j][d];
+            else return d ? bf16_hi(__float_as_uint(vraw[j][0])) : bf16_lo(__float_as_uint(vraw[j][0]));
         };
-        // The largest magnitude of the wave's values, and, where some row does
-        // not see some position, the smallest of a position's largest.
+        auto key_value = [&](int i, int e) {
+            if constexpr (F32) return kraw[i][e];
+            else return e & 1 ? bf16_hi(__float_as_uint(kraw[i][e / 2])) : bf16_lo(__float_as_uint(kraw[i][e / 2]));
+        };
+        // The largest magnitude of the wave's keys and values, and, where some
+        // row does not see some position, the smallest of a position's largest.
         auto look = [&](uint32_t c0, uint32_t tile) {
-            uint32_t most = 0, least = 0x7f000000u;
+            uint32_t ktop = 0, vtop = 0, kleast = 0x7f000000u, vleast = 0x7f000000u;
+            if (c0 + KT > it.k1) {  // past the last position is anything: zero
+                const int tid = thread();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                for (int i = 0; i < KU; ++i)
 #pragma unroll
-                for (int d = 0; d < VD; ++d) most = max(most, magnitude(value(c0, j, d)));
-            most = lanes_max<64>(most);
+                    for (int e = 0; e < (F32 ? 8 : 4); ++e)
+                        kraw[i][e] = c0 + tid / LPK + KT / KU * i < it.k1 ? kraw[i][e] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int d = 0; d < (F32 ? VD : 1); ++d)
+                        vraw[j][d] = c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? vraw[j][d] : 0.f;
+            }
             if (c0 + KT > seq.context) {
-#pragma unroll 1
+#pragma unroll
+                for (int i = 0; i < KU; ++i) {
+                    uint32_t own = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) own = max(own, magnitude(key_value(i, e)));
+                    own = LPK == 16 ? row_max(own) : dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(own)));  // row_half_mirror
+                    ktop = max(ktop, own);
+                    kleast = own ? min(kleast, own) : kleast;
+                }
+                kleast = ~across_max(row_max(~kleast));
+#pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     uint32_t own = 0;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-#pragma unroll
-                        for (int d = 0; d < VD; ++d) own = k == j ? max(own, magnitude(value(c0, k, d))) : own;
-                    own = lanes_max<64>(own);
-                    least = own ? min(least, own) : least;
+                    for (int d = 0; d < VD; ++d) own = max(own, magnitude(value(j, d)));
+                    own = across_max(row_max(own));
+                    vtop = max(vtop, own);
+                    vleast = own ? min(vleast, own) : vleast;
                 }
+                ktop = across_max(row_max(ktop));
+            } else {
+                float k = 0.f, v = 0.f;
+#pragma unroll
+                for (int i = 0; i < KU; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        k = max_or_nan(max_or_nan(k, __builtin_fabsf(key_value(i, e))), __builtin_fabsf(key_value(i, e + 1)));
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+#pragma unroll
+                    for (int d = 0; d < VD; ++d)
+                        v = max_or_nan(max_or_nan(v, __builtin_fabsf(value(j, d))), __builtin_fabsf(value(j + 1, d)));
+                ktop = across_max(row_max(magnitude(k)));
+                vtop = across_max(row_max(magnitude(v)));
             }
-            if (lane == 0) {
-                top_of[tile & 1][wave] = most;
-                least_of[tile & 1][wave] = least;
-            }
+            if (lane == 0) looked[tile & 1][wave] = make_uint4(ktop, vtop, kleast, vleast);
         };
         int shift = 1 << 20;  // of the last tile's values; at first more than any
-        // The tile in registers to LDS. Returns its values' shift.
-        auto store = [&](uint32_t c0, uint32_t tile) {
-            uint32_t most = 0, least = 0x7f000000u;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                most = max(most, top_of[tile & 1][w]);
-                least = min(least, least_of[tile & 1][w]);
-            }
-            // Infinities and NaN; positions 2^12 apart that not all rows see.
-            bool odd = most >= 0x7f800000u || (least < most && (most >> 23) - (least >> 23) > 12);
-            if (!odd) shift = min(shift, shift_of(most));
-            const uint32_t buf = (tile & 1) * kBuf;
+        int kshift = 0;       // of the last tile's keys
+        // The tile in registers to LDS.
+        auto store = [&](uint32_t tile) {
+            // A wave's part a lane, the eight of them over each 16 lanes.
             const int tid = thread(), kkey = tid / LPK, kch = tid % LPK;
-            const uint32_t kput = buf + (kkey * KS + 8 * kch) * 2, vput = buf + kVH + (VD * (tid & 63) * VS + 8 * wave) * 2;
+            const uint4 w = looked[tile & 1][tid & 7];
+            auto uniform_max = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(v)); };
+            const uint32_t ktop = uniform_max(w.x), vtop = uniform_max(w.y), kleast = ~uniform_max(~w.z), vleast = ~uniform_max(~w.w);
+            // Infinities and NaN; positions 2^12 apart that not all rows see.
+            const bool odd = max(ktop, vtop) >= 0x7f800000u || (kleast < ktop && (ktop >> 23) - (kleast >> 23) > 12) ||
+                             (vleast < vtop && (vtop >> 23) - (vleast >> 23) > 12);
+            if (!odd) shift = min(shift, shift_of(vtop));
+            kshift = shift_of(ktop);
+            const uint32_t buf = (tile & 1) * kBuf;
+            const uint32_t kput = buf + swizzled(KB, kkey, kch);
 #pragma unroll
             for (int i = 0; i < KU; ++i) {
-                float f[8];
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = kraw[i][e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f[2 * e] = bf16_lo(__float_as_uint(kraw[i][e]));
-                        f[2 * e + 1] = bf16_hi(__float_as_uint(kraw[i][e]));
-                    }
-                }
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, magnitude(f[e]));
-                top = lanes_max<LPK>(top);
-                const int key = kkey + KT / KU * i, sh = shift_of(top);
-                if (top >= 0x7f800000u && c0 + key < it.k1) odd = true;
                 uint32_t h[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_f16<F32>(ldexpf(f[2 * e], sh), ldexpf(f[2 * e + 1], sh), h[e], lo[e]);
-                const uint32_t to = kput + KT / KU * i * KS * 2;
+                for (int e = 0; e < 4; ++e)
+                    split_f16<F32>(ldexpf(key_value(i, 2 * e), kshift), ldexpf(key_value(i, 2 * e + 1), kshift), h[e], lo[e]);
+                const uint32_t to = kput + KT / KU * i * KB;
                 at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
                 if constexpr (F32) at_lds(to + kKL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                if (kch == 0) kscale[tile & 1][key] = ldexpf(1.f, -sh);
             }
 #pragma unroll
             for (int d = 0; d < VD; ++d) {
                 uint32_t h[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    split_f16<F32>(ldexpf(value(c0, 2 * e, d), shift), ldexpf(value(c0, 2 * e + 1, d), shift), h[e], lo[e]);
-                const uint32_t to = vput + d * VS * 2;
+                    split_f16<F32>(ldexpf(value(2 * e, d), shift), ldexpf(value(2 * e + 1, d), shift), h[e], lo[e]);
+                const uint32_t to = buf + kVH + swizzled(VB, VD * (tid & 63) + d, wave);
                 at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
                 if constexpr (F32) at_lds(to + kVL - kVH) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             if (odd) odd_of[tile & 3] = 1;
         };
-        // A row's maximum moves to `top`: what to multiply its sums by.
-        auto moved = [&](int s, float top) {
-            const float alpha = mx[s] == -INFINITY ? (l[s] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mx[s] - top);
-            mx[s] = top;
-            return alpha;
-        };
         // Scores, weights and sums of 32 positions at a time (of 64: 16 more
         // registers for scores and 16 for weights than there are).
-        auto products = [&](uint32_t c0, uint32_t tile, int tile_shift) {
+        auto products = [&](uint32_t c0, uint32_t tile, int tile_shift, int tile_kshift) {
             auto mfma = [](const uint4 &x, const uint4 &y, const f32x4 &z) {
                 return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
             };
             const bool masked = c0 + KT > all_see || c0 + KT > it.k1;
             const int tid = thread(), li = tid & 15, lg = tid >> 4 & 3;
-            const uint32_t buf = (tile & 1) * kBuf, kget = buf + (li * KS + 8 * lg) * 2, vget = buf + kVH + (li * VS + 8 * lg) * 2;
+            const uint32_t buf = (tile & 1) * kBuf, kget = buf + swizzled(KB, li, lg), vget = buf + kVH + swizzled(VB, li, lg);
 #pragma unroll 1
             for (int h = 0; h < KT / 32; ++h) {
                 f32x4 st[SETS][2];
@@ -622,45 +667,46 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
                 for (int s = 0; s < SETS; ++s)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) st[s][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const uint32_t kb = kget + 32 * h * KS * 2, vb = vget + 32 * h * 2;
+                const uint32_t vb = vget ^ 64 * h;  // the chunk 4 h + lg
+                // A step's fragments are requested before the products of the
+                // one before it.
+                uint4 x[2][2], y[2][F32 ? 2 : 1];
+                auto key_fragments = [&](int c) {
+                    const uint32_t kb = (kget ^ 64 * c) + 32 * h * KB;  // the chunk 4 c + lg
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        x[c & 1][j] = at_lds(kb + 16 * j * KB);
+                        if constexpr (F32) y[c & 1][j] = at_lds(kb + kKL + 16 * j * KB);
+                    }
+                };
+                key_fragments(0);
+                __builtin_amdgcn_s_setprio(1);  // products before another wave's conversions
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
-                    __builtin_amdgcn_sched_barrier(0);  // one step's fragments in registers
-                    uint4 x[2], y[F32 ? 2 : 1];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) x[j] = at_lds(kb + (16 * j * KS + 32 * c) * 2);
-                    if constexpr (F32)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) y[j] = at_lds(kb + kKL + (16 * j * KS + 32 * c) * 2);
+                    if (c + 1 < HD / 32) key_fragments(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[j], qh[s][c], st[s][j]);
+                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], qh[s][c], st[s][j]);
 #pragma unroll
                     for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[j], ql[s][c], st[s][j]);
+                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], ql[s][c], st[s][j]);
                     if constexpr (F32)
 #pragma unroll
                         for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) st[s][j] = mfma(y[j], qh[s][c], st[s][j]);
+                            for (int j = 0; j < 2; ++j) st[s][j] = mfma(y[c & 1][j], qh[s][c], st[s][j]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(0);
                 uint4 ph[SETS], pl[SETS];
 #pragma unroll
                 for (int s = 0; s < SETS; ++s) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float4 kf = *reinterpret_cast<const float4 *>(&kscale[tile & 1][32 * h + 16 * j + 4 * lg]);
-                        const float f[4] = {kf.x, kf.y, kf.z, kf.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) st[s][j][e] *= f[e] * qf[s];
-                    }
                     if (masked) {
                         uint32_t own = token[s];
-                        asm volatile("" : "+v"(own));  // (as in one_by_one)
+                        asm volatile("" : "+v"(own));  // (nothing of it formed ahead)
                         uint64_t all = seen64(seq, a.b.tree, own, c0);
                         if (it.k1 - c0 < 64) all &= (1ull << (it.k1 - c0)) - 1;
                         const uint32_t seen = (uint32_t)(all >> 32 * h) >> 4 * lg;
@@ -669,59 +715,69 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
 #pragma unroll
                             for (int e = 0; e < 4; ++e) st[s][j][e] = seen >> (16 * j + e) & 1 ? st[s][j][e] : -INFINITY;
                     }
+                    float top = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) top = max_nn(top, st[s][j][e]);
-                    top = rows_max_nn(top);
+                        for (int e = 0; e < 4; e += 2) top = max_or_nan(max_or_nan(top, st[s][j][e]), st[s][j][e + 1]);
+                    // Scores in units of log2. (Neither zero nor infinite: what is
+                    // not seen is -inf, and stays it.)
+                    const float f = fminf(fmaxf(ldexpf(qf[s], -tile_kshift), 0x1p-126f), 0x1p127f);
+                    top = rows_max_nn(top) * f;
                     const bool any = top != -INFINITY;  // the row sees some
-                    top = max_nn(mx[s], top);
-                    if (__any(top != mx[s] || (any && units[s] != tile_shift))) {
-                        const float alpha = moved(s, top);
+                    // The reference moves when the maximum is 2^kGrow past it.
+                    if (__any(top > mx[s] + kGrow || (any && units[s] != tile_shift))) {
+                        const float next = max_nn(mx[s], top);
+                        const float alpha = mx[s] == next ? 1.f : __builtin_amdgcn_exp2f(mx[s] - next);
+                        mx[s] = next;
                         l[s] *= alpha;
                         const int by = any ? tile_shift - units[s] : 0;
                         units[s] += by;
-                        const float f = ldexpf(alpha, by);
+                        const float g = ldexpf(alpha, by);
 #pragma unroll
-                        for (int d = 0; d < HD / 16; ++d) o[s][d] *= f;
+                        for (int d = 0; d < HD / 16; ++d) o[s][d] *= g;
                     }
-                    const float base = top == -INFINITY ? 0.f : top - 14.f;
-                    uint32_t x[4], y[4];
+                    const float base = mx[s] == -INFINITY ? 0.f : kBase - mx[s];
+                    uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            st[s][j][e] = __builtin_amdgcn_exp2f(st[s][j][e] - base);
+                            st[s][j][e] = __builtin_amdgcn_exp2f(fmaf(st[s][j][e], f, base));
                             l[s] += st[s][j][e];
                         }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        split_f16<true>(st[s][e / 2][2 * (e & 1)], st[s][e / 2][2 * (e & 1) + 1], x[e], y[e]);
-                    ph[s] = make_uint4(x[0], x[1], x[2], x[3]);
-                    pl[s] = make_uint4(y[0], y[1], y[2], y[3]);
+                        split_f16<true>(st[s][e / 2][2 * (e & 1)], st[s][e / 2][2 * (e & 1) + 1], hi[e], lo[e]);
+                    ph[s] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    pl[s] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
+                auto value_fragments = [&](int n) {
 #pragma unroll
-                for (int d0 = 0; d0 < HD / 16; d0 += 2) {
+                    for (int i = 0; i < 2; ++i) {
+                        x[n & 1][i] = at_lds(vb + 16 * (2 * n + i) * VB);
+                        if constexpr (F32) y[n & 1][i] = at_lds(vb + kVL - kVH + 16 * (2 * n + i) * VB);
+                    }
+                };
+                value_fragments(0);
+#pragma unroll
+                for (int n = 0; n < HD / 32; ++n) {
+                    if (n + 1 < HD / 32) value_fragments(n + 1);
                     __builtin_amdgcn_sched_barrier(0);
-                    uint4 x[2], y[F32 ? 2 : 1];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) x[i] = at_lds(vb + 16 * (d0 + i) * VS * 2);
-                    if constexpr (F32)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) y[i] = at_lds(vb + kVL - kVH + 16 * (d0 + i) * VS * 2);
 #pragma unroll
                     for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(x[i], ph[s], o[s][d0 + i]);
+                        for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], ph[s], o[s][2 * n + i]);
 #pragma unroll
                     for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(x[i], pl[s], o[s][d0 + i]);
+                        for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], pl[s], o[s][2 * n + i]);
                     if constexpr (F32)
 #pragma unroll
                         for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) o[s][d0 + i] = mfma(y[i], ph[s], o[s][d0 + i]);
+                            for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(y[n & 1][i], ph[s], o[s][2 * n + i]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         };
@@ -786,8 +842,8 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
         fetch(it.k0);
         look(it.k0, 0);
         __syncthreads();
-        store(it.k0, 0);
-        int now = shift;
+        store(0);
+        int now = shift, know = kshift;
         if (tiles > 1) fetch(it.k0 + KT);
         uint32_t t = 0;
         for (; t < tiles; ++t) {
@@ -796,80 +852,96 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
             __syncthreads();  // tile t is stored, the other buffer free, the next one looked at
             if (odd_of[t & 3]) break;
             if (threadIdx.x == 0) odd_of[(t + 3) & 3] = 0;  // tile t - 1's, for tile t + 3
-            if (t + 1 < tiles) store(c0 + KT, t + 1);
+            if (t + 1 < tiles) store(t + 1);
             if (t + 2 < tiles) fetch(c0 + 2 * KT);
-            if (!idle && c0 < none_sees) products(c0, t, now);
+            if (c0 < none_sees) products(c0, t, now, know);
             now = shift;
+            know = kshift;
         }
-        if (!idle) {
+        if (none_sees) {
             if (__builtin_expect(t < tiles, 0)) {
 #pragma unroll
                 for (int s = 0; s < SETS; ++s) one_by_one(s);
             } else {
 #pragma unroll
-                for (int s = 0; s < SETS; ++s) put(s, o[s], mx[s] - 14.f, rows_sum(l[s]), units[s]);
+                for (int s = 0; s < SETS; ++s) put(s, o[s], mx[s] - kBase, rows_sum(l[s]), units[s]);
             }
         }
         __syncthreads();  // LDS is written again
     }
 }
 
-// Joins a split tile's parts: a block a row, its waves over the parts.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-    constexpr int E = HD / 64;
-    __shared__ float red[4][HD], stat[4][2];
+// Joins a split tile's parts, `W` waves a row: four for few rows of many parts,
+// which then wait for a quarter of them, one for many rows.
+template <int HD, int W>
+__device__ __forceinline__ void join_rows(const PagedAttnArgs &a, const BatchHead &head) {
+    constexpr int E = HD / 64, ROWS = 4 / W;  // a block's rows
+    __shared__ float red[W == 1 ? 1 : 4][W == 1 ? 1 : HD], stat[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // Rows of a join: those of its tile, for each KV head. gridDim.x walks them.
-    for (uint32_t j = blockIdx.y; j < a.b.head->n_joins; j += gridDim.y) {
-        const JoinAt join = a.b.joins[j];
-        const SeqAt seq = a.b.seqs[join.seq];
+    // gridDim.y walks the tiles, gridDim.x their rows, for each KV head.
+    for (uint32_t j = blockIdx.y; j < head.n_joins; j += gridDim.y) {
+        const JoinAt join = scalar_load(a.b.joins, j);
+        const SeqAt seq = scalar_load(a.b.seqs, join.seq);
         const uint32_t rows = min(16 * join.slabs, seq.n_new * a.group - join.row0);
-        for (uint32_t i = blockIdx.x; i < rows * a.n_kv_heads; i += gridDim.x) {
+        for (uint32_t i = blockIdx.x * ROWS + (W == 1 ? wave : 0); i < rows * a.n_kv_heads; i += gridDim.x * ROWS) {
             const uint32_t row = i % rows, kvh = i / rows;
             const float *part = a.part + (size_t)(join.part + kvh * join.slabs + row / 16) * slab_floats(HD);
             const size_t step = (size_t)join.slabs * a.n_kv_heads * slab_floats(HD);
-            float top = -INFINITY, l = 0.f, acc[E];
+            // The maximum first, so that the parts' sums wait for nothing.
+            float top = -INFINITY;
+            for (uint32_t p = lane; p < join.n_parts; p += 64) top = fmaxf(top, part[p * step + 16 * HD + 2 * (row % 16)]);
+            top = wave_max_dpp(top);
+            float l = 0.f, acc[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-            for (uint32_t p = wave; p < join.n_parts; p += 4) {
+#pragma unroll 8
+            for (uint32_t p = W == 1 ? 0 : wave; p < join.n_parts; p += W) {
                 const float *s = part + p * step;
                 const float2 ml = *reinterpret_cast<const float2 *>(s + 16 * HD + 2 * (row % 16));
                 float x[E];
+                if constexpr (E == 2) {
+                    const float2 v = *reinterpret_cast<const float2 *>(s + (row % 16) * HD + 2 * lane);
+                    x[0] = v.x;
+                    x[1] = v.y;
+                } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = s[(row % 16) * HD + E * lane + e];
-                const float now = fmaxf(top, ml.x);
-                const float before = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
-                // A part of no weight has no maximum; one of NaN has none either.
-                const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - now);
-                l = l * (top == -INFINITY && l != 0.f ? 1.f : before) + ml.y * f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e] * before);
-                top = now;
-            }
-            if (lane == 0) {
-                stat[wave][0] = top;
-                stat[wave][1] = l;
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) red[wave][E * lane + e] = acc[e];
-            __syncthreads();
-            if (threadIdx.x < HD) {
-                const float all = fmaxf(fmaxf(stat[0][0], stat[1][0]), fmaxf(stat[2][0], stat[3][0]));
-                float sum = 0.f, ls = 0.f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = stat[w][0] == -INFINITY ? (stat[w][1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(stat[w][0] - all);
-                    sum = fmaf(red[w][threadIdx.x], f, sum);
-                    ls = fmaf(stat[w][1], f, ls);
+                    for (int e = 0; e < E; ++e) x[e] = s[(row % 16) * HD + E * lane + e];
                 }
-                const uint32_t r = join.row0 + row;
-                a.out[((size_t)(seq.token0 + r / a.group) * a.n_heads + (size_t)kvh * a.group + r % a.group) * HD + threadIdx.x] = sum / ls;
+                // A part of no weight has no maximum; one of NaN has none either.
+                const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - top);
+                l = fmaf(ml.y, f, l);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e]);
             }
-            __syncthreads();
+            const uint32_t r = join.row0 + row;
+            float *out = a.out + ((size_t)(seq.token0 + r / a.group) * a.n_heads + (size_t)kvh * a.group + r % a.group) * HD;
+            if constexpr (W == 1) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) out[E * lane + e] = acc[e] / l;
+            } else {
+                if (lane == 0) stat[wave] = l;
+#pragma unroll
+                for (int e = 0; e < E; ++e) red[wave][E * lane + e] = acc[e];
+                __syncthreads();
+                if (threadIdx.x < HD) {
+                    const float sum = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+                    out[threadIdx.x] = sum / ((stat[0] + stat[1]) + (stat[2] + stat[3]));
+                }
+                __syncthreads();
+            }
         }
     }
+}
+
+constexpr uint32_t kManyRows = 2048;  // of a join's launch
+
+// (Which of the two goes by the plan alone: a captured launch gives the bits of
+// any other.)
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+    const BatchHead head = scalar_load(a.b.head, 0);
+    if (head.join_rows * a.n_kv_heads * head.n_joins > kManyRows) join_rows<HD, 1>(a, head);
+    else join_rows<HD, 4>(a, head);
 }
 
 // A captured launch's grid, whatever is set later: its blocks walk the items.
@@ -898,15 +970,15 @@ hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &cou
         hipError_t e = hipSuccess;
         if (c == 0) e = few<HD, 1>(s, a, c, grid, bf16);
         if constexpr (HD < 256) {
-            if (c == 1) e = few<HD, 2>(s, a, c, grid, bf16);
-            if (c == 2) e = few<HD, 4>(s, a, c, grid, bf16);
-            if (c == 3) e = many<HD, 1>(s, a, c, grid, bf16);
-            if (c == 4) e = many<HD, 2>(s, a, c, grid, bf16);
+            if (c == 1) e = few<HD, 4>(s, a, c, grid, bf16);
+            if (c == 2) e = many<HD, 1>(s, a, c, grid, bf16);
+            if (c == 3) e = many<HD, 2>(s, a, c, grid, bf16);
         }
         if (e != hipSuccess) return e;
     }
     if (!count.n_joins && !captured) return hipSuccess;
-    const dim3 grid = captured ? dim3(64, 64) : dim3(std::min(count.join_rows * a.n_kv_heads, 4096u), std::min(count.n_joins, 4096u));
+    const uint32_t rows = count.join_rows * a.n_kv_heads, blocks = rows * count.n_joins > kManyRows ? (rows + 3) / 4 : rows;
+    const dim3 grid = captured ? dim3(64, 64) : dim3(std::min(blocks, 4096u), std::min(count.n_joins, 4096u));
     paged_join_kernel<HD><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }

@@ -8,10 +8,10 @@ namespace th {
 
 namespace {
 
-// Blocks that a step is split for, where its positions allow: two of four
-// waves a CU.
-constexpr size_t kBlocks = 512;
-// A block's fewest positions: one step of its four waves.
+// The blocks that a class's positions are split for, where they allow: what the
+// chip holds of them at once.
+constexpr size_t kBlocks[kClasses] = {512, 256, 256, 256};
+// A block's fewest positions: one step of its waves.
 constexpr size_t kStep = 64;
 
 }  // namespace
@@ -21,12 +21,13 @@ size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max
 }
 
 size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens) {
-    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kBlocks;
+    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kBlocks[0] + kBlocks[1] + kBlocks[2] + kBlocks[3];
 }
 
 void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins) {
-    // A tile takes the smallest class that holds what is left of its sequence,
-    // or the largest there is.
+    // A sequence takes the smallest class that holds its rows, or the largest
+    // there is, with all of its tiles: a few rows that are left over run beside
+    // the others.
     auto class_of = [&](size_t rows) {
         int best = 0;
         for (int c = 0; c < kClasses; ++c)
@@ -36,29 +37,27 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
             }
         return best;
     };
-    // f(class, sequence, first row, positions) for each tile.
-    auto each_tile = [&](auto f) {
+    // f(sequence, first row, positions) for each tile of a class, in order.
+    auto each_tile = [&](int c, auto f) {
         for (uint32_t s = 0; s < head->n_seqs; ++s) {
             const size_t rows = seqs[s].n_new * shape.group;
-            for (size_t r = 0; r < rows;) {
-                const int c = class_of(rows - r);
+            if (rows == 0 || class_of(rows) != c) continue;
+            for (size_t r = 0; r < rows; r += kClassRows[c]) {
                 const size_t end = std::min(rows, r + kClassRows[c]);
-                f(c, s, (uint32_t)r, (size_t)seqs[s].context + (end - 1) / shape.group + 1);
-                r = end;
+                f(s, (uint32_t)r, (size_t)seqs[s].context + (end - 1) / shape.group + 1);
             }
         }
     };
-    size_t steps = 0;
-    each_tile([&](int, uint32_t, uint32_t, size_t len) { steps += (len + kStep - 1) / kStep; });
-    const size_t target = std::max<size_t>(1, kBlocks / shape.n_kv_heads);
-    const size_t most = std::max<size_t>(1, (steps + target - 1) / target);  // steps of an item
     uint32_t n_items = 0, part = 0;
     const uint32_t parts = (uint32_t)slabs_of(shape.head_dim);
     head->n_joins = head->join_rows = 0;
     for (int c = 0; c < kClasses; ++c) {
         head->first[c] = n_items;
-        each_tile([&](int of, uint32_t s, uint32_t row0, size_t len) {
-            if (of != c) return;
+        size_t steps = 0;
+        each_tile(c, [&](uint32_t, uint32_t, size_t len) { steps += (len + kStep - 1) / kStep; });
+        const size_t target = std::max<size_t>(1, kBlocks[c] / shape.n_kv_heads);
+        const size_t most = std::max<size_t>(1, (steps + target - 1) / target);  // steps of an item
+        each_tile(c, [&](uint32_t s, uint32_t row0, size_t len) {
             const size_t n = (len + kStep - 1) / kStep;
             size_t splits = (n + most - 1) / most;
             const uint32_t slabs = kClassRows[c] / 16, each = slabs * (uint32_t)shape.n_kv_heads;
@@ -72,6 +71,11 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
                 items[n_items++] = {s, row0, (uint32_t)k0, (uint32_t)k1, splits > 1 ? part : kNoPart};
                 if (splits > 1) part += each;
             }
+        });
+        // The longest first: blocks start in order, and short ones fill the end.
+        std::sort(items + head->first[c], items + n_items, [](const ItemAt &x, const ItemAt &y) {
+            const uint32_t m = x.k1 - x.k0, n = y.k1 - y.k0;
+            return m != n ? m > n : x.seq != y.seq ? x.seq < y.seq : x.row0 != y.row0 ? x.row0 < y.row0 : x.k0 < y.k0;
         });
     }
     head->first[kClasses] = n_items;
