@@ -36,15 +36,18 @@ struct SeqAt {
 // head of the group) [row0, row0 + the class's tile) of a sequence over its
 // positions [k0, k1), for each KV head. Where a tile's positions are split,
 // `part` is the first slab of its partials (kNoPart: none).
-constexpr int kClasses = 4;
-constexpr int kClassRows[kClasses] = {16, 64, 128, 256};
+constexpr int kClasses = 3;
+constexpr int kClassRows[kClasses] = {16, 128, 256};
 constexpr uint32_t kNoPart = 0xffffffffu;
+// With its sequence's fields, so that a block's chain of loads is one shorter.
 struct ItemAt {
-    uint32_t seq, row0, k0, k1, part;
+    SeqAt seq;
+    uint32_t row0, k0, k1, part;
 };
-// A split tile: `n_parts` items, each with `slabs` slabs for each KV head.
+// A split tile's rows, of the sequence at token0: `n_parts` items, each with
+// `slabs` slabs for each KV head.
 struct JoinAt {
-    uint32_t seq, row0, part, n_parts, slabs;
+    uint32_t token0, rows, row0, part, n_parts, slabs;
 };
 // A slab: the unnormalized results of 16 rows, then their maxima and sums.
 constexpr size_t slab_floats(size_t head_dim) { return 16 * (head_dim + 2); }

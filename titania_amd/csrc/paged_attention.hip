@@ -14,6 +14,13 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// A class's items: as they are set, or, of a captured launch, as the head says.
+struct Launch {
+    uint32_t first, n;
+    int cls;
+    bool captured;
+};
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFewThreads = 256;
 
@@ -69,7 +76,7 @@ __device__ __forceinline__ uint32_t seen16(const SeqAt &seq, const uint64_t *tre
     return ((bits << before) | ((1u << before) - 1)) & 0xffffu;
 }
 
-// Tiles of up to 16 R rows. Each of four waves takes 16 of every 64 positions
+// Tiles of up to 16 rows. Each of four waves takes 16 of every 64 positions
 // on its own, with no barrier before the end: keys and values go from memory
 // straight into the operands of v_mfma_f32_16x16x4_f32, whose products and
 // sums are those of f32, so nothing is converted or lost and any value counts
@@ -84,11 +91,12 @@ __device__ __forceinline__ uint32_t seen16(const SeqAt &seq, const uint64_t *tre
 // O^T = V^T P^T with positions 4 g + i at step i, for which the lane loads
 // those rows of V.
 //
-// A step's 64 products of 32 cycles take a wave 2048 cycles a row set, while
-// the block's 64 KB of f32 keys and values take a CU's share of HBM 8000: up to
-// 64 rows cost what one costs (32 with a bf16 cache).
-template <int HD, int R, typename KV>
-__global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a, int cls) {
+// A step's 64 products of 32 cycles take a wave 2048 cycles, while the block's
+// 64 KB of f32 keys and values take a CU's share of HBM 8000: 16 rows cost what
+// one costs. (With more sets of 16 a wave, 17 to 64 rows took 1.3 to 1.7 times
+// what the kernel for many rows takes for them.)
+template <int HD, typename KV>
+__global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a, Launch launch) {
     constexpr int VE = 16 / sizeof(KV);         // values of 16 bytes
     constexpr int KJ = HD / (4 * VE);           // 16-byte loads of a lane's part of a key
     constexpr int VV = VE <= HD / 16 ? VE : HD / 16;  // values of a load of a value row, which 16 lanes share
@@ -96,50 +104,42 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
     using VLoad = std::conditional_t<VV == VE, th_u32x4, u32x2>;
     constexpr int QS = HD + 4;                  // floats between rows of Q in LDS
     constexpr int kMerge = 4 * 16 * (HD + 4);   // the waves' results of 16 rows
-    constexpr int kLds = R * 16 * QS > kMerge ? R * 16 * QS : kMerge;
-    __shared__ __align__(16) float lds[kLds];
-    __shared__ float stat[4][16 * R][2];
+    __shared__ __align__(16) float lds[kMerge];  // Q's rows at first
+    __shared__ float stat[4][16][2];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t first = scalar_load(a.b.head->first, cls), n = (scalar_load(a.b.head->first, cls + 1) - first) * a.n_kv_heads;
+    uint32_t first = launch.first, n = launch.n;
+    if (launch.captured) {
+        first = scalar_load(a.b.head->first, launch.cls);
+        n = scalar_load(a.b.head->first, launch.cls + 1) - first;
+    }
+    n *= a.n_kv_heads;
     const float c2 = a.scale * kLog2e;
     for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
         const ItemAt it = scalar_load(a.b.items, first + at / a.n_kv_heads);
         const int kvh = at % a.n_kv_heads;
-        const SeqAt seq = scalar_load(a.b.seqs, it.seq);
-        const uint32_t rows = min((uint32_t)(16 * R), seq.n_new * a.group - it.row0);
+        const SeqAt &seq = it.seq;
+        const uint32_t rows = min(16u, seq.n_new * a.group - it.row0);
         const float *const qb = a.q + ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
         // Row `row` of the sequence, in q and out.
         auto row_at = [&](uint32_t row) { return ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
-        for (int i = threadIdx.x; i < 16 * R * (HD / 4); i += kFewThreads) {
+        for (int i = threadIdx.x; i < 16 * (HD / 4); i += kFewThreads) {
             const uint32_t r = i / (HD / 4), c = i % (HD / 4);  // rows past the last repeat it
             *reinterpret_cast<float4 *>(&lds[r * QS + 4 * c]) =
                 *reinterpret_cast<const float4 *>(qb + row_at(it.row0 + min(r, rows - 1)) + 4 * c);
         }
-        uint32_t token[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) token[r] = (it.row0 + min((uint32_t)(16 * r + m), rows - 1)) / a.group;
+        const uint32_t token = (it.row0 + min((uint32_t)m, rows - 1)) / a.group;
         __syncthreads();
-        // Q's operands: of one row set in registers, of more from LDS each time.
-        float qr[R == 1 ? KJ : 1][VE];
-        auto load_q = [&](int r, int j, float (&f)[VE]) {
+        float q[KJ][VE];
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
 #pragma unroll
             for (int e = 0; e < VE; e += 4)
-                *reinterpret_cast<float4 *>(&f[e]) =
-                    *reinterpret_cast<const float4 *>(&lds[(16 * r + m) * QS + j * 4 * VE + g * VE + e]);
-        };
-        if constexpr (R == 1)
+                *reinterpret_cast<float4 *>(&q[j][e]) = *reinterpret_cast<const float4 *>(&lds[m * QS + j * 4 * VE + g * VE + e]);
+        f32x4 o[HD / 16];
+        float mx = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) load_q(0, j, qr[j]);
-        f32x4 o[R][HD / 16];
-        float mx[R], l[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            mx[r] = -INFINITY;
-            l[r] = 0.f;
-#pragma unroll
-            for (int d = 0; d < HD / 16; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         const uint32_t *const pages = a.b.pages + seq.page0;
         const uint32_t mask = (1u << a.b.page_shift) - 1;
         // 16 positions from c on, a multiple of 16, lie in one page.
@@ -197,126 +197,102 @@ __global__ __launch_bounds__(kFewThreads, R == 1 && HD < 256 ? 2 : 1) void paged
                 }
                 odd = __ballot(here);
             }
+            f32x4 s{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (16u * r >= rows) break;
-                // One row set's operands and scores at a time.
-                if constexpr (R > 1) asm volatile("" ::: "memory");
-                f32x4 s{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < KJ; ++j)
 #pragma unroll
-                for (int j = 0; j < KJ; ++j) {
-                    float q[VE];
-                    if constexpr (R == 1) {
+                for (int e = 0; e < VE; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], q[j][e], s, 0, 0, 0);
+            float x[4], top = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) q[e] = qr[j][e];
-                    } else {
-                        load_q(r, j, q);
-                    }
+            for (int i = 0; i < 4; ++i) x[i] = s[i] * c2;
+            uint32_t seen = 0xffff;
+            if (partly) {
+                seen = seen16(seq, a.b.tree, token, c) & (it.k1 - c < 16 ? (1u << (it.k1 - c)) - 1 : 0xffffu);
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], q[e], s, 0, 0, 0);
-                }
-                float x[4], top = -INFINITY;
+                for (int i = 0; i < 4; ++i) x[i] = seen >> (4 * g + i) & 1 ? x[i] : -INFINITY;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = s[i] * c2;
-                uint32_t seen = 0xffff;
-                if (partly) {
-                    seen = seen16(seq, a.b.tree, token[r], c) & (it.k1 - c < 16 ? (1u << (it.k1 - c)) - 1 : 0xffffu);
+            for (int i = 0; i < 4; ++i) top = max_nn(top, x[i]);
+            top = max_nn(mx, rows_max_nn(top));
+            const float base = top == -INFINITY ? 0.f : top;
+            if (__any(top != mx)) {
+                const float alpha = __builtin_amdgcn_exp2f(mx - base);
+                l *= alpha;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = seen >> (4 * g + i) & 1 ? x[i] : -INFINITY;
-                }
+                for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
+                mx = top;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = max_nn(top, x[i]);
-                top = max_nn(mx[r], rows_max_nn(top));
-                const float base = top == -INFINITY ? 0.f : top;
-                if (__any(top != mx[r])) {
-                    const float alpha = __builtin_amdgcn_exp2f(mx[r] - base);
-                    l[r] *= alpha;
+            for (int i = 0; i < 4; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(x[i] - base);
+                l += s[i];
+            }
 #pragma unroll
-                    for (int d = 0; d < HD / 16; ++d) o[r][d] *= alpha;
-                    mx[r] = top;
-                }
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[i] = __builtin_amdgcn_exp2f(x[i] - base);
-                    l[r] += s[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int d = 0; d < HD / 16; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][d / VV][d % VV], s[i], o[d], 0, 0, 0);
+            // Values that are no numbers, which the products left out: for the
+            // rows that see them alone.
+            if (__builtin_expect(odd != 0, 0)) {
+#pragma unroll 1
+                for (int key = 0; key < 16 && c + key < it.k1; ++key) {
+                    if (!(odd >> (key & ~3) * 4 & 0xffff)) continue;
+                    const KV *vr = rows_of(page_of(c), c) + to_v + key * HD;
+                    const float mine = (key & 2) ? ((key & 1) ? s[3] : s[2]) : ((key & 1) ? s[1] : s[0]);
+                    const float p = __shfl(mine, (key >> 2) * 16 + m, 64);
+                    if (!(seen >> key & 1)) continue;
 #pragma unroll
                     for (int d = 0; d < HD / 16; ++d)
-                        o[r][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][d / VV][d % VV], s[i], o[r][d], 0, 0, 0);
-                // Values that are no numbers, which the products left out: for
-                // the rows that see them alone.
-                if (__builtin_expect(odd != 0, 0)) {
-#pragma unroll 1
-                    for (int key = 0; key < 16 && c + key < it.k1; ++key) {
-                        if (!(odd >> (key & ~3) * 4 & 0xffff)) continue;
-                        const KV *vr = rows_of(page_of(c), c) + to_v + key * HD;
-                        const float mine = (key & 2) ? ((key & 1) ? s[3] : s[2]) : ((key & 1) ? s[1] : s[0]);
-                        const float p = __shfl(mine, (key >> 2) * 16 + m, 64);
-                        if (!(seen >> key & 1)) continue;
 #pragma unroll
-                        for (int d = 0; d < HD / 16; ++d)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const KV w = vr[(d / VV) * 16 * VV + (4 * g + i) * VV + d % VV];
-                                const float f = sizeof(KV) == 4 ? (float)w : bf16_to_f32((uint16_t)w);
-                                if (!finite(f)) o[r][d][i] = fmaf(p, f, o[r][d][i]);
-                            }
-                    }
+                        for (int i = 0; i < 4; ++i) {
+                            const KV w = vr[(d / VV) * 16 * VV + (4 * g + i) * VV + d % VV];
+                            const float f = sizeof(KV) == 4 ? (float)w : bf16_to_f32((uint16_t)w);
+                            if (!finite(f)) o[d][i] = fmaf(p, f, o[d][i]);
+                        }
                 }
             }
         }
-        // The four waves' results: o[r][d][i] is dimension (d / VV) 16 VV +
+        // The four waves' results: o[d][i] is dimension (d / VV) 16 VV +
         // (4 g + i) VV + d % VV of row m.
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            l[r] = rows_sum(l[r]);
-            if (g == 0) {
-                stat[wave][16 * r + m][0] = mx[r];
-                stat[wave][16 * r + m][1] = l[r];
-            }
+        l = rows_sum(l);
+        if (g == 0) {
+            stat[wave][m][0] = mx;
+            stat[wave][m][1] = l;
         }
         __syncthreads();
+        float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (16u * r >= rows) break;
-            float top = -INFINITY;
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][m][0]);
+        const float f = mx == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mx - top);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][16 * r + m][0]);
-            const float f = mx[r] == -INFINITY ? (l[r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mx[r] - top);
+        for (int d = 0; d < HD / 16; d += 4)
 #pragma unroll
-            for (int d = 0; d < HD / 16; d += 4)
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(&lds[(wave * 16 + m) * QS + (d / VV) * 16 * VV + (4 * g + i) * VV + d % VV]) =
+                    make_float4(o[d][i] * f, o[d + 1][i] * f, o[d + 2][i] * f, o[d + 3][i] * f);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < rows * (HD / 4); i += kFewThreads) {
+            const uint32_t row = i / (HD / 4), col = 4 * (i % (HD / 4));
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            float ms = -INFINITY, ls = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float4 *>(
-                        &lds[(wave * 16 + m) * (HD + 4) + (d / VV) * 16 * VV + (4 * g + i) * VV + d % VV]) =
-                        make_float4(o[r][d][i] * f, o[r][d + 1][i] * f, o[r][d + 2][i] * f, o[r][d + 3][i] * f);
-            __syncthreads();
-            for (int i = threadIdx.x; i < 16 * (HD / 4); i += kFewThreads) {
-                const uint32_t row = i / (HD / 4), col = 4 * (i % (HD / 4));
-                if (16 * r + row >= rows) break;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                float ms = -INFINITY, ls = 0.f;
+            for (int w = 0; w < 4; ++w) ms = fmaxf(ms, stat[w][row][0]);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) ms = fmaxf(ms, stat[w][16 * r + row][0]);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float4 x = *reinterpret_cast<const float4 *>(&lds[(w * 16 + row) * (HD + 4) + col]);
-                    sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
-                    const float mw = stat[w][16 * r + row][0], lw = stat[w][16 * r + row][1];
-                    ls += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - ms);
-                }
-                if (it.part == kNoPart) {
-                    float *dst = a.out + ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD + row_at(it.row0 + 16 * r + row);
-                    *reinterpret_cast<float4 *>(dst + col) = make_float4(sum.x / ls, sum.y / ls, sum.z / ls, sum.w / ls);
-                } else {
-                    float *slab = a.part + (size_t)(it.part + kvh * R + r) * slab_floats(HD);
-                    *reinterpret_cast<float4 *>(slab + row * HD + col) = sum;
-                    if (col == 0) *reinterpret_cast<float2 *>(slab + 16 * HD + 2 * row) = make_float2(ms, ls);
-                }
+            for (int w = 0; w < 4; ++w) {
+                const float4 x = *reinterpret_cast<const float4 *>(&lds[(w * 16 + row) * QS + col]);
+                sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+                const float mw = stat[w][row][0], lw = stat[w][row][1];
+                ls += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f(mw - ms);
             }
-            __syncthreads();
+            if (it.part == kNoPart) {
+                float *dst = a.out + ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD + row_at(it.row0 + row);
+                *reinterpret_cast<float4 *>(dst + col) = make_float4(sum.x / ls, sum.y / ls, sum.z / ls, sum.w / ls);
+            } else {
+                float *slab = a.part + (size_t)(it.part + kvh) * slab_floats(HD);
+                *reinterpret_cast<float4 *>(slab + row * HD + col) = sum;
+                if (col == 0) *reinterpret_cast<float2 *>(slab + 16 * HD + 2 * row) = make_float2(ms, ls);
+            }
         }
         __syncthreads();  // lds and stat are written again
     }
@@ -408,7 +384,7 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // summed from memory in f32, a position at a time, by each row for itself:
 // what it does not see does not reach it.
 template <int HD, int SETS, typename KV>
-__global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnArgs a, int cls) {
+__global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnArgs a, Launch launch) {
     constexpr bool F32 = sizeof(KV) == 4;
     constexpr int KT = kManyKeys, RW = 16 * SETS;
     constexpr float kGrow = 5.f, kBase = 10.f;  // weights below 2^15
@@ -423,12 +399,17 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
     __shared__ uint32_t odd_of[4];
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t first = scalar_load(a.b.head->first, cls), n = (scalar_load(a.b.head->first, cls + 1) - first) * a.n_kv_heads;
+    uint32_t first = launch.first, n = launch.n;
+    if (launch.captured) {
+        first = scalar_load(a.b.head->first, launch.cls);
+        n = scalar_load(a.b.head->first, launch.cls + 1) - first;
+    }
+    n *= a.n_kv_heads;
     const float c2 = a.scale * kLog2e;
     for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
         const ItemAt it = scalar_load(a.b.items, first + at / a.n_kv_heads);
         const int kvh = at % a.n_kv_heads;
-        const SeqAt seq = scalar_load(a.b.seqs, it.seq);
+        const SeqAt &seq = it.seq;
         const uint32_t rows = min((uint32_t)(8 * RW), seq.n_new * a.group - it.row0);
         const size_t qbase = ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
         auto row_at = [&](uint32_t row) { return qbase + ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
@@ -881,8 +862,7 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, const BatchHea
     // gridDim.y walks the tiles, gridDim.x their rows, for each KV head.
     for (uint32_t j = blockIdx.y; j < head.n_joins; j += gridDim.y) {
         const JoinAt join = scalar_load(a.b.joins, j);
-        const SeqAt seq = scalar_load(a.b.seqs, join.seq);
-        const uint32_t rows = min(16 * join.slabs, seq.n_new * a.group - join.row0);
+        const uint32_t rows = join.rows;
         for (uint32_t i = blockIdx.x * ROWS + (W == 1 ? wave : 0); i < rows * a.n_kv_heads; i += gridDim.x * ROWS) {
             const uint32_t row = i % rows, kvh = i / rows;
             const float *part = a.part + (size_t)(join.part + kvh * join.slabs + row / 16) * slab_floats(HD);
@@ -914,7 +894,7 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, const BatchHea
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e]);
             }
             const uint32_t r = join.row0 + row;
-            float *out = a.out + ((size_t)(seq.token0 + r / a.group) * a.n_heads + (size_t)kvh * a.group + r % a.group) * HD;
+            float *out = a.out + ((size_t)(join.token0 + r / a.group) * a.n_heads + (size_t)kvh * a.group + r % a.group) * HD;
             if constexpr (W == 1) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) out[E * lane + e] = acc[e] / l;
@@ -947,32 +927,32 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 // A captured launch's grid, whatever is set later: its blocks walk the items.
 constexpr unsigned kCapturedBlocks = 1024;
 
-template <int HD, int R>
-hipError_t few(hipStream_t s, const PagedAttnArgs &a, int cls, unsigned grid, bool bf16) {
-    if (bf16) paged_few_kernel<HD, R, uint16_t><<<grid, kFewThreads, 0, s>>>(a, cls);
-    else paged_few_kernel<HD, R, float><<<grid, kFewThreads, 0, s>>>(a, cls);
+template <int HD>
+hipError_t few(hipStream_t s, const PagedAttnArgs &a, const Launch &l, unsigned grid, bool bf16) {
+    if (bf16) paged_few_kernel<HD, uint16_t><<<grid, kFewThreads, 0, s>>>(a, l);
+    else paged_few_kernel<HD, float><<<grid, kFewThreads, 0, s>>>(a, l);
     return hipGetLastError();
 }
 
 template <int HD, int SETS>
-hipError_t many(hipStream_t s, const PagedAttnArgs &a, int cls, unsigned grid, bool bf16) {
-    if (bf16) paged_many_kernel<HD, SETS, uint16_t><<<grid, kManyThreads, 0, s>>>(a, cls);
-    else paged_many_kernel<HD, SETS, float><<<grid, kManyThreads, 0, s>>>(a, cls);
+hipError_t many(hipStream_t s, const PagedAttnArgs &a, const Launch &l, unsigned grid, bool bf16) {
+    if (bf16) paged_many_kernel<HD, SETS, uint16_t><<<grid, kManyThreads, 0, s>>>(a, l);
+    else paged_many_kernel<HD, SETS, float><<<grid, kManyThreads, 0, s>>>(a, l);
     return hipGetLastError();
 }
 
 template <int HD>
 hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, bool bf16, bool captured) {
     for (int c = 0; c < kClasses; ++c) {
-        const size_t items = (size_t)(count.first[c + 1] - count.first[c]) * a.n_kv_heads;
-        if (!items && !(captured && c == 0)) continue;
-        const unsigned grid = captured ? kCapturedBlocks : (unsigned)std::min<size_t>(items, 0x7fffffu);
+        const Launch l{count.first[c], count.first[c + 1] - count.first[c], c, captured};
+        const size_t blocks = (size_t)l.n * a.n_kv_heads;
+        if (!blocks && !(captured && c == 0)) continue;
+        const unsigned grid = captured ? kCapturedBlocks : (unsigned)std::min<size_t>(blocks, 0x7fffffu);
         hipError_t e = hipSuccess;
-        if (c == 0) e = few<HD, 1>(s, a, c, grid, bf16);
+        if (c == 0) e = few<HD>(s, a, l, grid, bf16);
         if constexpr (HD < 256) {
-            if (c == 1) e = few<HD, 4>(s, a, c, grid, bf16);
-            if (c == 2) e = many<HD, 1>(s, a, c, grid, bf16);
-            if (c == 3) e = many<HD, 2>(s, a, c, grid, bf16);
+            if (c == 1) e = many<HD, 1>(s, a, l, grid, bf16);
+            if (c == 2) e = many<HD, 2>(s, a, l, grid, bf16);
         }
         if (e != hipSuccess) return e;
     }

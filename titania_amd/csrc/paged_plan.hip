@@ -8,9 +8,14 @@ namespace th {
 
 namespace {
 
-// The blocks that a class's positions are split for, where they allow: what the
-// chip holds of them at once.
-constexpr size_t kBlocks[kClasses] = {512, 256, 256, 256};
+// What the chip holds of a class's blocks at once.
+constexpr size_t kSlots[kClasses] = {512, 256, 256};
+// An estimate of a block's time in us: for each 64 positions, and for the rest of it.
+constexpr double kStepUs[kClasses] = {5.0, 3.5, 6.0}, kBlockUs[kClasses] = {5.0, 8.0, 10.0};
+// Of the second launch that joins split tiles.
+constexpr double kJoinUs = 5.0;
+// The most rounds of blocks that a class is split into.
+constexpr size_t kRounds = 4;
 // A block's fewest positions: one step of its waves.
 constexpr size_t kStep = 64;
 
@@ -21,7 +26,7 @@ size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max
 }
 
 size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens) {
-    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kBlocks[0] + kBlocks[1] + kBlocks[2] + kBlocks[3];
+    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kRounds * (kSlots[0] + kSlots[1] + kSlots[2]);
 }
 
 void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins) {
@@ -53,29 +58,62 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
     head->n_joins = head->join_rows = 0;
     for (int c = 0; c < kClasses; ++c) {
         head->first[c] = n_items;
-        size_t steps = 0;
-        each_tile(c, [&](uint32_t, uint32_t, size_t len) { steps += (len + kStep - 1) / kStep; });
-        const size_t target = std::max<size_t>(1, kBlocks[c] / shape.n_kv_heads);
-        const size_t most = std::max<size_t>(1, (steps + target - 1) / target);  // steps of an item
+        size_t steps = 0, tiles = 0, longest = 0;
+        each_tile(c, [&](uint32_t, uint32_t, size_t len) {
+            const size_t n = (len + kStep - 1) / kStep;
+            steps += n;
+            ++tiles;
+            longest = std::max(longest, n);
+        });
+        if (!tiles) continue;
+        // The most steps of an item: as they are, in ceil(blocks / slots)
+        // rounds or what the longest first leaves of them, or such that the
+        // blocks fill 1 to kRounds rounds.
+        auto items_at = [&](size_t most) {
+            size_t items = 0;
+            each_tile(c, [&](uint32_t, uint32_t, size_t len) { items += ((len + kStep - 1) / kStep + most - 1) / most; });
+            return items;
+        };
+        const double slots = (double)kSlots[c] / shape.n_kv_heads;  // of items
+        size_t most = longest;
+        double best = std::max((double)longest, steps / slots) * kStepUs[c] + std::max(1.0, tiles / slots) * kBlockUs[c];
+        for (size_t r = 1; r <= kRounds; ++r) {
+            const size_t room = std::max<size_t>(1, (size_t)(r * slots));
+            if (room <= tiles) continue;
+            size_t low = std::max<size_t>(1, (steps + room - 1) / room), high = longest;
+            while (low < high) {
+                const size_t mid = (low + high) / 2;
+                if (items_at(mid) <= room) high = mid;
+                else low = mid + 1;
+            }
+            const double us = r * (low * kStepUs[c] + kBlockUs[c]) + (low < longest ? kJoinUs : 0);
+            if (us < best) {
+                best = us;
+                most = low;
+            }
+        }
         each_tile(c, [&](uint32_t s, uint32_t row0, size_t len) {
             const size_t n = (len + kStep - 1) / kStep;
             size_t splits = (n + most - 1) / most;
             const uint32_t slabs = kClassRows[c] / 16, each = slabs * (uint32_t)shape.n_kv_heads;
             if (splits * each > parts - part || head->n_joins == shape.max_joins) splits = 1;
             if (splits > 1) {
-                joins[head->n_joins++] = {s, row0, part, (uint32_t)splits, slabs};
-                head->join_rows = std::max(head->join_rows, std::min<uint32_t>(kClassRows[c], seqs[s].n_new * shape.group - row0));
+                const uint32_t rows = std::min<uint32_t>(kClassRows[c], seqs[s].n_new * shape.group - row0);
+                joins[head->n_joins++] = {seqs[s].token0, rows, row0, part, (uint32_t)splits, slabs};
+                head->join_rows = std::max(head->join_rows, rows);
             }
             for (size_t i = 0; i < splits; ++i) {
                 const size_t k0 = i * n / splits * kStep, k1 = std::min(len, (i + 1) * n / splits * kStep);
-                items[n_items++] = {s, row0, (uint32_t)k0, (uint32_t)k1, splits > 1 ? part : kNoPart};
+                items[n_items++] = {seqs[s], row0, (uint32_t)k0, (uint32_t)k1, splits > 1 ? part : kNoPart};
                 if (splits > 1) part += each;
             }
         });
         // The longest first: blocks start in order, and short ones fill the end.
         std::sort(items + head->first[c], items + n_items, [](const ItemAt &x, const ItemAt &y) {
             const uint32_t m = x.k1 - x.k0, n = y.k1 - y.k0;
-            return m != n ? m > n : x.seq != y.seq ? x.seq < y.seq : x.row0 != y.row0 ? x.row0 < y.row0 : x.k0 < y.k0;
+            return m != n ? m > n : x.seq.token0 != y.seq.token0 ? x.seq.token0 < y.seq.token0
+                            : x.row0 != y.row0   ? x.row0 < y.row0
+                                                 : x.k0 < y.k0;
         });
     }
     head->first[kClasses] = n_items;
