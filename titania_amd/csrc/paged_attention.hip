@@ -102,9 +102,9 @@ __global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kerne
     constexpr int VV = VE <= HD / 16 ? VE : HD / 16;  // values of a load of a value row, which 16 lanes share
     constexpr int VJ = HD / (16 * VV);          // such loads
     using VLoad = std::conditional_t<VV == VE, th_u32x4, u32x2>;
-    constexpr int QS = HD + 4;                  // floats between rows of Q in LDS
+    constexpr int QS = HD + 4;                  // floats between rows in LDS
     constexpr int kMerge = 4 * 16 * (HD + 4);   // the waves' results of 16 rows
-    __shared__ __align__(16) float lds[kMerge];  // Q's rows at first
+    __shared__ __align__(16) float lds[kMerge];
     __shared__ float stat[4][16][2];
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,23 +123,18 @@ __global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kerne
         const float *const qb = a.q + ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
         // Row `row` of the sequence, in q and out.
         auto row_at = [&](uint32_t row) { return ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
-        for (int i = threadIdx.x; i < 16 * (HD / 4); i += kFewThreads) {
-            const uint32_t r = i / (HD / 4), c = i % (HD / 4);  // rows past the last repeat it
-            *reinterpret_cast<float4 *>(&lds[r * QS + 4 * c]) =
-                *reinterpret_cast<const float4 *>(qb + row_at(it.row0 + min(r, rows - 1)) + 4 * c);
-        }
-        const uint32_t token = (it.row0 + min((uint32_t)m, rows - 1)) / a.group;
-        __syncthreads();
+        // Rows past the last repeat it. (Through LDS, to be read from memory once a
+        // block, they would wait for each other's loads.)
+        const uint32_t own = it.row0 + min((uint32_t)m, rows - 1), token = own / a.group;
         float q[KJ][VE];
+        {
+            const float *const qr = qb + row_at(own) + g * VE;
 #pragma unroll
-        for (int j = 0; j < KJ; ++j)
+            for (int j = 0; j < KJ; ++j)
 #pragma unroll
-            for (int e = 0; e < VE; e += 4)
-                *reinterpret_cast<float4 *>(&q[j][e]) = *reinterpret_cast<const float4 *>(&lds[m * QS + j * 4 * VE + g * VE + e]);
-        f32x4 o[HD / 16];
-        float mx = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int e = 0; e < VE; e += 4)
+                    *reinterpret_cast<float4 *>(&q[j][e]) = *reinterpret_cast<const float4 *>(qr + j * 4 * VE + e);
+        }
         const uint32_t *const pages = a.b.pages + seq.page0;
         const uint32_t mask = (1u << a.b.page_shift) - 1;
         // 16 positions from c on, a multiple of 16, lie in one page.
@@ -166,6 +161,10 @@ __global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kerne
             fetch(page_of(c), c);
             next = page_of(c + 64);
         }
+        f32x4 o[HD / 16];
+        float mx = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (; c < it.k1; c += 64) {
             float kf[KJ][VE], vf[4][VJ][VV];
 #pragma unroll
