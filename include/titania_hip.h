@@ -255,12 +255,12 @@ TH_API int th_paged_read(th_device *dev, const th_paged *cache, size_t page, flo
 TH_API int th_paged_write(th_device *dev, th_paged *cache, size_t page, const float *k, const float *v);
 
 /* A step's sequences and their new tokens, for the calls of all layers (whose
- * caches have one shape). A token's activations lie at its place in the batch:
+ * caches have one shape and type). A token's activations lie at its place in the batch:
  * first the tokens of sequence 0, then those of sequence 1, and so on. */
 typedef struct th_batch th_batch;
 /* Room for max_seqs sequences (at most 65536) with max_tokens new tokens in
  * all (max_tokens * n_heads <= 2^24) and max_pages entries of pages (at most
- * 2^26), over caches of the shape of `cache`; n_heads: query heads, 1 to 16 for
+ * 2^26), over caches of the shape and type of `cache`; n_heads: query heads, 1 to 16 for
  * each KV head. Nothing is set. A batch belongs to `dev`: calls with another
  * device refuse it. */
 TH_API int th_batch_alloc(th_device *dev, const th_paged *cache, size_t n_heads, size_t max_seqs, size_t max_tokens,
@@ -313,7 +313,7 @@ TH_API int th_batch_accept(th_device *dev, const th_batch *batch, const th_buffe
                            uint32_t *picks, uint32_t *n_kept, int32_t *kept);
 /* The keys and values of the tokens kept (rising places, as th_batch_accept
  * gives them, or any other verification), moved up behind the context in each
- * of the caches, different ones of one type: that of the j-th goes from
+ * of the caches, which differ from each other: that of the j-th goes from
  * position context[s] + kept[..] to context[s] + j. The context of the next
  * step is then context[s] + n_kept[s]. Refused while capturing. */
 TH_API int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, const th_batch *batch,

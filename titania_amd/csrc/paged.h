@@ -71,9 +71,12 @@ struct BatchView {
     int page_shift;
 };
 
+// The most blocks that a class's splits come to: four rounds of 512.
+constexpr size_t kMostSplitBlocks = 2048;
 // What a plan may hold, and what it is made for.
 struct PlanShape {
     size_t n_kv_heads, head_dim, group, max_items, max_joins;
+    bool bf16;
     unsigned classes;  // a bit for each class that may be used: the first always
 };
 // The most items and split tiles of a batch.
@@ -139,3 +142,48 @@ struct Upload {
 hipError_t launch_upload(hipStream_t s, const Upload &u);
 
 }  // namespace th
+
+// A step's sequences. The arrays exist twice: in pinned host memory, where
+// th_batch_set writes them, and on the device, where one launch copies what is
+// in use. Their places never change, so that a captured call reads what was
+// set last.
+struct th_batch {
+    // What its caches are.
+    size_t pages = 0, page_len = 0, n_kv_heads = 0, head_dim = 0;
+    int kv_dtype = TH_KV_F32;
+    const th_device *dev = nullptr;  // whose stream it is copied on
+    int page_shift = 0;
+    size_t n_heads = 0, max_seqs = 0, max_tokens = 0, max_pages = 0;
+    // Of what is set: sequences, tokens, entries of pages, the positions that a
+    // rotation's table holds at least.
+    size_t n_seqs = 0, n_tokens = 0, n_pages = 0, positions = 0;
+    // The fewest tokens that a captured call was launched for.
+    size_t captured_tokens = SIZE_MAX;
+    // The classes of the attention's items that every captured call launches.
+    unsigned classes = (1u << th::kClasses) - 1;
+    char *device = nullptr, *pinned = nullptr;
+    // Offsets, the same in both.
+    size_t at_seqs = 0, at_tokens = 0, at_pages = 0, at_tree = 0, at_items = 0, at_joins = 0;
+    hipEvent_t copied = nullptr;  // the pinned memory has been read
+    int32_t *parents = nullptr;   // [max_tokens], -1: the context
+    uint32_t *stamp = nullptr;    // [pages]: the last set() that wrote to a page
+    uint32_t epoch = 0;
+
+    th::BatchHead *head() const { return reinterpret_cast<th::BatchHead *>(pinned); }
+    th::SeqAt *seqs() const { return reinterpret_cast<th::SeqAt *>(pinned + at_seqs); }
+    uint32_t *page_list() const { return reinterpret_cast<uint32_t *>(pinned + at_pages); }
+    th::PlanShape plan_shape() const {
+        return {n_kv_heads, head_dim, n_heads / n_kv_heads, th::most_items(n_heads, n_kv_heads, max_seqs, max_tokens),
+                th::most_joins(n_heads, n_kv_heads, max_seqs, max_tokens), kv_dtype == TH_KV_BF16, classes};
+    }
+    th::BatchView view() const {
+        return {reinterpret_cast<const th::BatchHead *>(device),
+                reinterpret_cast<const th::SeqAt *>(device + at_seqs),
+                reinterpret_cast<const th::TokenAt *>(device + at_tokens),
+                reinterpret_cast<const uint32_t *>(device + at_pages),
+                reinterpret_cast<const uint64_t *>(device + at_tree),
+                reinterpret_cast<const th::ItemAt *>(device + at_items),
+                reinterpret_cast<const th::JoinAt *>(device + at_joins),
+                page_shift};
+    }
+};

@@ -5,54 +5,10 @@
 #include <cstring>
 #include <new>
 
-#include "device_util.h"
+#include "../../include/titania_hip_test_paged.h"
 #include "paged.h"
 
 using th::fail;
-
-// A step's sequences. The arrays exist twice: in pinned host memory, where
-// th_batch_set writes them, and on the device, where one launch copies what is
-// in use. Their places never change, so that a captured call reads what was
-// set last.
-struct th_batch {
-    // What its caches are.
-    size_t pages = 0, page_len = 0, n_kv_heads = 0, head_dim = 0;
-    const th_device *dev = nullptr;  // whose stream it is copied on
-    int page_shift = 0;
-    size_t n_heads = 0, max_seqs = 0, max_tokens = 0, max_pages = 0;
-    // Of what is set: sequences, tokens, entries of pages, the positions that a
-    // rotation's table holds at least.
-    size_t n_seqs = 0, n_tokens = 0, n_pages = 0, positions = 0;
-    // The fewest tokens that a captured call was launched for.
-    size_t captured_tokens = SIZE_MAX;
-    // The classes of the attention's items that every captured call launches.
-    unsigned classes = (1u << th::kClasses) - 1;
-    char *device = nullptr, *pinned = nullptr;
-    // Offsets, the same in both.
-    size_t at_seqs = 0, at_tokens = 0, at_pages = 0, at_tree = 0, at_items = 0, at_joins = 0;
-    hipEvent_t copied = nullptr;  // the pinned memory has been read
-    int32_t *parents = nullptr;   // [max_tokens], -1: the context
-    uint32_t *stamp = nullptr;    // [pages]: the last set() that wrote to a page
-    uint32_t epoch = 0;
-
-    th::BatchHead *head() const { return reinterpret_cast<th::BatchHead *>(pinned); }
-    th::SeqAt *seqs() const { return reinterpret_cast<th::SeqAt *>(pinned + at_seqs); }
-    uint32_t *page_list() const { return reinterpret_cast<uint32_t *>(pinned + at_pages); }
-    th::PlanShape plan_shape() const {
-        return {n_kv_heads, head_dim, n_heads / n_kv_heads, th::most_items(n_heads, n_kv_heads, max_seqs, max_tokens),
-                th::most_joins(n_heads, n_kv_heads, max_seqs, max_tokens), classes};
-    }
-    th::BatchView view() const {
-        return {reinterpret_cast<const th::BatchHead *>(device),
-                reinterpret_cast<const th::SeqAt *>(device + at_seqs),
-                reinterpret_cast<const th::TokenAt *>(device + at_tokens),
-                reinterpret_cast<const uint32_t *>(device + at_pages),
-                reinterpret_cast<const uint64_t *>(device + at_tree),
-                reinterpret_cast<const th::ItemAt *>(device + at_items),
-                reinterpret_cast<const th::JoinAt *>(device + at_joins),
-                page_shift};
-    }
-};
 
 namespace {
 
@@ -108,10 +64,137 @@ int same_cache(const th_device *dev, const th_paged *c, const th_batch *b) {
     TH_PAGED_HERE(dev, c);
     TH_BATCH_OF(dev, b);
     TH_REQUIRE(c->pages == b->pages && c->page_len == b->page_len && c->n_kv_heads == b->n_kv_heads &&
-                   c->head_dim == b->head_dim,
-               "a cache of %zu pages of %zu positions of %zu x %zu, a batch for %zu of %zu of %zu x %zu", c->pages,
-               c->page_len, c->n_kv_heads, c->head_dim, b->pages, b->page_len, b->n_kv_heads, b->head_dim);
+                   c->head_dim == b->head_dim && c->kv_dtype == b->kv_dtype,
+               "a cache of %zu pages of %zu positions of %zu x %zu in type %d, a batch for %zu of %zu of %zu x %zu in type %d",
+               c->pages, c->page_len, c->n_kv_heads, c->head_dim, c->kv_dtype, b->pages, b->page_len, b->n_kv_heads, b->head_dim,
+               b->kv_dtype);
     return TH_OK;
+}
+
+// Whether a batch can be set to this. Changes nothing but the stamps.
+int check_set(th_batch *b, size_t n_seqs, const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
+              const int32_t *parents) {
+    TH_REQUIRE(n_seqs == 0 || (context && n_new), "th_batch_set: null argument");
+    TH_REQUIRE(n_pages == 0 || pages, "th_batch_set: null pages");
+    TH_REQUIRE(n_seqs <= b->max_seqs, "%zu sequences, a batch of at most %zu", n_seqs, b->max_seqs);
+    TH_REQUIRE(n_pages <= b->max_pages, "%zu pages, a batch of at most %zu", n_pages, b->max_pages);
+    // Everything is checked before anything is changed.
+    size_t tokens = 0, entries = 0;
+    const size_t L = b->page_len;
+    for (size_t s = 0; s < n_seqs; ++s) {
+        const size_t len = (size_t)context[s] + n_new[s];
+        entries += (len + L - 1) / L;
+        tokens += n_new[s];
+        TH_REQUIRE(entries <= n_pages, "sequence %zu of %zu positions is past the end of %zu pages", s, len, n_pages);
+        TH_REQUIRE(tokens <= b->max_tokens, "%zu tokens up to sequence %zu, a batch of at most %zu", tokens, s, b->max_tokens);
+    }
+    TH_REQUIRE(entries == n_pages, "%zu pages for sequences of %zu", n_pages, entries);
+    TH_REQUIRE(tokens <= b->captured_tokens,
+               "%zu tokens: a graph was captured with this batch at %zu, and its launches take no more", tokens,
+               b->captured_tokens);
+    for (size_t i = 0; i < n_pages; ++i)
+        TH_REQUIRE(pages[i] < b->pages, "page %u at index %zu of a cache of %zu", pages[i], i, b->pages);
+    // A page that gets new rows is in no other place of a sequence with tokens.
+    if (++b->epoch == 0) {
+        memset(b->stamp, 0, b->pages * sizeof(uint32_t));
+        b->epoch = 1;
+    }
+    for (size_t s = 0, p0 = 0; s < n_seqs; ++s) {
+        const size_t len = (size_t)context[s] + n_new[s], end = p0 + (len + L - 1) / L;
+        for (size_t p = p0 + context[s] / L; n_new[s] && p < end; ++p) {
+            TH_REQUIRE(b->stamp[pages[p]] != b->epoch, "page %u gets new rows in two places, one of them of sequence %zu",
+                       pages[p], s);
+            b->stamp[pages[p]] = b->epoch;
+        }
+        p0 = end;
+    }
+    for (size_t s = 0, p0 = 0; s < n_seqs; ++s) {
+        const size_t len = (size_t)context[s] + n_new[s], end = p0 + (len + L - 1) / L;
+        for (size_t p = p0; n_new[s] && p < p0 + context[s] / L; ++p)
+            TH_REQUIRE(b->stamp[pages[p]] != b->epoch, "page %u gets new rows, and is in the context of sequence %zu", pages[p], s);
+        p0 = end;
+    }
+    for (size_t s = 0, t0 = 0; parents && s < n_seqs; t0 += n_new[s++]) {
+        bool chain = true;
+        for (size_t i = 0; i < n_new[s]; ++i) {
+            TH_REQUIRE(parents[t0 + i] >= -1 && parents[t0 + i] < (int64_t)i, "parent %d of token %zu of sequence %zu",
+                       parents[t0 + i], i, s);
+            chain = chain && parents[t0 + i] == (int64_t)i - 1;
+        }
+        TH_REQUIRE(chain || n_new[s] <= th::kTreeTokens, "a tree of %u tokens: at most %zu", n_new[s], th::kTreeTokens);
+    }
+    return TH_OK;
+}
+
+// Its arrays in pinned memory. Returns the tokens up to the end of the last tree.
+size_t lay_out(th_batch *b, size_t n_seqs, const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
+               const int32_t *parents) {
+    const size_t L = b->page_len;
+    size_t tokens = 0;
+    for (size_t s = 0; s < n_seqs; ++s) tokens += n_new[s];
+    auto *head = b->head();
+    auto *seqs = b->seqs();
+    auto *toks = reinterpret_cast<th::TokenAt *>(b->pinned + b->at_tokens);
+    auto *tree = reinterpret_cast<uint64_t *>(b->pinned + b->at_tree);
+    head->n_seqs = (uint32_t)n_seqs;
+    head->n_tokens = (uint32_t)tokens;
+    if (n_pages) memcpy(b->page_list(), pages, n_pages * sizeof(uint32_t));
+    size_t positions = 0, t0 = 0, p0 = 0, trees = 0;
+    for (size_t s = 0; s < n_seqs; ++s) {
+        const uint32_t n = n_new[s], ctx = context[s];
+        int32_t *par = b->parents + t0;
+        bool chain = true;
+        for (uint32_t i = 0; i < n; ++i) {
+            par[i] = parents ? parents[t0 + i] : (int32_t)i - 1;
+            chain = chain && par[i] == (int32_t)i - 1;
+        }
+        seqs[s] = {(uint32_t)t0, n, ctx, (uint32_t)p0, !chain};
+        for (uint32_t i = 0; i < n; ++i) {
+            const size_t at = (size_t)ctx + i;
+            th::TokenAt &t = toks[t0 + i];
+            t.slot = pages[p0 + at / L] << b->page_shift | (uint32_t)(at & (L - 1));
+            t.pos = par[i] < 0 ? ctx : toks[t0 + par[i]].pos + 1;
+            t.seq = (uint32_t)s;
+            t.index = i;
+            positions = std::max<size_t>(positions, (size_t)t.pos + 1);
+            if (chain) continue;
+            uint64_t *bits = tree + (t0 + i) * th::kTreeWords;
+            for (int w = 0; w < th::kTreeWords; ++w) bits[w] = par[i] < 0 ? 0 : tree[(t0 + par[i]) * th::kTreeWords + w];
+            bits[i / 64] |= (uint64_t)1 << (i & 63);
+        }
+        if (!chain) trees = t0 + n;
+        t0 += n;
+        p0 += ((size_t)ctx + n + L - 1) / L;
+    }
+    b->n_seqs = n_seqs;
+    b->n_tokens = tokens;
+    b->n_pages = n_pages;
+    b->positions = positions;
+    auto *items = reinterpret_cast<th::ItemAt *>(b->pinned + b->at_items);
+    auto *joins = reinterpret_cast<th::JoinAt *>(b->pinned + b->at_joins);
+    th::plan_attention(b->plan_shape(), seqs, head, items, joins);
+    return trees;
+}
+
+// A batch's offsets, and its host memory but for the pinned. False: there is none.
+bool place_arrays(th_batch *b, size_t *bytes) {
+    size_t at = 64;
+    auto place = [&at](size_t n) {
+        const size_t here = at;
+        at += (n + 63) / 64 * 64;
+        return here;
+    };
+    b->page_shift = __builtin_ctzll(b->page_len);
+    b->at_seqs = place(b->max_seqs * sizeof(th::SeqAt));
+    b->at_tokens = place(b->max_tokens * sizeof(th::TokenAt));
+    b->at_pages = place(b->max_pages * sizeof(uint32_t));
+    b->at_tree = place(b->max_tokens * th::kTreeWords * sizeof(uint64_t));
+    b->at_items = place(b->plan_shape().max_items * sizeof(th::ItemAt));
+    b->at_joins = place(b->plan_shape().max_joins * sizeof(th::JoinAt));
+    *bytes = at;
+    b->parents = static_cast<int32_t *>(malloc(b->max_tokens * sizeof(int32_t)));
+    b->stamp = static_cast<uint32_t *>(calloc(b->pages, sizeof(uint32_t)));
+    return b->parents && b->stamp;
 }
 
 // A captured call is launched for the tokens that are set now: later sets may
@@ -247,29 +330,16 @@ int th_batch_alloc(th_device *dev, const th_paged *c, size_t n_heads, size_t max
     if (!b) return fail(TH_ERR_NOMEM, "out of host memory");
     b->pages = c->pages;
     b->page_len = c->page_len;
-    b->page_shift = __builtin_ctzll(c->page_len);
     b->n_kv_heads = c->n_kv_heads;
     b->head_dim = c->head_dim;
+    b->kv_dtype = c->kv_dtype;
     b->dev = dev;
     b->n_heads = n_heads;
     b->max_seqs = max_seqs;
     b->max_tokens = max_tokens;
     b->max_pages = max_pages;
-    size_t at = 64;
-    auto place = [&at](size_t bytes) {
-        const size_t here = at;
-        at += (bytes + 63) / 64 * 64;
-        return here;
-    };
-    b->at_seqs = place(max_seqs * sizeof(th::SeqAt));
-    b->at_tokens = place(max_tokens * sizeof(th::TokenAt));
-    b->at_pages = place(max_pages * sizeof(uint32_t));
-    b->at_tree = place(max_tokens * th::kTreeWords * sizeof(uint64_t));
-    b->at_items = place(th::most_items(n_heads, c->n_kv_heads, max_seqs, max_tokens) * sizeof(th::ItemAt));
-    b->at_joins = place(th::most_joins(n_heads, c->n_kv_heads, max_seqs, max_tokens) * sizeof(th::JoinAt));
-    b->parents = static_cast<int32_t *>(malloc(max_tokens * sizeof(int32_t)));
-    b->stamp = static_cast<uint32_t *>(calloc(c->pages, sizeof(uint32_t)));
-    if (!b->parents || !b->stamp) {
+    size_t at = 0;
+    if (!place_arrays(b, &at)) {
         th_batch_free(nullptr, b);
         return fail(TH_ERR_NOMEM, "out of host memory");
     }
@@ -292,98 +362,11 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     TH_REQUIRE(dev && b, "th_batch_set: null argument");
     TH_NOT_CAPTURING(dev, "th_batch_set");
     TH_BATCH_OF(dev, b);
-    TH_REQUIRE(n_seqs == 0 || (context && n_new), "th_batch_set: null argument");
-    TH_REQUIRE(n_pages == 0 || pages, "th_batch_set: null pages");
-    TH_REQUIRE(n_seqs <= b->max_seqs, "%zu sequences, a batch of at most %zu", n_seqs, b->max_seqs);
-    TH_REQUIRE(n_pages <= b->max_pages, "%zu pages, a batch of at most %zu", n_pages, b->max_pages);
-    // Everything is checked before anything is changed.
-    size_t tokens = 0, entries = 0;
-    const size_t L = b->page_len;
-    for (size_t s = 0; s < n_seqs; ++s) {
-        const size_t len = (size_t)context[s] + n_new[s];
-        entries += (len + L - 1) / L;
-        tokens += n_new[s];
-        TH_REQUIRE(entries <= n_pages, "sequence %zu of %zu positions is past the end of %zu pages", s, len, n_pages);
-        TH_REQUIRE(tokens <= b->max_tokens, "%zu tokens up to sequence %zu, a batch of at most %zu", tokens, s, b->max_tokens);
-    }
-    TH_REQUIRE(entries == n_pages, "%zu pages for sequences of %zu", n_pages, entries);
-    TH_REQUIRE(tokens <= b->captured_tokens,
-               "%zu tokens: a graph was captured with this batch at %zu, and its launches take no more", tokens,
-               b->captured_tokens);
-    for (size_t i = 0; i < n_pages; ++i)
-        TH_REQUIRE(pages[i] < b->pages, "page %u at index %zu of a cache of %zu", pages[i], i, b->pages);
-    // A page that gets new rows is in no other place of a sequence with tokens.
-    if (++b->epoch == 0) {
-        memset(b->stamp, 0, b->pages * sizeof(uint32_t));
-        b->epoch = 1;
-    }
-    for (size_t s = 0, p0 = 0; s < n_seqs; ++s) {
-        const size_t len = (size_t)context[s] + n_new[s], end = p0 + (len + L - 1) / L;
-        for (size_t p = p0 + context[s] / L; n_new[s] && p < end; ++p) {
-            TH_REQUIRE(b->stamp[pages[p]] != b->epoch, "page %u gets new rows in two places, one of them of sequence %zu",
-                       pages[p], s);
-            b->stamp[pages[p]] = b->epoch;
-        }
-        p0 = end;
-    }
-    for (size_t s = 0, p0 = 0; s < n_seqs; ++s) {
-        const size_t len = (size_t)context[s] + n_new[s], end = p0 + (len + L - 1) / L;
-        for (size_t p = p0; n_new[s] && p < p0 + context[s] / L; ++p)
-            TH_REQUIRE(b->stamp[pages[p]] != b->epoch, "page %u gets new rows, and is in the context of sequence %zu", pages[p], s);
-        p0 = end;
-    }
-    for (size_t s = 0, t0 = 0; parents && s < n_seqs; t0 += n_new[s++]) {
-        bool chain = true;
-        for (size_t i = 0; i < n_new[s]; ++i) {
-            TH_REQUIRE(parents[t0 + i] >= -1 && parents[t0 + i] < (int64_t)i, "parent %d of token %zu of sequence %zu",
-                       parents[t0 + i], i, s);
-            chain = chain && parents[t0 + i] == (int64_t)i - 1;
-        }
-        TH_REQUIRE(chain || n_new[s] <= th::kTreeTokens, "a tree of %u tokens: at most %zu", n_new[s], th::kTreeTokens);
-    }
+    TRY(check_set(b, n_seqs, context, n_new, pages, n_pages, parents));
     TH_PAGED_CURRENT(dev);
     TH_HIP(hipEventSynchronize(b->copied));  // the copy before has read the pinned memory
-    auto *head = b->head();
-    auto *seqs = b->seqs();
-    auto *toks = reinterpret_cast<th::TokenAt *>(b->pinned + b->at_tokens);
-    auto *tree = reinterpret_cast<uint64_t *>(b->pinned + b->at_tree);
-    head->n_seqs = (uint32_t)n_seqs;
-    head->n_tokens = (uint32_t)tokens;
-    if (n_pages) memcpy(b->page_list(), pages, n_pages * sizeof(uint32_t));
-    size_t positions = 0, t0 = 0, p0 = 0, trees = 0;
-    for (size_t s = 0; s < n_seqs; ++s) {
-        const uint32_t n = n_new[s], ctx = context[s];
-        int32_t *par = b->parents + t0;
-        bool chain = true;
-        for (uint32_t i = 0; i < n; ++i) {
-            par[i] = parents ? parents[t0 + i] : (int32_t)i - 1;
-            chain = chain && par[i] == (int32_t)i - 1;
-        }
-        seqs[s] = {(uint32_t)t0, n, ctx, (uint32_t)p0, !chain};
-        for (uint32_t i = 0; i < n; ++i) {
-            const size_t at = (size_t)ctx + i;
-            th::TokenAt &t = toks[t0 + i];
-            t.slot = pages[p0 + at / L] << b->page_shift | (uint32_t)(at & (L - 1));
-            t.pos = par[i] < 0 ? ctx : toks[t0 + par[i]].pos + 1;
-            t.seq = (uint32_t)s;
-            t.index = i;
-            positions = std::max<size_t>(positions, (size_t)t.pos + 1);
-            if (chain) continue;
-            uint64_t *bits = tree + (t0 + i) * th::kTreeWords;
-            for (int w = 0; w < th::kTreeWords; ++w) bits[w] = par[i] < 0 ? 0 : tree[(t0 + par[i]) * th::kTreeWords + w];
-            bits[i / 64] |= (uint64_t)1 << (i & 63);
-        }
-        if (!chain) trees = t0 + n;
-        t0 += n;
-        p0 += ((size_t)ctx + n + L - 1) / L;
-    }
-    b->n_seqs = n_seqs;
-    b->n_tokens = tokens;
-    b->n_pages = n_pages;
-    b->positions = positions;
-    auto *items = reinterpret_cast<th::ItemAt *>(b->pinned + b->at_items);
-    auto *joins = reinterpret_cast<th::JoinAt *>(b->pinned + b->at_joins);
-    th::plan_attention(b->plan_shape(), seqs, head, items, joins);
+    const size_t trees = lay_out(b, n_seqs, context, n_new, pages, n_pages, parents);
+    const th::BatchHead *head = b->head();
     th::Upload u{};
     int k = 0;
     auto add = [&](size_t at, size_t bytes) {
@@ -393,7 +376,7 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     };
     add(0, sizeof(th::BatchHead));
     add(b->at_seqs, n_seqs * sizeof(th::SeqAt));
-    add(b->at_tokens, tokens * sizeof(th::TokenAt));
+    add(b->at_tokens, b->n_tokens * sizeof(th::TokenAt));
     add(b->at_pages, n_pages * sizeof(uint32_t));
     add(b->at_tree, trees * th::kTreeWords * sizeof(uint64_t));
     add(b->at_items, head->first[th::kClasses] * sizeof(th::ItemAt));
@@ -496,7 +479,6 @@ int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, cons
     for (size_t i = 0; i < n_caches; ++i) {
         TH_REQUIRE(caches[i], "th_paged_keep: null cache");
         TRY(same_cache(dev, caches[i], b));
-        TH_REQUIRE(caches[i]->kv_dtype == caches[0]->kv_dtype, "caches of two types");
         for (size_t j = 0; j < i; ++j) TH_REQUIRE(caches[i] != caches[j], "the same cache twice");
     }
     TH_REQUIRE(b->n_seqs == 0 || n_kept, "th_paged_keep: null argument");
@@ -552,6 +534,46 @@ int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, cons
     }
     TH_HIP(flush());
     return TH_OK;
+}
+
+int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tokens, size_t n_seqs, const uint32_t *context,
+                      const uint32_t *n_new, const uint32_t *pages, size_t n_pages, const int32_t *parents, uint32_t *tokens,
+                      uint64_t *tree, uint32_t *items, size_t *n_items, uint32_t *joins, size_t *n_joins, uint32_t *first) {
+    th_batch b;
+    b.pages = shape[0];
+    b.page_len = shape[1];
+    b.n_kv_heads = shape[2];
+    b.head_dim = shape[3];
+    b.kv_dtype = (int)shape[4];
+    b.n_heads = shape[5];
+    b.max_seqs = shape[6];
+    b.max_tokens = shape[7];
+    b.max_pages = shape[8];
+    b.classes = classes;
+    b.captured_tokens = captured_tokens;
+    size_t bytes = 0;
+    const bool held = place_arrays(&b, &bytes) && (b.pinned = static_cast<char *>(calloc(1, bytes)));
+    int rc = held ? check_set(&b, n_seqs, context, n_new, pages, n_pages, parents) : fail(TH_ERR_NOMEM, "out of host memory");
+    if (rc == TH_OK) {
+        lay_out(&b, n_seqs, context, n_new, pages, n_pages, parents);
+        const th::BatchHead *head = b.head();
+        const size_t most_items = *n_items, most_joins = *n_joins;
+        *n_items = head->first[th::kClasses];
+        *n_joins = head->n_joins;
+        if (*n_items > std::min(most_items, b.plan_shape().max_items) || *n_joins > std::min(most_joins, b.plan_shape().max_joins)) {
+            rc = fail(TH_ERR_INVALID, "%zu items and %zu joins", *n_items, *n_joins);
+        } else {
+            memcpy(tokens, b.pinned + b.at_tokens, b.n_tokens * sizeof(th::TokenAt));
+            memcpy(tree, b.pinned + b.at_tree, b.n_tokens * th::kTreeWords * sizeof(uint64_t));
+            memcpy(items, b.pinned + b.at_items, *n_items * sizeof(th::ItemAt));
+            memcpy(joins, b.pinned + b.at_joins, *n_joins * sizeof(th::JoinAt));
+            memcpy(first, head->first, sizeof head->first);
+        }
+    }
+    free(b.pinned);
+    free(b.parents);
+    free(b.stamp);
+    return rc;
 }
 
 }  // extern "C"

@@ -378,14 +378,15 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // the tile's four sixteens, which with V^T's columns in that order are the
 // operand of O^T = V^T P^T.
 //
-// A tile with an infinity or a NaN, or where rows do not see all positions and
-// the positions' values differ by more than 2^12, and the ones after it, are
-// summed from memory in f32, a position at a time, by each row for itself:
-// what it does not see does not reach it.
+// Where a tile has an infinity or a NaN, or where rows do not see all positions
+// and these differ by more than 2^12, the item is done again from memory, in
+// f32, a position at a time and each row for itself: what it does not see does
+// not reach it. (Some 3 us a position: these are no numbers to be fast with.)
 template <int HD, int SETS, typename KV>
-__global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnArgs a, Launch launch) {
+__global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2) void paged_many_kernel(PagedAttnArgs a, Launch launch) {
     constexpr bool F32 = sizeof(KV) == 4;
     constexpr int KT = kManyKeys, RW = 16 * SETS;
+    constexpr bool kAhead = F32 || SETS > 1;
     constexpr float kGrow = 5.f, kBase = 10.f;  // weights below 2^15
     constexpr uint32_t KB = 2 * HD, VB = 2 * KT;  // bytes of a key, and of a dimension's positions
     constexpr int LPK = HD / 8;                // lanes a key
@@ -405,449 +406,452 @@ __global__ __launch_bounds__(kManyThreads, 2) void paged_many_kernel(PagedAttnAr
     }
     n *= a.n_kv_heads;
     const float c2 = a.scale * kLog2e;
-    for (uint32_t at = blockIdx.x; at < n; at += gridDim.x) {
-        const ItemAt it = scalar_load(a.b.items, first + at / a.n_kv_heads);
-        const int kvh = at % a.n_kv_heads;
-        const SeqAt &seq = it.seq;
-        const uint32_t rows = min((uint32_t)(8 * RW), seq.n_new * a.group - it.row0);
-        const size_t qbase = ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
-        auto row_at = [&](uint32_t row) { return qbase + ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
-        uint32_t token[SETS];
-        uint4 qh[SETS][HD / 32], ql[SETS][HD / 32];
-        float qf[SETS];  // the scale of a row's scores, c2 in it
+    if (blockIdx.x >= n) return;
+    const ItemAt it = scalar_load(a.b.items, first + blockIdx.x / a.n_kv_heads);
+    const int kvh = blockIdx.x % a.n_kv_heads;
+    const SeqAt &seq = it.seq;
+    const uint32_t rows = min((uint32_t)(8 * RW), seq.n_new * a.group - it.row0);
+    const int wrow = RW * wave;  // the wave's first row
+    const size_t qbase = ((size_t)seq.token0 * a.n_heads + (size_t)kvh * a.group) * HD;
+    auto row_at = [&](uint32_t row) { return qbase + ((size_t)(row / a.group) * a.n_heads + row % a.group) * HD; };
+    uint32_t token[SETS];
+    uint4 qh[SETS][HD / 32], ql[SETS][HD / 32];
+    float qf[SETS];  // the scale of a row's scores, c2 in it
 #pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-            const uint32_t row = it.row0 + min((uint32_t)(RW * wave + 16 * s + li), rows - 1);  // past the last: it again
-            token[s] = row / a.group;
-            const float *const src = a.q + row_at(row) + 8 * lg;
-            float f[HD / 32][8];
-            uint32_t most = 0;
+    for (int s = 0; s < SETS; ++s) {
+        const uint32_t row = it.row0 + min((uint32_t)(wrow + 16 * s + li), rows - 1);  // past the last: it again
+        token[s] = row / a.group;
+        const float *const src = a.q + row_at(row) + 8 * lg;
+        float f[HD / 32][8];
+        uint32_t most = 0;
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                const float4 x = *reinterpret_cast<const float4 *>(src + 32 * c);
-                const float4 y = *reinterpret_cast<const float4 *>(src + 32 * c + 4);
+        for (int c = 0; c < HD / 32; ++c) {
+            const float4 x = *reinterpret_cast<const float4 *>(src + 32 * c);
+            const float4 y = *reinterpret_cast<const float4 *>(src + 32 * c + 4);
+            const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[c][e] = v[e];
+                most = max(most, magnitude(v[e]));
+            }
+        }
+        most = across_max(most);
+        const int sh = shift_of(most);
+        qf[s] = ldexpf(c2, -sh);
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_f16<true>(ldexpf(f[c][2 * e], sh), ldexpf(f[c][2 * e + 1], sh), h[e], l[e]);
+            qh[s][c] = make_uint4(h[0], h[1], h[2], h[3]);
+            ql[s][c] = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+    }
+    // Of the wave's rows: the first position that one does not see, and the
+    // first that none sees (zero: there are no such rows).
+    const uint32_t w0 = wrow, w1 = min(w0 + RW, rows) - 1;
+    const uint32_t all_see = seq.context + (seq.is_tree ? 0 : (it.row0 + min(w0, rows - 1)) / a.group + 1);
+    const uint32_t none_sees = w0 >= rows ? 0 : seq.context + (it.row0 + w1) / a.group + 1;
+    f32x4 o[SETS][HD / 16];
+    float mx[SETS], l[SETS];
+    int units[SETS];  // o is of values times 2^units
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+        mx[s] = -INFINITY;
+        l[s] = 0.f;
+        units[s] = 0;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[s][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const uint32_t *const pages = a.b.pages + seq.page0;
+    const uint32_t mask = (1u << a.b.page_shift) - 1;
+    const size_t to_v = ((size_t)a.n_kv_heads << a.b.page_shift) * HD;
+    // A key's row, with its sixteen's page: positions past the last repeat its page.
+    auto row_of = [&](uint32_t pos) {
+        const size_t page = scalar_load(pages, min(pos, it.k1 - 1) >> a.b.page_shift);
+        return static_cast<const KV *>(a.cache) +
+               ((((page * 2 * a.n_kv_heads + kvh)) << a.b.page_shift) + (pos & mask)) * HD;
+    };
+    // What a thread stages: keys kkey + KT / KU i, 8 values from 8 kch;
+    // values of dimensions VD lane + {0, ..}, of the 8 positions that are
+    // operand group `wave`: sixteens 2 sigma and 2 sigma + 1, four of each.
+    // (Formed from the thread's number where they are used: with all of them
+    // kept, the registers do not suffice.)
+    const int wkey = wave * (64 / LPK);  // the wave's first
+    const int vkey = 32 * (wave >> 2) + 4 * (wave & 3);
+    auto thread = [] {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        return t;
+    };
+    // Where 16 bytes of a row lie: rows of 256 bytes cover the banks, two of
+    // 128 do. What the lanes of a fragment's read take, and neighbouring
+    // lanes write, is in as many banks.
+    auto swizzled = [](uint32_t bytes, uint32_t row, uint32_t chunk) {
+        return row * bytes + 16 * (chunk ^ (bytes == 256 ? row & 15 : row >> 1 & 7));
+    };
+    auto at_lds = [&](uint32_t o) -> uint4 & { return *reinterpret_cast<uint4 *>(lds + o); };
+    float kraw[KU][8], vraw[8][VD];
+    auto fetch = [&](uint32_t c0) {
+        const int tid = thread();
+        const uint32_t klane = ((tid / LPK - (wkey & ~15)) * HD + 8 * (tid % LPK)) * sizeof(KV);
+        const uint32_t vlane = VD * (tid & 63) * sizeof(KV);
+#pragma unroll
+        for (int i = 0; i < KU; ++i) {
+            const KV *src = reinterpret_cast<const KV *>(
+                reinterpret_cast<const char *>(row_of(c0 + (wkey & ~15) + KT / KU * i)) + klane);
+            if constexpr (F32) {
+                const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
                 const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    f[c][e] = v[e];
-                    most = max(most, magnitude(v[e]));
+                for (int e = 0; e < 8; ++e) kraw[i][e] = v[e];
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4 *>(src);
+                kraw[i][0] = __uint_as_float(w.x); kraw[i][1] = __uint_as_float(w.y);
+                kraw[i][2] = __uint_as_float(w.z); kraw[i][3] = __uint_as_float(w.w);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const KV *src = reinterpret_cast<const KV *>(
+                reinterpret_cast<const char *>(row_of(c0 + 32 * (wave >> 2) + 16 * h) + to_v + 4 * (wave & 3) * HD) + vlane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (F32 && VD == 2) {
+                    const float2 x = *reinterpret_cast<const float2 *>(src + j * HD);
+                    vraw[4 * h + j][0] = x.x;
+                    vraw[4 * h + j][1] = x.y;
+                } else if constexpr (F32) {
+                    vraw[4 * h + j][0] = src[j * HD];
+                } else if constexpr (VD == 2) {
+                    vraw[4 * h + j][0] = __uint_as_float(*reinterpret_cast<const uint32_t *>(src + j * HD));
+                } else {
+                    vraw[4 * h + j][0] = __uint_as_float((uint32_t)src[j * HD]);
                 }
             }
-            most = across_max(most);
-            const int sh = shift_of(most);
-            qf[s] = ldexpf(c2, -sh);
+        }
+    };
+    // As f32 from what is in registers.
+    auto value = [&](int j, int d) {
+        if constexpr (F32) return vraw[j][d];
+        else return d ? bf16_hi(__float_as_uint(vraw[j][0])) : bf16_lo(__float_as_uint(vraw[j][0]));
+    };
+    auto key_value = [&](int i, int e) {
+        if constexpr (F32) return kraw[i][e];
+        else return e & 1 ? bf16_hi(__float_as_uint(kraw[i][e / 2])) : bf16_lo(__float_as_uint(kraw[i][e / 2]));
+    };
+    // The largest magnitude of the wave's keys and values, and, where some
+    // row does not see some position, the smallest of a position's largest.
+    auto look = [&](uint32_t c0, uint32_t tile) {
+        uint32_t ktop = 0, vtop = 0, kleast = 0x7f000000u, vleast = 0x7f000000u;
+        if (c0 + KT > it.k1) {  // past the last position is anything: zero
+            const int tid = thread();
+#pragma unroll
+            for (int i = 0; i < KU; ++i)
+#pragma unroll
+                for (int e = 0; e < (F32 ? 8 : 4); ++e)
+                    kraw[i][e] = c0 + tid / LPK + KT / KU * i < it.k1 ? kraw[i][e] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int d = 0; d < (F32 ? VD : 1); ++d)
+                    vraw[j][d] = c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? vraw[j][d] : 0.f;
+        }
+        if (c0 + KT > seq.context) {
+#pragma unroll
+            for (int i = 0; i < KU; ++i) {
+                uint32_t own = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) own = max(own, magnitude(key_value(i, e)));
+                own = LPK == 16 ? row_max(own) : dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(own)));  // row_half_mirror
+                ktop = max(ktop, own);
+                kleast = own ? min(kleast, own) : kleast;
+            }
+            kleast = ~across_max(row_max(~kleast));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t own = 0;
+#pragma unroll
+                for (int d = 0; d < VD; ++d) own = max(own, magnitude(value(j, d)));
+                own = across_max(row_max(own));
+                vtop = max(vtop, own);
+                vleast = own ? min(vleast, own) : vleast;
+            }
+            ktop = across_max(row_max(ktop));
+        } else {
+            float k = 0.f, v = 0.f;
+#pragma unroll
+            for (int i = 0; i < KU; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    k = max_or_nan(max_or_nan(k, __builtin_fabsf(key_value(i, e))), __builtin_fabsf(key_value(i, e + 1)));
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+#pragma unroll
+                for (int d = 0; d < VD; ++d)
+                    v = max_or_nan(max_or_nan(v, __builtin_fabsf(value(j, d))), __builtin_fabsf(value(j + 1, d)));
+            ktop = across_max(row_max(magnitude(k)));
+            vtop = across_max(row_max(magnitude(v)));
+        }
+        if ((thread() & 63) == 0) looked[tile & 1][wave] = make_uint4(ktop, vtop, kleast, vleast);
+    };
+    int shift = 1 << 20;  // of the last tile's values; at first more than any
+    int kshift = 0;       // of the last tile's keys
+    // The tile in registers to LDS.
+    auto store = [&](uint32_t tile) {
+        // A wave's part a lane, the eight of them over each 16 lanes.
+        const int tid = thread(), kkey = tid / LPK, kch = tid % LPK;
+        const uint4 w = looked[tile & 1][tid & 7];
+        auto uniform_max = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(v)); };
+        const uint32_t ktop = uniform_max(w.x), vtop = uniform_max(w.y), kleast = ~uniform_max(~w.z), vleast = ~uniform_max(~w.w);
+        // Infinities and NaN; positions 2^12 apart that not all rows see.
+        const bool odd = max(ktop, vtop) >= 0x7f800000u || (kleast < ktop && (ktop >> 23) - (kleast >> 23) > 12) ||
+                         (vleast < vtop && (vtop >> 23) - (vleast >> 23) > 12);
+        if (!odd) shift = min(shift, shift_of(vtop));
+        kshift = shift_of(ktop);
+        const uint32_t buf = (tile & 1) * kBuf;
+        const uint32_t kput = buf + swizzled(KB, kkey, kch);
+#pragma unroll
+        for (int i = 0; i < KU; ++i) {
+            uint32_t h[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                split_f16<F32>(ldexpf(key_value(i, 2 * e), kshift), ldexpf(key_value(i, 2 * e + 1), kshift), h[e], lo[e]);
+            const uint32_t to = kput + KT / KU * i * KB;
+            at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
+            if constexpr (F32) at_lds(to + kKL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+            uint32_t h[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                split_f16<F32>(ldexpf(value(2 * e, d), shift), ldexpf(value(2 * e + 1, d), shift), h[e], lo[e]);
+            const uint32_t to = buf + kVH + swizzled(VB, VD * (tid & 63) + d, wave);
+            at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
+            if constexpr (F32) at_lds(to + kVL - kVH) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (odd) odd_of[tile & 3] = 1;
+    };
+    // Scores, weights and sums of 32 positions at a time (of 64: 16 more
+    // registers for scores and 16 for weights than there are).
+    auto products = [&](uint32_t c0, uint32_t tile, int tile_shift, int tile_kshift) {
+        auto mfma = [](const uint4 &x, const uint4 &y, const f32x4 &z) {
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
+        };
+        const bool masked = c0 + KT > all_see || c0 + KT > it.k1;
+        const int tid = thread(), li = tid & 15, lg = tid >> 4 & 3;
+        const uint32_t buf = (tile & 1) * kBuf, kget = buf + swizzled(KB, li, lg), vget = buf + kVH + swizzled(VB, li, lg);
+#pragma unroll 1
+        for (int h = 0; h < KT / 32; ++h) {
+            f32x4 st[SETS][2];
+#pragma unroll
+            for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) st[s][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const uint32_t vb = vget ^ 64 * h;  // the chunk 4 h + lg
+            // A step's fragments are requested before the products of the
+            // one before it (where there are registers for both).
+            uint4 x[2][2], y[2][F32 ? 2 : 1];
+            auto key_fragments = [&](int c) {
+                const uint32_t kb = (kget ^ 64 * c) + 32 * h * KB;  // the chunk 4 c + lg
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x[c & 1][j] = at_lds(kb + 16 * j * KB);
+                    if constexpr (F32) y[c & 1][j] = at_lds(kb + kKL + 16 * j * KB);
+                }
+            };
+            if (kAhead) key_fragments(0);
+            __builtin_amdgcn_s_setprio(1);  // products before another wave's conversions
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) split_f16<true>(ldexpf(f[c][2 * e], sh), ldexpf(f[c][2 * e + 1], sh), h[e], l[e]);
-                qh[s][c] = make_uint4(h[0], h[1], h[2], h[3]);
-                ql[s][c] = make_uint4(l[0], l[1], l[2], l[3]);
-            }
-        }
-        // Of the wave's rows: the first position that one does not see, and the
-        // first that none sees (zero: there are no such rows).
-        const uint32_t w0 = RW * wave, w1 = min(w0 + RW, rows) - 1;
-        const uint32_t all_see = seq.context + (seq.is_tree ? 0 : (it.row0 + min(w0, rows - 1)) / a.group + 1);
-        const uint32_t none_sees = w0 >= rows ? 0 : seq.context + (it.row0 + w1) / a.group + 1;
-        f32x4 o[SETS][HD / 16];
-        float mx[SETS], l[SETS];
-        int units[SETS];  // o is of values times 2^units
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-            mx[s] = -INFINITY;
-            l[s] = 0.f;
-            units[s] = 0;
-#pragma unroll
-            for (int d = 0; d < HD / 16; ++d) o[s][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        const uint32_t *const pages = a.b.pages + seq.page0;
-        const uint32_t mask = (1u << a.b.page_shift) - 1;
-        const size_t to_v = ((size_t)a.n_kv_heads << a.b.page_shift) * HD;
-        // A key's row, with its sixteen's page: positions past the last repeat its page.
-        auto row_of = [&](uint32_t pos) {
-            const size_t page = scalar_load(pages, min(pos, it.k1 - 1) >> a.b.page_shift);
-            return static_cast<const KV *>(a.cache) +
-                   ((((page * 2 * a.n_kv_heads + kvh)) << a.b.page_shift) + (pos & mask)) * HD;
-        };
-        // What a thread stages: keys kkey + KT / KU i, 8 values from 8 kch;
-        // values of dimensions VD lane + {0, ..}, of the 8 positions that are
-        // operand group `wave`: sixteens 2 sigma and 2 sigma + 1, four of each.
-        // (Formed from the thread's number where they are used: with all of them
-        // kept, the registers do not suffice.)
-        const int wkey = wave * (64 / LPK);  // the wave's first
-        const int vkey = 32 * (wave >> 2) + 4 * (wave & 3);
-        auto thread = [] {
-            int t = threadIdx.x;
-            asm volatile("" : "+v"(t));
-            return t;
-        };
-        // Where 16 bytes of a row lie: rows of 256 bytes cover the banks, two of
-        // 128 do. What the lanes of a fragment's read take, and neighbouring
-        // lanes write, is in as many banks.
-        auto swizzled = [](uint32_t bytes, uint32_t row, uint32_t chunk) {
-            return row * bytes + 16 * (chunk ^ (bytes == 256 ? row & 15 : row >> 1 & 7));
-        };
-        auto at_lds = [&](uint32_t o) -> uint4 & { return *reinterpret_cast<uint4 *>(lds + o); };
-        float kraw[KU][8], vraw[8][VD];
-        auto fetch = [&](uint32_t c0) {
-            const int tid = thread();
-            const uint32_t klane = ((tid / LPK - (wkey & ~15)) * HD + 8 * (tid % LPK)) * sizeof(KV);
-            const uint32_t vlane = VD * (tid & 63) * sizeof(KV);
-#pragma unroll
-            for (int i = 0; i < KU; ++i) {
-                const KV *src = reinterpret_cast<const KV *>(
-                    reinterpret_cast<const char *>(row_of(c0 + (wkey & ~15) + KT / KU * i)) + klane);
-                if constexpr (F32) {
-                    const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
-                    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) kraw[i][e] = v[e];
-                } else {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(src);
-                    kraw[i][0] = __uint_as_float(w.x); kraw[i][1] = __uint_as_float(w.y);
-                    kraw[i][2] = __uint_as_float(w.z); kraw[i][3] = __uint_as_float(w.w);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const KV *src = reinterpret_cast<const KV *>(
-                    reinterpret_cast<const char *>(row_of(c0 + 32 * (wave >> 2) + 16 * h) + to_v + 4 * (wave & 3) * HD) + vlane);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (F32 && VD == 2) {
-                        const float2 x = *reinterpret_cast<const float2 *>(src + j * HD);
-                        vraw[4 * h + j][0] = x.x;
-                        vraw[4 * h + j][1] = x.y;
-                    } else if constexpr (F32) {
-                        vraw[4 * h + j][0] = src[j * HD];
-                    } else if constexpr (VD == 2) {
-                        vraw[4 * h + j][0] = __uint_as_float(*reinterpret_cast<const uint32_t *>(src + j * HD));
-                    } else {
-                        vraw[4 * h + j][0] = __uint_as_float((uint32_t)src[j * HD]);
-                    }
-                }
-            }
-        };
-        // As f32 from what is in registers.
-        auto value = [&](int j, int d) {
-            if constexpr (F32) return vraw[j][d];
-            else return d ? bf16_hi(__float_as_uint(vraw[j][0])) : bf16_lo(__float_as_uint(vraw[j][0]));
-        };
-        auto key_value = [&](int i, int e) {
-            if constexpr (F32) return kraw[i][e];
-            else return e & 1 ? bf16_hi(__float_as_uint(kraw[i][e / 2])) : bf16_lo(__float_as_uint(kraw[i][e / 2]));
-        };
-        // The largest magnitude of the wave's keys and values, and, where some
-        // row does not see some position, the smallest of a position's largest.
-        auto look = [&](uint32_t c0, uint32_t tile) {
-            uint32_t ktop = 0, vtop = 0, kleast = 0x7f000000u, vleast = 0x7f000000u;
-            if (c0 + KT > it.k1) {  // past the last position is anything: zero
-                const int tid = thread();
-#pragma unroll
-                for (int i = 0; i < KU; ++i)
-#pragma unroll
-                    for (int e = 0; e < (F32 ? 8 : 4); ++e)
-                        kraw[i][e] = c0 + tid / LPK + KT / KU * i < it.k1 ? kraw[i][e] : 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int d = 0; d < (F32 ? VD : 1); ++d)
-                        vraw[j][d] = c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? vraw[j][d] : 0.f;
-            }
-            if (c0 + KT > seq.context) {
-#pragma unroll
-                for (int i = 0; i < KU; ++i) {
-                    uint32_t own = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) own = max(own, magnitude(key_value(i, e)));
-                    own = LPK == 16 ? row_max(own) : dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(own)));  // row_half_mirror
-                    ktop = max(ktop, own);
-                    kleast = own ? min(kleast, own) : kleast;
-                }
-                kleast = ~across_max(row_max(~kleast));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t own = 0;
-#pragma unroll
-                    for (int d = 0; d < VD; ++d) own = max(own, magnitude(value(j, d)));
-                    own = across_max(row_max(own));
-                    vtop = max(vtop, own);
-                    vleast = own ? min(vleast, own) : vleast;
-                }
-                ktop = across_max(row_max(ktop));
-            } else {
-                float k = 0.f, v = 0.f;
-#pragma unroll
-                for (int i = 0; i < KU; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        k = max_or_nan(max_or_nan(k, __builtin_fabsf(key_value(i, e))), __builtin_fabsf(key_value(i, e + 1)));
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-#pragma unroll
-                    for (int d = 0; d < VD; ++d)
-                        v = max_or_nan(max_or_nan(v, __builtin_fabsf(value(j, d))), __builtin_fabsf(value(j + 1, d)));
-                ktop = across_max(row_max(magnitude(k)));
-                vtop = across_max(row_max(magnitude(v)));
-            }
-            if (lane == 0) looked[tile & 1][wave] = make_uint4(ktop, vtop, kleast, vleast);
-        };
-        int shift = 1 << 20;  // of the last tile's values; at first more than any
-        int kshift = 0;       // of the last tile's keys
-        // The tile in registers to LDS.
-        auto store = [&](uint32_t tile) {
-            // A wave's part a lane, the eight of them over each 16 lanes.
-            const int tid = thread(), kkey = tid / LPK, kch = tid % LPK;
-            const uint4 w = looked[tile & 1][tid & 7];
-            auto uniform_max = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(v)); };
-            const uint32_t ktop = uniform_max(w.x), vtop = uniform_max(w.y), kleast = ~uniform_max(~w.z), vleast = ~uniform_max(~w.w);
-            // Infinities and NaN; positions 2^12 apart that not all rows see.
-            const bool odd = max(ktop, vtop) >= 0x7f800000u || (kleast < ktop && (ktop >> 23) - (kleast >> 23) > 12) ||
-                             (vleast < vtop && (vtop >> 23) - (vleast >> 23) > 12);
-            if (!odd) shift = min(shift, shift_of(vtop));
-            kshift = shift_of(ktop);
-            const uint32_t buf = (tile & 1) * kBuf;
-            const uint32_t kput = buf + swizzled(KB, kkey, kch);
-#pragma unroll
-            for (int i = 0; i < KU; ++i) {
-                uint32_t h[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    split_f16<F32>(ldexpf(key_value(i, 2 * e), kshift), ldexpf(key_value(i, 2 * e + 1), kshift), h[e], lo[e]);
-                const uint32_t to = kput + KT / KU * i * KB;
-                at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                if constexpr (F32) at_lds(to + kKL) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-#pragma unroll
-            for (int d = 0; d < VD; ++d) {
-                uint32_t h[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    split_f16<F32>(ldexpf(value(2 * e, d), shift), ldexpf(value(2 * e + 1, d), shift), h[e], lo[e]);
-                const uint32_t to = buf + kVH + swizzled(VB, VD * (tid & 63) + d, wave);
-                at_lds(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                if constexpr (F32) at_lds(to + kVL - kVH) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-            if (odd) odd_of[tile & 3] = 1;
-        };
-        // Scores, weights and sums of 32 positions at a time (of 64: 16 more
-        // registers for scores and 16 for weights than there are).
-        auto products = [&](uint32_t c0, uint32_t tile, int tile_shift, int tile_kshift) {
-            auto mfma = [](const uint4 &x, const uint4 &y, const f32x4 &z) {
-                return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
-            };
-            const bool masked = c0 + KT > all_see || c0 + KT > it.k1;
-            const int tid = thread(), li = tid & 15, lg = tid >> 4 & 3;
-            const uint32_t buf = (tile & 1) * kBuf, kget = buf + swizzled(KB, li, lg), vget = buf + kVH + swizzled(VB, li, lg);
-#pragma unroll 1
-            for (int h = 0; h < KT / 32; ++h) {
-                f32x4 st[SETS][2];
+                if (!kAhead) key_fragments(c);
+                else if (c + 1 < HD / 32) key_fragments(c + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) st[s][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const uint32_t vb = vget ^ 64 * h;  // the chunk 4 h + lg
-                // A step's fragments are requested before the products of the
-                // one before it.
-                uint4 x[2][2], y[2][F32 ? 2 : 1];
-                auto key_fragments = [&](int c) {
-                    const uint32_t kb = (kget ^ 64 * c) + 32 * h * KB;  // the chunk 4 c + lg
+                    for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], qh[s][c], st[s][j]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        x[c & 1][j] = at_lds(kb + 16 * j * KB);
-                        if constexpr (F32) y[c & 1][j] = at_lds(kb + kKL + 16 * j * KB);
-                    }
-                };
-                key_fragments(0);
-                __builtin_amdgcn_s_setprio(1);  // products before another wave's conversions
+                for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    if (c + 1 < HD / 32) key_fragments(c + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], ql[s][c], st[s][j]);
+                if constexpr (F32)
 #pragma unroll
                     for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], qh[s][c], st[s][j]);
+                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(y[c & 1][j], qh[s][c], st[s][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            uint4 ph[SETS], pl[SETS];
 #pragma unroll
-                    for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) st[s][j] = mfma(x[c & 1][j], ql[s][c], st[s][j]);
-                    if constexpr (F32)
-#pragma unroll
-                        for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) st[s][j] = mfma(y[c & 1][j], qh[s][c], st[s][j]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                __builtin_amdgcn_s_setprio(0);
-                uint4 ph[SETS], pl[SETS];
-#pragma unroll
-                for (int s = 0; s < SETS; ++s) {
-                    if (masked) {
-                        uint32_t own = token[s];
-                        asm volatile("" : "+v"(own));  // (nothing of it formed ahead)
-                        uint64_t all = seen64(seq, a.b.tree, own, c0);
-                        if (it.k1 - c0 < 64) all &= (1ull << (it.k1 - c0)) - 1;
-                        const uint32_t seen = (uint32_t)(all >> 32 * h) >> 4 * lg;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) st[s][j][e] = seen >> (16 * j + e) & 1 ? st[s][j][e] : -INFINITY;
-                    }
-                    float top = -INFINITY;
+            for (int s = 0; s < SETS; ++s) {
+                if (masked) {
+                    uint32_t own = token[s];
+                    asm volatile("" : "+v"(own));  // (nothing of it formed ahead)
+                    uint64_t all = seen64(seq, a.b.tree, own, c0);
+                    if (it.k1 - c0 < 64) all &= (1ull << (it.k1 - c0)) - 1;
+                    const uint32_t seen = (uint32_t)(all >> 32 * h) >> 4 * lg;
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; e += 2) top = max_or_nan(max_or_nan(top, st[s][j][e]), st[s][j][e + 1]);
-                    // Scores in units of log2. (Neither zero nor infinite: what is
-                    // not seen is -inf, and stays it.)
-                    const float f = fminf(fmaxf(ldexpf(qf[s], -tile_kshift), 0x1p-126f), 0x1p127f);
-                    top = rows_max_nn(top) * f;
-                    const bool any = top != -INFINITY;  // the row sees some
-                    // The reference moves when the maximum is 2^kGrow past it.
-                    if (__any(top > mx[s] + kGrow || (any && units[s] != tile_shift))) {
-                        const float next = max_nn(mx[s], top);
-                        const float alpha = mx[s] == next ? 1.f : __builtin_amdgcn_exp2f(mx[s] - next);
-                        mx[s] = next;
-                        l[s] *= alpha;
-                        const int by = any ? tile_shift - units[s] : 0;
-                        units[s] += by;
-                        const float g = ldexpf(alpha, by);
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d) o[s][d] *= g;
-                    }
-                    const float base = mx[s] == -INFINITY ? 0.f : kBase - mx[s];
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            st[s][j][e] = __builtin_amdgcn_exp2f(fmaf(st[s][j][e], f, base));
-                            l[s] += st[s][j][e];
-                        }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        split_f16<true>(st[s][e / 2][2 * (e & 1)], st[s][e / 2][2 * (e & 1) + 1], hi[e], lo[e]);
-                    ph[s] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    pl[s] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        for (int e = 0; e < 4; ++e) st[s][j][e] = seen >> (16 * j + e) & 1 ? st[s][j][e] : -INFINITY;
                 }
-                auto value_fragments = [&](int n) {
+                float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[n & 1][i] = at_lds(vb + 16 * (2 * n + i) * VB);
-                        if constexpr (F32) y[n & 1][i] = at_lds(vb + kVL - kVH + 16 * (2 * n + i) * VB);
-                    }
-                };
-                value_fragments(0);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int n = 0; n < HD / 32; ++n) {
-                    if (n + 1 < HD / 32) value_fragments(n + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int e = 0; e < 4; e += 2) top = max_or_nan(max_or_nan(top, st[s][j][e]), st[s][j][e + 1]);
+                // Scores in units of log2. (Neither zero nor infinite: what is
+                // not seen is -inf, and stays it.)
+                const float f = fminf(fmaxf(ldexpf(qf[s], -tile_kshift), 0x1p-126f), 0x1p127f);
+                top = rows_max_nn(top) * f;
+                const bool any = top != -INFINITY;  // the row sees some
+                // The reference moves when the maximum is 2^kGrow past it.
+                if (__any(top > mx[s] + kGrow || (any && units[s] != tile_shift))) {
+                    const float next = max_nn(mx[s], top);
+                    const float alpha = mx[s] == next ? 1.f : __builtin_amdgcn_exp2f(mx[s] - next);
+                    mx[s] = next;
+                    l[s] *= alpha;
+                    const int by = any ? tile_shift - units[s] : 0;
+                    units[s] += by;
+                    const float g = ldexpf(alpha, by);
 #pragma unroll
-                    for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], ph[s], o[s][2 * n + i]);
-#pragma unroll
-                    for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], pl[s], o[s][2 * n + i]);
-                    if constexpr (F32)
-#pragma unroll
-                        for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(y[n & 1][i], ph[s], o[s][2 * n + i]);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int d = 0; d < HD / 16; ++d) o[s][d] *= g;
                 }
-            }
-        };
-        // A row set's results, or partial ones: x[d][e] 2^-by is dimension
-        // 16 d + 4 lg + e of the lane's row, of weights exp2(. - top).
-        auto put = [&](int s, const f32x4 (&x)[HD / 16], float top, float sum, int by) {
-            const int tid = thread(), li = tid & 15, g4 = 4 * (tid >> 4 & 3);
-            const uint32_t r = RW * wave + 16 * s + li;
-            if (r >= rows) return;
-            float *dst;
-            float f;
-            if (it.part == kNoPart) {
-                dst = a.out + row_at(it.row0 + r);
-                f = 1.f / sum;
-            } else {
-                dst = a.part + (size_t)(it.part + kvh * 8 * SETS + r / 16) * slab_floats(HD);
-                f = 1.f;
-                if (g4 == 0) *reinterpret_cast<float2 *>(dst + 16 * HD + 2 * li) = make_float2(top, sum);
-                dst += li * HD;
-            }
+                const float base = mx[s] == -INFINITY ? 0.f : kBase - mx[s];
+                uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d)
-                *reinterpret_cast<float4 *>(dst + 16 * d + g4) = make_float4(ldexpf(x[d][0] * f, -by), ldexpf(x[d][1] * f, -by),
-                                                                            ldexpf(x[d][2] * f, -by), ldexpf(x[d][3] * f, -by));
-        };
-        // A row set from memory, from the first position on, one at a time.
-        auto one_by_one = [&](int s) {
-            auto as_f32 = [](KV w) { return F32 ? (float)w : bf16_to_f32((uint16_t)w); };
-            const int own = thread() & 63, g4 = 4 * (own >> 4);
-            const uint32_t row = it.row0 + min((uint32_t)(RW * wave + 16 * s + (own & 15)), rows - 1);
-            const float *const qr = a.q + row_at(row) + g4;
-            f32x4 x[HD / 16];
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int d = 0; d < HD / 16; ++d) x[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-            for (uint32_t key = it.k0; key < it.k1; ++key) {
-                const KV *const kr = row_of(key) + g4, *const vr = kr + to_v;
-                float y = 0.f;
-#pragma unroll 1
-                for (int i = 0; i < HD / 4; ++i) y = fmaf(qr[16 * (i / 4) + i % 4], as_f32(kr[16 * (i / 4) + i % 4]), y);
-                y = rows_sum(y) * c2;
-                const bool sees = seen64(seq, a.b.tree, row / a.group, key) & 1;
-                y = sees ? y : -INFINITY;
-                const float next = max_nn(top, y), base = next == -INFINITY ? 0.f : next;
-                const float alpha = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top - base);
-                const float p = __builtin_amdgcn_exp2f(y - base);
-                top = next;
-                sum = sum * alpha + p;
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float more = fmaf(p, as_f32(vr[16 * d + e]), x[d][e] * alpha);
-                        x[d][e] = sees ? more : x[d][e];
+                        st[s][j][e] = __builtin_amdgcn_exp2f(fmaf(st[s][j][e], f, base));
+                        l[s] += st[s][j][e];
                     }
-            }
-            put(s, x, top, sum, 0);
-        };
-        const uint32_t tiles = (it.k1 - it.k0 + KT - 1) / KT;
-        if (threadIdx.x < 4) odd_of[threadIdx.x] = 0;
-        fetch(it.k0);
-        look(it.k0, 0);
-        __syncthreads();
-        store(0);
-        int now = shift, know = kshift;
-        if (tiles > 1) fetch(it.k0 + KT);
-        uint32_t t = 0;
-        for (; t < tiles; ++t) {
-            const uint32_t c0 = it.k0 + t * KT;
-            if (t + 1 < tiles) look(c0 + KT, t + 1);
-            __syncthreads();  // tile t is stored, the other buffer free, the next one looked at
-            if (odd_of[t & 3]) break;
-            if (threadIdx.x == 0) odd_of[(t + 3) & 3] = 0;  // tile t - 1's, for tile t + 3
-            if (t + 1 < tiles) store(t + 1);
-            if (t + 2 < tiles) fetch(c0 + 2 * KT);
-            if (c0 < none_sees) products(c0, t, now, know);
-            now = shift;
-            know = kshift;
-        }
-        if (none_sees) {
-            if (__builtin_expect(t < tiles, 0)) {
 #pragma unroll
-                for (int s = 0; s < SETS; ++s) one_by_one(s);
-            } else {
+                for (int e = 0; e < 4; ++e)
+                    split_f16<true>(st[s][e / 2][2 * (e & 1)], st[s][e / 2][2 * (e & 1) + 1], hi[e], lo[e]);
+                ph[s] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                pl[s] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            auto value_fragments = [&](int n) {
 #pragma unroll
-                for (int s = 0; s < SETS; ++s) put(s, o[s], mx[s] - kBase, rows_sum(l[s]), units[s]);
+                for (int i = 0; i < 2; ++i) {
+                    x[n & 1][i] = at_lds(vb + 16 * (2 * n + i) * VB);
+                    if constexpr (F32) y[n & 1][i] = at_lds(vb + kVL - kVH + 16 * (2 * n + i) * VB);
+                }
+            };
+            if (kAhead) value_fragments(0);
+#pragma unroll
+            for (int n = 0; n < HD / 32; ++n) {
+                if (!kAhead) value_fragments(n);
+                else if (n + 1 < HD / 32) value_fragments(n + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], ph[s], o[s][2 * n + i]);
+#pragma unroll
+                for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(x[n & 1][i], pl[s], o[s][2 * n + i]);
+                if constexpr (F32)
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[s][2 * n + i] = mfma(y[n & 1][i], ph[s], o[s][2 * n + i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __syncthreads();  // LDS is written again
+    };
+    // A row set's results, or partial ones: x[d][e] 2^-by is dimension
+    // 16 d + 4 lg + e of the lane's row, of weights exp2(. - top).
+    auto put = [&](int s, const f32x4 (&x)[HD / 16], float top, float sum, int by) {
+        const int tid = thread(), li = tid & 15, g4 = 4 * (tid >> 4 & 3);
+        const uint32_t r = wrow + 16 * s + li;
+        if (r >= rows) return;
+        float *dst;
+        float f;
+        if (it.part == kNoPart) {
+            dst = a.out + row_at(it.row0 + r);
+            f = 1.f / sum;
+        } else {
+            dst = a.part + (size_t)(it.part + kvh * 8 * SETS + r / 16) * slab_floats(HD);
+            f = 1.f;
+            if (g4 == 0) *reinterpret_cast<float2 *>(dst + 16 * HD + 2 * li) = make_float2(top, sum);
+            dst += li * HD;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+            *reinterpret_cast<float4 *>(dst + 16 * d + g4) = make_float4(ldexpf(x[d][0] * f, -by), ldexpf(x[d][1] * f, -by),
+                                                                        ldexpf(x[d][2] * f, -by), ldexpf(x[d][3] * f, -by));
+    };
+    // A row set from memory, from the first position on, one at a time.
+    auto one_by_one = [&](int s) {
+        auto as_f32 = [](KV w) { return F32 ? (float)w : bf16_to_f32((uint16_t)w); };
+        const int own = thread() & 63, g4 = 4 * (own >> 4);
+        const uint32_t row = it.row0 + min((uint32_t)(wrow + 16 * s + (own & 15)), rows - 1);
+        const float *const qr = a.q + row_at(row) + g4;
+        f32x4 x[HD / 16];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) x[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (uint32_t key = it.k0; key < it.k1; ++key) {
+            const KV *const kr = row_of(key) + g4, *const vr = kr + to_v;
+            float y = 0.f;
+#pragma unroll 2
+            for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y = fmaf(qr[16 * d + e], as_f32(kr[16 * d + e]), y);
+            y = rows_sum(y) * c2;
+            const bool sees = seen64(seq, a.b.tree, row / a.group, key) & 1;
+            y = sees ? y : -INFINITY;
+            const float next = max_nn(top, y), base = next == -INFINITY ? 0.f : next;
+            const float alpha = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top - base);
+            const float p = __builtin_amdgcn_exp2f(y - base);
+            top = next;
+            sum = sum * alpha + p;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float more = fmaf(p, as_f32(vr[16 * d + e]), x[d][e] * alpha);
+                    x[d][e] = sees ? more : x[d][e];
+                }
+        }
+        put(s, x, top, sum, 0);
+    };
+    const uint32_t tiles = (it.k1 - it.k0 + KT - 1) / KT;
+    if (threadIdx.x < 4) odd_of[threadIdx.x] = 0;
+    fetch(it.k0);
+    look(it.k0, 0);
+    __syncthreads();
+    store(0);
+    int now = shift, know = kshift;
+    if (tiles > 1) fetch(it.k0 + KT);
+    uint32_t t = 0;
+    for (; t < tiles; ++t) {
+        const uint32_t c0 = it.k0 + t * KT;
+        if (t + 1 < tiles) look(c0 + KT, t + 1);
+        __syncthreads();  // tile t is stored, the other buffer free, the next one looked at
+        if (odd_of[t & 3]) break;
+        if (threadIdx.x == 0) odd_of[(t + 3) & 3] = 0;  // tile t - 1's, for tile t + 3
+        if (t + 1 < tiles) store(t + 1);
+        if (t + 2 < tiles) fetch(c0 + 2 * KT);
+        if (c0 < none_sees) products(c0, t, now, know);
+        now = shift;
+        know = kshift;
+    }
+    if (none_sees) {
+        if (__builtin_expect(t < tiles, 0)) {
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) one_by_one(s);
+        } else {
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) put(s, o[s], mx[s] - kBase, rows_sum(l[s]), units[s]);
+        }
     }
 }
 
@@ -923,8 +927,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     else join_rows<HD, 4>(a, head);
 }
 
-// A captured launch's grid, whatever is set later: its blocks walk the items.
+// A captured launch's grid, whatever is set later: the few-row kernel's blocks
+// walk the items, the others' have one each, of the most that there can be: a
+// sequence has 17 rows at least, a whole tile 128, and the rounds bound the splits.
 constexpr unsigned kCapturedBlocks = 1024;
+unsigned captured_blocks(const PagedAttnArgs &a, const BatchHead &count) {
+    const size_t rows = (size_t)count.n_tokens * a.group;
+    return (unsigned)((rows / 17 + rows / 128 + 2) * a.n_kv_heads + kMostSplitBlocks);
+}
 
 template <int HD>
 hipError_t few(hipStream_t s, const PagedAttnArgs &a, const Launch &l, unsigned grid, bool bf16) {
@@ -946,7 +956,9 @@ hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &cou
         const Launch l{count.first[c], count.first[c + 1] - count.first[c], c, captured};
         const size_t blocks = (size_t)l.n * a.n_kv_heads;
         if (!blocks && !(captured && c == 0)) continue;
-        const unsigned grid = captured ? kCapturedBlocks : (unsigned)std::min<size_t>(blocks, 0x7fffffu);
+        // (The few-row kernel's blocks walk the items past 2^22, too.)
+        const unsigned grid = c == 0 ? (unsigned)std::min<size_t>(captured ? kCapturedBlocks : blocks, (size_t)1 << 22)
+                                     : captured ? captured_blocks(a, count) : (unsigned)blocks;
         hipError_t e = hipSuccess;
         if (c == 0) e = few<HD>(s, a, l, grid, bf16);
         if constexpr (HD < 256) {

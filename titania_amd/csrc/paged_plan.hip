@@ -9,13 +9,14 @@ namespace th {
 namespace {
 
 // What the chip holds of a class's blocks at once.
-constexpr size_t kSlots[kClasses] = {512, 256, 256};
+constexpr size_t kSlots[kClasses] = {512, 256, 256}, kSlotsBf16[kClasses] = {512, 512, 256};
 // An estimate of a block's time in us: for each 64 positions, and for the rest of it.
 constexpr double kStepUs[kClasses] = {5.0, 3.5, 6.0}, kBlockUs[kClasses] = {5.0, 8.0, 10.0};
 // Of the second launch that joins split tiles.
 constexpr double kJoinUs = 5.0;
 // The most rounds of blocks that a class is split into.
 constexpr size_t kRounds = 4;
+static_assert(kRounds * kSlotsBf16[0] <= kMostSplitBlocks && kRounds * kSlotsBf16[1] <= kMostSplitBlocks, "splits");
 // A block's fewest positions: one step of its waves.
 constexpr size_t kStep = 64;
 
@@ -26,7 +27,7 @@ size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max
 }
 
 size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens) {
-    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kRounds * (kSlots[0] + kSlots[1] + kSlots[2]);
+    return most_joins(n_heads, n_kv_heads, max_seqs, max_tokens) + kClasses * kMostSplitBlocks;
 }
 
 void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins) {
@@ -74,7 +75,7 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
             each_tile(c, [&](uint32_t, uint32_t, size_t len) { items += ((len + kStep - 1) / kStep + most - 1) / most; });
             return items;
         };
-        const double slots = (double)kSlots[c] / shape.n_kv_heads;  // of items
+        const double slots = (double)(shape.bf16 ? kSlotsBf16 : kSlots)[c] / shape.n_kv_heads;  // of items
         size_t most = longest;
         double best = std::max((double)longest, steps / slots) * kStepUs[c] + std::max(1.0, tiles / slots) * kBlockUs[c];
         for (size_t r = 1; r <= kRounds; ++r) {
