@@ -182,6 +182,8 @@ class Batch:
 
 def _ints(a, dtype) -> np.ndarray:
     """Whole numbers as `dtype`, those that it does not hold refused."""
+    if type(a) is np.ndarray and a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     a = np.asarray(a)
     if a.size and not np.issubdtype(a.dtype, np.integer):
         raise TypeError(f"whole numbers, not {a.dtype}")
@@ -449,7 +451,7 @@ class Hip:
         n, k = _ints(n_kept, np.uint32), _ints(kept, np.int32)
         if n.size != batch.n_seqs or k.size != batch.n_tokens:
             raise ValueError(f"{n.size} counts and {k.size} places for {batch.n_seqs} sequences of {batch.n_tokens} tokens")
-        handles = (C.c_void_p * len(caches))(*(c.handle for c in caches))
+        handles = (C.c_void_p * len(caches))(*[c.handle for c in caches])
         check(lib().th_paged_keep(self.handle, handles, len(caches), batch.handle, n.ctypes.data, k.ctypes.data))
 
     # ---- the next token ----
