@@ -635,15 +635,14 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
     };
     // Scores, weights and sums of 32 positions at a time (of 64: 16 more
     // registers for scores and 16 for weights than there are).
-    auto products = [&](uint32_t c0, uint32_t tile, int tile_shift, int tile_kshift) {
+    auto products = [&](int h, uint32_t c0, uint32_t tile, int tile_shift, int tile_kshift) {
         auto mfma = [](const uint4 &x, const uint4 &y, const f32x4 &z) {
             return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), z, 0, 0, 0);
         };
         const bool masked = c0 + KT > all_see || c0 + KT > it.k1;
         const int tid = thread(), li = tid & 15, lg = tid >> 4 & 3;
         const uint32_t buf = (tile & 1) * kBuf, kget = buf + swizzled(KB, li, lg), vget = buf + kVH + swizzled(VB, li, lg);
-#pragma unroll 1
-        for (int h = 0; h < KT / 32; ++h) {
+        {
             f32x4 st[SETS][2];
 #pragma unroll
             for (int s = 0; s < SETS; ++s)
@@ -838,9 +837,14 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
         __syncthreads();  // tile t is stored, the other buffer free, the next one looked at
         if (odd_of[t & 3]) break;
         if (threadIdx.x == 0) odd_of[(t + 3) & 3] = 0;  // tile t - 1's, for tile t + 3
-        if (t + 1 < tiles) store(t + 1);
-        if (t + 2 < tiles) fetch(c0 + 2 * KT);
-        if (c0 < none_sees) products(c0, t, now, know);
+        auto next = [&] {
+            if (t + 1 < tiles) store(t + 1);
+            if (t + 2 < tiles) fetch(c0 + 2 * KT);
+        };
+        if (wave < 4) next();
+        if (c0 < none_sees) products(0, c0, t, now, know);
+        if (wave >= 4) next();
+        if (c0 < none_sees) products(1, c0, t, now, know);
         now = shift;
         know = kshift;
     }
