@@ -273,7 +273,8 @@ TH_API void th_batch_free(th_device *dev, th_batch *batch);
  * may be nobody else's. parents: NULL, or for each token the one of its own
  * sequence that it follows, by its place there, lower than its own, or -1 for
  * the context. Tokens that each follow the one before (always so with NULL)
- * are a chain; other sequences are trees, of at most 256 tokens. Token i is
+ * are a chain; other sequences are trees, of at most 256 tokens. A sequence
+ * has at most 2^30 positions. Token i is
  * written to position context[s] + i; it is rotated by context[s] plus its
  * depth, i in a chain, and sees the context, itself and what it follows, up to
  * the root. The arrays are copied before the call returns, to the device in
@@ -281,8 +282,11 @@ TH_API void th_batch_free(th_device *dev, th_batch *batch);
  *
  * Captured calls (th_graph_begin) read what is set when they run, so that one
  * graph serves any step: from then on th_batch_set refuses more tokens than
- * were set at the capture. Rows of activations behind the last token stay as
- * they are. */
+ * were set at the capture and positions past the end of a captured append's
+ * table, and plans the attention for the kernels that all the graphs hold: those
+ * for 1 to 16 query rows a KV head, always, and for up to 128 and for more where
+ * the step set at the capture had such sequences. Rows of activations behind
+ * the last token stay as they are. */
 TH_API int th_batch_set(th_device *dev, th_batch *batch, size_t n_seqs, const uint32_t *context, const uint32_t *n_new,
                         const uint32_t *pages, size_t n_pages, const int32_t *parents);
 /* For each token of the batch: q_out = q RMSNorm'd per head by q_norm and

@@ -14,15 +14,15 @@ extern "C" {
 /* th_batch_set for a batch of shape {pages, page_len, n_kv_heads, head_dim,
  * kv_dtype, n_heads, max_seqs, max_tokens, max_pages} whose captured calls
  * launch `classes` of the attention's kernels (a bit each, the first always)
- * and captured_tokens tokens. Writes the tokens [n][4] (row of the cache,
+ * and captured_tokens tokens, with a table of captured_positions. Writes the tokens [n][4] (row of the cache,
  * position, sequence, place), what those of trees see [n][4], the attention's
  * items [..][9] (the sequence's first token, tokens, context, first page,
  * whether it is a tree; first row, first position, end, first slab), its joins
  * [..][6] (first token, rows, first row, first slab, parts, slabs of a part),
  * of which *n_items and *n_joins say how many there is room for, then are, and
  * the classes' first items [4]. */
-TH_API int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tokens, size_t n_seqs,
-                             const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
+TH_API int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tokens, size_t captured_positions,
+                             size_t n_seqs, const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
                              const int32_t *parents, uint32_t *tokens, uint64_t *tree, uint32_t *items, size_t *n_items,
                              uint32_t *joins, size_t *n_joins, uint32_t *first);
 

@@ -525,6 +525,49 @@ def test_captured_calls_take_any_step(hip, at, kv):
     graph.free()
 
 
+@gpu
+def test_two_captured_batches_of_calls(hip):
+    """A graph captured with a long and a short sequence and one with 21 single
+    tokens, over one batch and tables of 100 and 102 positions: both take any
+    step that is set later, in turn and with eager calls between, and none is
+    set whose replay would read past a table or have more tokens."""
+    r = np.random.default_rng(18)
+    heads, kvh, hd, page, tokens = 16, 8, 128, 16, 30
+    steps = [Step(r, c, n, page, None, spare=0) for c, n in [([20, 3], [25, 5]), ([99], [1]), ([0, 70], [3, 18]), ([4] * 21, [1] * 21)]]
+    most = max(s.pages for s in steps)
+    pool = pool_of(r, most, page, kvh, hd, TH_KV_F32)
+    cache = cache_of(hip, pool, TH_KV_F32)
+    batch = hip.alloc_batch(cache, heads, 21, tokens, most)
+    q, k, v = (r.standard_normal((tokens, h, hd), dtype=np.float32) for h in (heads, kvh, kvh))
+    rope, long_rope = buf(hip, rope_table(100, hd)), buf(hip, rope_table(102, hd))
+    graphs = []
+    for step, table in [(steps[0], rope), (steps[3], long_rope)]:
+        step.set(hip, batch)
+        x = [buf(hip, a[:step.tokens]) for a in (q, k, v)]
+        out = hip.alloc(len(x[0]))
+        hip.graph_begin()
+        hip.paged_append(x[0], x[0], x[1], x[2], None, None, table, cache, batch, EPS)
+        hip.paged_attention(out, x[0], cache, batch)
+        graphs.append((hip.graph_end(), x, out))
+    for again in range(2):
+        for step in steps[:0:-1] if again else steps[1:]:
+            step.set(hip, batch)
+            now = [buf(hip, a[:step.tokens]) for a in (q, k, v)]
+            eager = hip.alloc(len(now[0]))
+            hip.paged_append(now[0], now[0], now[1], now[2], None, None, rope, cache, batch, EPS)
+            hip.paged_attention(eager, now[0], cache, batch)
+            want = hip.read(eager)
+            for graph, x, out in graphs:
+                hip.write(x[0], q.ravel()[:len(x[0])])
+                graph.launch()
+                assert np.array_equal(hip.read(out)[:want.size], want)
+    for context, new, what in [([100], [1], "position 100"), ([98, 99], [1, 2], "position 100"), ([0], [22], "captured with this batch at 21")]:
+        with pytest.raises(InvalidArgument, match=what):
+            hip.set_batch(batch, context, new, range(sum(-(-(c + n) // page) for c, n in zip(context, new))))
+    for graph, *_ in graphs:
+        graph.free()
+
+
 # ---- refusals ----
 
 @gpu

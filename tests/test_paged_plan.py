@@ -22,9 +22,9 @@ SPLIT_BLOCKS = 2048  # the most of a class's blocks where it is split
 
 
 def batch_set(context, new, pages, parents=None, cache=(64, 16, 2, 128), bf16=False, heads=4, room=(8, 400, 64), classes=ALL,
-              captured=1 << 62):
+              captured=1 << 62, table=1 << 62):
     f = C.CDLL(str(LIB_PATH)).th_test_batch_set
-    f.argtypes = [C.c_void_p, C.c_uint, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+    f.argtypes = [C.c_void_p, C.c_uint, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
                   C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t), C.c_void_p, C.POINTER(C.c_size_t), C.c_void_p]
     shape = (C.c_size_t * 9)(*cache, int(bf16), heads, *room)
     c, n, p = (np.array(x, np.uint32) for x in (context, new, pages))
@@ -34,8 +34,8 @@ def batch_set(context, new, pages, parents=None, cache=(64, 16, 2, 128), bf16=Fa
     most = total * 16 + 4 * len(new) + 4 * SPLIT_BLOCKS
     items, joins, first = np.zeros((most, 9), np.uint32), np.zeros((most, 6), np.uint32), np.zeros(4, np.uint32)
     n_items, n_joins = C.c_size_t(most), C.c_size_t(most)
-    check(f(shape, classes, captured, len(c), c.ctypes.data, n.ctypes.data, p.ctypes.data, len(p), None if t is None else t.ctypes.data,
-            tokens.ctypes.data, tree.ctypes.data, items.ctypes.data, C.byref(n_items), joins.ctypes.data, C.byref(n_joins),
+    check(f(shape, classes, captured, table, len(c), c.ctypes.data, n.ctypes.data, p.ctypes.data, len(p),
+            None if t is None else t.ctypes.data, tokens.ctypes.data, tree.ctypes.data, items.ctypes.data, C.byref(n_items), joins.ctypes.data, C.byref(n_joins),
             first.ctypes.data))
     return tokens, tree, items[:n_items.value], joins[:n_joins.value], first
 
@@ -59,6 +59,11 @@ def batch_set(context, new, pages, parents=None, cache=(64, 16, 2, 128), bf16=Fa
     ("parent 0 of token 0 of sequence 1", dict(context=[0, 0], new=[2, 1], pages=[0, 1], parents=[-1, 0, 0])),
     ("a tree of 257 tokens", dict(context=[0], new=[257], pages=range(17), parents=[-1] * 257)),
     ("captured with this batch at 9", dict(context=[0], new=[10], pages=[0], captured=9)),
+    ("position 40: a graph", dict(context=[3, 40, 0], new=[1, 1, 2], pages=[0, 1, 2, 3, 4], table=40)),
+    ("position 12: a graph", dict(context=[10], new=[4], pages=[0], parents=[-1, 0, 1, 0], table=12)),
+    ("position 13: a graph", dict(context=[10], new=[4], pages=[0], parents=[-1, 0, 1, 2], table=13)),
+    ("1073741825 positions of sequence 1", dict(context=[0, 1 << 30], new=[1, 1], pages=[1] + [0] * ((1 << 22) + 1),
+                                                cache=(64, 256, 2, 128), room=(8, 400, 1 << 23))),
 ])
 def test_refused(what, args):
     with pytest.raises(InvalidArgument, match=what):
@@ -72,6 +77,9 @@ def test_allowed():
     batch_set([0], [400], range(25), parents=[i - 1 for i in range(400)])  # a chain, however long
     batch_set([0], [256], range(16), parents=[-1] * 256)
     batch_set([0], [9], [0], captured=9)
+    batch_set([3, 39, 60], [1, 1, 0], range(8), captured=2, table=40)  # what has no tokens is not rotated
+    batch_set([10], [4], [0], parents=[-1, 0, 1, 0], table=13)
+    batch_set([(1 << 30) - 1], [1], [0] * ((1 << 22) - 1) + [1], cache=(64, 256, 2, 128), room=(8, 400, 1 << 23))
 
 
 def test_tokens_and_trees():

@@ -19,6 +19,7 @@ namespace th {
 constexpr size_t kTreeTokens = 256;  // drafted tokens of one sequence's tree
 constexpr int kTreeWords = (int)kTreeTokens / 64;
 constexpr size_t kPagedMaxGroup = 16;  // query heads per KV head
+constexpr size_t kMostPositions = (size_t)1 << 30;  // of a sequence, whose kernels count in 32 bits
 
 // What the kernels read of a batch. A token: the row of the cache that it is
 // written to (page * page_len + row), the position of its rotation, its
@@ -157,8 +158,9 @@ struct th_batch {
     // Of what is set: sequences, tokens, entries of pages, the positions that a
     // rotation's table holds at least.
     size_t n_seqs = 0, n_tokens = 0, n_pages = 0, positions = 0;
-    // The fewest tokens that a captured call was launched for.
-    size_t captured_tokens = SIZE_MAX;
+    // The fewest tokens that a captured call was launched for, and the fewest
+    // positions that a rotation's table of one holds.
+    size_t captured_tokens = SIZE_MAX, captured_positions = SIZE_MAX;
     // The classes of the attention's items that every captured call launches.
     unsigned classes = (1u << th::kClasses) - 1;
     char *device = nullptr, *pinned = nullptr;

@@ -89,6 +89,7 @@ int check_set(th_batch *b, size_t n_seqs, const uint32_t *context, const uint32_
         tokens += n_new[s];
         TH_REQUIRE(entries <= n_pages, "sequence %zu of %zu positions is past the end of %zu pages", s, len, n_pages);
         TH_REQUIRE(tokens <= b->max_tokens, "%zu tokens up to sequence %zu, a batch of at most %zu", tokens, s, b->max_tokens);
+        TH_REQUIRE(len <= th::kMostPositions, "%zu positions of sequence %zu: at most %zu", len, s, th::kMostPositions);
     }
     TH_REQUIRE(entries == n_pages, "%zu pages for sequences of %zu", n_pages, entries);
     TH_REQUIRE(tokens <= b->captured_tokens,
@@ -116,15 +117,25 @@ int check_set(th_batch *b, size_t n_seqs, const uint32_t *context, const uint32_
             TH_REQUIRE(b->stamp[pages[p]] != b->epoch, "page %u gets new rows, and is in the context of sequence %zu", pages[p], s);
         p0 = end;
     }
-    for (size_t s = 0, t0 = 0; parents && s < n_seqs; t0 += n_new[s++]) {
+    size_t positions = 0;  // that are rotated by
+    for (size_t s = 0, t0 = 0; s < n_seqs; t0 += n_new[s++]) {
         bool chain = true;
-        for (size_t i = 0; i < n_new[s]; ++i) {
+        for (size_t i = 0; parents && i < n_new[s]; ++i) {
             TH_REQUIRE(parents[t0 + i] >= -1 && parents[t0 + i] < (int64_t)i, "parent %d of token %zu of sequence %zu",
                        parents[t0 + i], i, s);
             chain = chain && parents[t0 + i] == (int64_t)i - 1;
         }
         TH_REQUIRE(chain || n_new[s] <= th::kTreeTokens, "a tree of %u tokens: at most %zu", n_new[s], th::kTreeTokens);
+        size_t deep = chain ? n_new[s] : 0, level[th::kTreeTokens];
+        for (size_t i = 0; !chain && i < n_new[s]; ++i) {
+            level[i] = parents[t0 + i] < 0 ? 1 : level[parents[t0 + i]] + 1;
+            deep = std::max(deep, level[i]);
+        }
+        if (n_new[s]) positions = std::max(positions, context[s] + deep);
     }
+    TH_REQUIRE(positions <= b->captured_positions,
+               "position %zu: a graph was captured with this batch over a table of %zu, past whose end it would read",
+               positions - 1, b->captured_positions);
     return TH_OK;
 }
 
@@ -215,12 +226,14 @@ bool arrive(const uint64_t *words, size_t n) {
     return true;
 }
 
-// A captured call is launched for the tokens that are set now: later sets may
-// have fewer, not more.
-void note_capture(const th_device *dev, const th_batch *batch) {
+// A captured call is launched for the tokens that are set now, and an append
+// reads the table it was given: later sets may have no more tokens, and none
+// that are rotated by a position past the table's end.
+void note_capture(const th_device *dev, const th_batch *batch, size_t positions = SIZE_MAX) {
     if (!dev->capturing) return;
     auto *b = const_cast<th_batch *>(batch);
     b->captured_tokens = std::min(b->captured_tokens, b->n_tokens);
+    b->captured_positions = std::min(b->captured_positions, positions);
 }
 
 }  // namespace
@@ -414,14 +427,15 @@ int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q, const 
                "q and q_out hold %zu and %zu activations, not %zu tokens of %zu x %zu", q->len, q_out->len, n, b->n_heads, hd);
     TH_REQUIRE(k->len == n * b->n_kv_heads * hd && v->len == k->len,
                "k and v hold %zu and %zu activations, not %zu tokens of %zu x %zu", k->len, v->len, n, b->n_kv_heads, hd);
-    TH_REQUIRE(n == 0 || (q_out->ptr != k->ptr && q_out->ptr != v->ptr), "q_out may be q, not k or v");
+    TH_REQUIRE(n == 0 || (q_out->ptr != k->ptr && q_out->ptr != v->ptr && q_out->ptr != rope->ptr),
+               "q_out may be q, not k, v or the table");
     TH_REQUIRE((!q_norm || q_norm->numel == hd) && (!k_norm || k_norm->numel == hd), "q/k norms hold head_dim gains");
     TH_REQUIRE(b->positions * hd <= rope->len, "position %zu is past the end of the table", b->positions - 1);
     TH_PAGED_CURRENT(dev);
     th::PagedAppendArgs a{b->view(), q_out->ptr, q->ptr, k->ptr, v->ptr, q_norm ? q_norm->ptr : nullptr,
                           k_norm ? k_norm->ptr : nullptr, rope->ptr, c->ptr, (int)b->n_heads, (int)b->n_kv_heads, eps};
     TH_HIP(th::launch_paged_append(dev->stream, a, n, hd, c->kv_dtype == TH_KV_BF16));
-    note_capture(dev, b);
+    note_capture(dev, b, rope->len / hd);
     return TH_OK;
 }
 
@@ -555,9 +569,10 @@ int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, cons
     return TH_OK;
 }
 
-int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tokens, size_t n_seqs, const uint32_t *context,
-                      const uint32_t *n_new, const uint32_t *pages, size_t n_pages, const int32_t *parents, uint32_t *tokens,
-                      uint64_t *tree, uint32_t *items, size_t *n_items, uint32_t *joins, size_t *n_joins, uint32_t *first) {
+int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tokens, size_t captured_positions, size_t n_seqs,
+                      const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
+                      const int32_t *parents, uint32_t *tokens, uint64_t *tree, uint32_t *items, size_t *n_items,
+                      uint32_t *joins, size_t *n_joins, uint32_t *first) {
     th_batch b;
     b.pages = shape[0];
     b.page_len = shape[1];
@@ -570,6 +585,7 @@ int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tok
     b.max_pages = shape[8];
     b.classes = classes;
     b.captured_tokens = captured_tokens;
+    b.captured_positions = captured_positions;
     size_t bytes = 0;
     const bool held = place_arrays(&b, &bytes) && (b.pinned = static_cast<char *>(calloc(1, bytes)));
     int rc = held ? check_set(&b, n_seqs, context, n_new, pages, n_pages, parents) : fail(TH_ERR_NOMEM, "out of host memory");
