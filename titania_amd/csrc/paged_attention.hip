@@ -95,6 +95,11 @@ __device__ __forceinline__ uint32_t seen16(const SeqAt &seq, const uint64_t *tre
 // 64 KB of f32 keys and values take a CU's share of HBM 8000: 16 rows cost what
 // one costs. (With more sets of 16 a wave, 17 to 64 rows took 1.3 to 1.7 times
 // what the kernel for many rows takes for them.)
+//
+// Bound by HBM: one token at 32767, 16 / 8 heads, f32, 53.5 us with the join
+// (268 MB at 5.0 TB/s); 64 tokens at 120 to 8000, 32 / 8 heads, bf16, 202 us
+// (5.3 TB/s). One token at 40 takes 5.8 us: a launch, the item, its page, its
+// rows and two chains of products, each of which waits for the one before.
 template <int HD, typename KV>
 __global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a, Launch launch) {
     constexpr int VE = 16 / sizeof(KV);         // values of 16 bytes
@@ -381,7 +386,25 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // Where a tile has an infinity or a NaN, or where rows do not see all positions
 // and these differ by more than 2^12, the item is done again from memory, in
 // f32, a position at a time and each row for itself: what it does not see does
-// not reach it. (Some 3 us a position: these are no numbers to be fast with.)
+// not reach it. (These are no numbers to be fast with.)
+//
+// Bound by the matrix units, at what they and the conversions leave each other:
+// chunks of 2048, 1946 and 1592 tokens at 2500, 0 and 5000, 32 / 8 heads, f32,
+// take 0.82 ms, products at 1.06 to 1.1 PFLOP/s, the units busy half of the time
+// (a large matrix product of a library: 1.24 PFLOP/s). That case, step by step:
+// f32 products 3.87 ms; two f16 terms 1.60; one exponent for a tile's keys and
+// maxima by lane exchanges 1.12; rows swizzled in LDS, not padded, 1.07;
+// remainders by one mixed-precision fma, maxima of three 0.98; references that
+// move by 2^5 only 0.95; products before other waves' conversions 0.91; the
+// longest items first 0.85; half of the waves converting between their halves
+// of a tile 0.81. A tree of 60 tokens at 12001 takes 55 to 59 us, 8.5 of them
+// the join: 256 blocks of 6 tiles of 5.6 us, and 34 MB of partial results.
+// Not kept: two groups of four waves that halve a tile's positions, for up to
+// 64 rows (bf16 41 -> 44 us, f32 66 -> 63); 256 rows as two tiles of 128, which
+// is faster for that tree over f32 at 1900 (31.5 -> 27.3 us), equal at 8100 and
+// slower past it (at 48800 169 -> 199) and over bf16; two tiles requested ahead
+// (no change); blocks' rows on turned waves, so that the few that have some
+// share the SIMDs (no change).
 template <int HD, int SETS, typename KV>
 __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2) void paged_many_kernel(PagedAttnArgs a, Launch launch) {
     constexpr bool F32 = sizeof(KV) == 4;
@@ -860,7 +883,8 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
 }
 
 // Joins a split tile's parts, `W` waves a row: four for few rows of many parts,
-// which then wait for a quarter of them, one for many rows.
+// which then wait for a quarter of them, one for many rows (1920 rows of 32
+// parts, 32 MB, 8.5 us; 16 rows of 64 parts 4.9).
 template <int HD, int W>
 __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, const BatchHead &head) {
     constexpr int E = HD / 64, ROWS = 4 / W;  // a block's rows
