@@ -1,5 +1,6 @@
 /*
- * titania_hip_test_paged.h: for tests/test_paged_plan.py alone: what
+ * titania_hip_test_paged.h: for tests/test_paged.py and tests/test_paged_plan.py
+ * alone: the attention's kernels where a plan would take others, and what
  * th_batch_set checks and plans, without a GPU.
  */
 #ifndef TITANIA_HIP_TEST_PAGED_H
@@ -10,6 +11,11 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* Later sets plan for these kernels (a bit each: tiles of 16 rows, always, of 128
+ * and of 256), each for the sequences of 1 to 16, to 128 and of more rows, and for
+ * the others the next there is, whatever would be fastest. */
+TH_API int th_test_batch_classes(th_batch *batch, unsigned classes);
 
 /* th_batch_set for a batch of shape {pages, page_len, n_kv_heads, head_dim,
  * kv_dtype, n_heads, max_seqs, max_tokens, max_pages} whose captured calls

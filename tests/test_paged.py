@@ -21,6 +21,8 @@ import numpy as np
 import pytest
 
 from titania_amd import TH_KV_BF16, TH_KV_F32, Hip, InvalidArgument, Tensor
+from titania_amd._lib import LIB_PATH
+from titania_amd._lib import check as ok
 from titania_amd.synth import bf16_to_f32, f32_to_bf16
 
 EPS = 1e-6
@@ -34,6 +36,20 @@ def chain(n):
 
 def some_tree(r, n, back=6, roots=False):
     return [-1 if i == 0 or (roots and r.random() < 0.1) else int(r.integers(max(0, i - back), i)) for i in range(n)]
+
+
+@pytest.fixture(params=[0, 7, 5])
+def kernels(request):
+    """Of the attention: those that the plan takes; each for the rows that it is
+    made for; the one for up to 256 rows where the plan takes that for 128."""
+    return request.param
+
+
+def take(batch, kernels):
+    if kernels:
+        f = C.CDLL(str(LIB_PATH)).th_test_batch_classes
+        f.argtypes = [C.c_void_p, C.c_uint]
+        ok(f(batch.handle, kernels))
 
 
 class Step:
@@ -71,8 +87,9 @@ class Step:
         hip.set_batch(batch, self.context, self.new, [p for l in self.lists for p in l],
                       self.parents if self.has_parents else None)
 
-    def batch(self, hip, cache, heads, spare=0):
+    def batch(self, hip, cache, heads, spare=0, kernels=0):
         b = hip.alloc_batch(cache, heads, len(self.new) + spare, max(1, self.tokens) + spare, max(1, sum(map(len, self.lists))) + spare)
+        take(b, kernels)
         self.set(hip, b)
         return b
 
@@ -145,9 +162,9 @@ def check(got, want, tol, what=""):
     assert (off <= most).all(), f"{what}: {(off > most).sum()} of {off.size} off, by up to {np.max(off / most)} of the bound"
 
 
-def run_attention(hip, step, q, pool, heads, kv):
+def run_attention(hip, step, q, pool, heads, kv, kernels=0):
     cache = cache_of(hip, pool, kv)
-    batch = step.batch(hip, cache, heads)
+    batch = step.batch(hip, cache, heads, kernels=kernels)
     bq, out = buf(hip, q), buf(hip, np.full(q.size, 7, np.float32))
     hip.paged_attention(out, bq, cache, batch)
     return hip.read(out).reshape(q.shape)
@@ -165,46 +182,46 @@ SHAPES = [(16, 8, 128), (32, 8, 128), (4, 2, 128), (8, 1, 128), (3, 3, 64), (16,
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("lengths", range(len(LENGTHS)))
-def test_attention_lengths(hip, lengths, kv):
+def test_attention_lengths(hip, lengths, kv, kernels):
     r = np.random.default_rng(lengths)
     heads, kvh, hd = SHAPES[lengths % 3]
     step = Step(r, *LENGTHS[lengths], [16, 32, 64][lengths % 3])
     pool = pool_of(r, step.pages, step.L, kvh, hd, kv)
     q = r.standard_normal((step.tokens, heads, hd), dtype=np.float32)
-    check(run_attention(hip, step, q, pool, heads, kv), *attention64(step, q, pool, heads))
+    check(run_attention(hip, step, q, pool, heads, kv, kernels), *attention64(step, q, pool, heads))
 
 
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("page", [16, 256])
 @pytest.mark.parametrize("heads,kvh,hd", SHAPES)
-def test_attention_shapes(hip, heads, kvh, hd, page, kv):
+def test_attention_shapes(hip, heads, kvh, hd, page, kv, kernels):
     r = np.random.default_rng(heads * 31 + hd + page)
     step = Step(r, [100, 0, 31], [1, 40, 3], page, shared=1)
     pool = pool_of(r, step.pages, page, kvh, hd, kv)
     q = r.standard_normal((step.tokens, heads, hd), dtype=np.float32)
-    check(run_attention(hip, step, q, pool, heads, kv), *attention64(step, q, pool, heads))
+    check(run_attention(hip, step, q, pool, heads, kv, kernels), *attention64(step, q, pool, heads))
 
 
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("heads,kvh,hd", [(16, 8, 128), (32, 8, 128), (8, 1, 64), (6, 2, 256)])
 @pytest.mark.parametrize("new", [2, 9, 25, 64, 65, 256])
-def test_attention_trees(hip, new, heads, kvh, hd, kv):
+def test_attention_trees(hip, new, heads, kvh, hd, kv, kernels):
     r = np.random.default_rng(new * 7 + heads)
     context, counts = [130, 0, 57], [new, max(1, new // 2), 1]
     trees = [some_tree(r, new, back=new, roots=True), some_tree(r, counts[1]), None]
     step = Step(r, context, counts, 16, trees)
     pool = pool_of(r, step.pages, 16, kvh, hd, kv)
     q = r.standard_normal((step.tokens, heads, hd), dtype=np.float32)
-    check(run_attention(hip, step, q, pool, heads, kv), *attention64(step, q, pool, heads))
+    check(run_attention(hip, step, q, pool, heads, kv, kernels), *attention64(step, q, pool, heads))
 
 
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("heads,new", [(16, 5), (32, 30), (32, 90)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38, -1e20])
-def test_what_is_not_seen_does_not_count(hip, heads, new, bad, kv):
+def test_what_is_not_seen_does_not_count(hip, heads, new, bad, kv, kernels):
     """Rows behind the last position, and drafted tokens of other branches, hold
     NaN, infinities, or numbers beside which the others are nothing."""
     r = np.random.default_rng(new)
@@ -228,7 +245,7 @@ def test_what_is_not_seen_does_not_count(hip, heads, new, bad, kv):
     touched = np.zeros((step.tokens, heads), bool)
     for s, i in ((0, new - 2), (1, new - 1)):
         touched[step.first[s]:step.first[s] + new, 3 * group:4 * group] |= step.sees[s][:, i:i + 1]
-    got = run_attention(hip, step, q, pool, heads, kv)
+    got = run_attention(hip, step, q, pool, heads, kv, kernels)
     assert np.isfinite(got[~touched][:, :17]).all() and np.isfinite(got[~touched][:, 18:]).all()
     check(got[~touched], want[~touched], tol[~touched])
     # Where a key that is seen has such values, so has the result.
@@ -239,7 +256,7 @@ def test_what_is_not_seen_does_not_count(hip, heads, new, bad, kv):
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("new", [1, 20, 70])
 @pytest.mark.parametrize("scale", [1e-18, 1e-3, 30.0, 1e15])
-def test_attention_of_large_and_small_values(hip, scale, new, kv):
+def test_attention_of_large_and_small_values(hip, scale, new, kv, kernels):
     """Values and keys far from one: keys times `scale`, queries by its inverse, values by it."""
     r = np.random.default_rng(new)
     step = Step(r, [150], [new], 64)
@@ -247,13 +264,13 @@ def test_attention_of_large_and_small_values(hip, scale, new, kv):
     if kv == TH_KV_BF16:
         pool = bf16_to_f32(f32_to_bf16(pool))
     q = r.standard_normal((step.tokens, 8, 128), dtype=np.float32) / np.float32(scale)
-    check(run_attention(hip, step, q, pool, 8, kv), *attention64(step, q, pool, 8))
+    check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
 
 
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("new", [1, 12, 80])
-def test_attention_of_sharp_and_flat_scores(hip, new, kv):
+def test_attention_of_sharp_and_flat_scores(hip, new, kv, kernels):
     """Scores of hundreds (one key has it all) and of zero (an average)."""
     r = np.random.default_rng(new + 5)
     step = Step(r, [333], [new], 16)
@@ -261,19 +278,19 @@ def test_attention_of_sharp_and_flat_scores(hip, new, kv):
     q = r.standard_normal((step.tokens, 8, 128), dtype=np.float32)
     q[:, ::2] *= 60
     q[:, 1::4] = 0
-    check(run_attention(hip, step, q, pool, 8, kv), *attention64(step, q, pool, 8))
+    check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
 
 
 @gpu
 @pytest.mark.parametrize("heads,kvh,context,new,kv", [(16, 8, [33000], [1], TH_KV_F32), (32, 8, [9000], [60], TH_KV_F32),
                                                       (32, 8, [5000, 12, 2100], [7, 1, 300], TH_KV_BF16),
                                                       (8, 8, [20000, 100], [2, 1], TH_KV_BF16), (4, 4, [6000], [256], TH_KV_F32)])
-def test_attention_of_long_contexts(hip, heads, kvh, context, new, kv):
+def test_attention_of_long_contexts(hip, heads, kvh, context, new, kv, kernels):
     r = np.random.default_rng(sum(context))
     step = Step(r, context, new, 64, [some_tree(r, n) if n <= 60 else None for n in new])
     pool = pool_of(r, step.pages, 64, kvh, 128, kv)
     q = r.standard_normal((step.tokens, heads, 128), dtype=np.float32)
-    check(run_attention(hip, step, q, pool, heads, kv), *attention64(step, q, pool, heads))
+    check(run_attention(hip, step, q, pool, heads, kv, kernels), *attention64(step, q, pool, heads))
 
 
 @gpu
@@ -288,7 +305,7 @@ def test_attention_past_32_bits(hip):
     for i, p in enumerate([8999, 1, 8998, 8500]):
         hip.write_paged(cache, p, pool[i, 0], pool[i, 1])
     q = r.standard_normal((73, 16, 128), dtype=np.float32)
-    batch = step.batch(hip, cache, 16)
+    batch = step.batch(hip, cache, 16, kernels=7)
     bq, out = buf(hip, q), hip.alloc(q.size)
     hip.paged_attention(out, bq, cache, batch)
     got = hip.read(out).reshape(q.shape)
@@ -484,7 +501,7 @@ def test_keep(hip, layers, kvh, hd, page, context, new, kv):
 @gpu
 @pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
 @pytest.mark.parametrize("at", [([100, 7], [60, 13]), ([2] * 73, [1] * 73)])
-def test_captured_calls_take_any_step(hip, at, kv):
+def test_captured_calls_take_any_step(hip, at, kv, kernels):
     """One graph of an append and an attention, captured with two trees or with
     73 single tokens, over steps of other lengths, pages and trees, with the same
     calls run eagerly between the replays."""
@@ -496,6 +513,7 @@ def test_captured_calls_take_any_step(hip, at, kv):
     pool = pool_of(r, most, page, kvh, hd, kv)
     cache = cache_of(hip, pool, kv)
     batch = hip.alloc_batch(cache, heads, 73, tokens + 1, most)
+    take(batch, kernels)
     q, k, v = (r.standard_normal((tokens, h, hd), dtype=np.float32) for h in (heads, kvh, kvh))
     bq, bk, bv = buf(hip, q), buf(hip, k), buf(hip, v)
     gain = hip.upload(Tensor((hd,), f32_to_bf16(1 + 0.1 * r.standard_normal(hd).astype(np.float32))))
@@ -526,7 +544,7 @@ def test_captured_calls_take_any_step(hip, at, kv):
 
 
 @gpu
-def test_two_captured_batches_of_calls(hip):
+def test_two_captured_batches_of_calls(hip, kernels):
     """A graph captured with a long and a short sequence and one with 21 single
     tokens, over one batch and tables of 100 and 102 positions: both take any
     step that is set later, in turn and with eager calls between, and none is
@@ -538,6 +556,7 @@ def test_two_captured_batches_of_calls(hip):
     pool = pool_of(r, most, page, kvh, hd, TH_KV_F32)
     cache = cache_of(hip, pool, TH_KV_F32)
     batch = hip.alloc_batch(cache, heads, 21, tokens, most)
+    take(batch, kernels)
     q, k, v = (r.standard_normal((tokens, h, hd), dtype=np.float32) for h in (heads, kvh, kvh))
     rope, long_rope = buf(hip, rope_table(100, hd)), buf(hip, rope_table(102, hd))
     graphs = []

@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_paged import EPS, Step, attention64, buf, cache_of, check, pool_of, rope_table, some_tree
+from test_paged import EPS, Step, attention64, buf, cache_of, check, pool_of, rope_table, some_tree, take
 from titania_amd import TH_KV_BF16, TH_KV_F32, Hip
 
 gpu = pytest.mark.gpu
@@ -79,6 +79,7 @@ def test_as_many_heads_as_a_batch_takes(hip, seqs, new):
     per = -(-new // page)
     cache = hip.alloc_paged(seqs * per, page, kvh, hd, TH_KV_BF16)
     batch = hip.alloc_batch(cache, heads, seqs, seqs * new, seqs * per)
+    take(batch, 7)
     pages = np.arange(seqs * per, dtype=np.uint32)[::-1]
     hip.set_batch(batch, np.zeros(seqs, np.uint32), np.full(seqs, new, np.uint32), pages)
     q, k, v = (r.standard_normal((same, new, h, hd), dtype=np.float32) for h in (heads, kvh, kvh))

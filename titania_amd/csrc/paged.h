@@ -79,10 +79,14 @@ struct PlanShape {
     size_t n_kv_heads, head_dim, group, max_items, max_joins;
     bool bf16;
     unsigned classes;  // a bit for each class that may be used: the first always
+    bool all_classes;  // each is, for the rows it is made for, whatever the estimate (tests)
 };
 // The most items and split tiles of a batch.
 size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens);
 size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens);
+// The classes that a captured call launches: those of the sequences' rows, which
+// other lengths may want, those of the plan, and the first.
+unsigned classes_of(const PlanShape &shape, const BatchHead &head, const SeqAt *seqs);
 // Plans the attention of the head's sequences.
 void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins);
 
@@ -109,10 +113,10 @@ struct PagedAttnArgs {
     float scale;
     float *part;  // slabs
 };
-// `count`: what is set now, to be launched for. `captured`: what is set later is
-// launched for too, by the classes that are set now and the first.
+// `count`: what is set now, to be launched for. `captured`: not zero where what is
+// set later is launched for too, by these classes.
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, size_t head_dim, bool bf16,
-                                  bool captured);
+                                  unsigned captured);
 
 // picks[row * splits + split] = the packed argmax of a part of a row.
 hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, int splits, uint64_t *picks);
@@ -163,6 +167,7 @@ struct th_batch {
     size_t captured_tokens = SIZE_MAX, captured_positions = SIZE_MAX;
     // The classes of the attention's items that every captured call launches.
     unsigned classes = (1u << th::kClasses) - 1;
+    bool all_classes = false;
     char *device = nullptr, *pinned = nullptr;
     // Offsets, the same in both.
     size_t at_seqs = 0, at_tokens = 0, at_pages = 0, at_tree = 0, at_items = 0, at_joins = 0;
@@ -176,7 +181,7 @@ struct th_batch {
     uint32_t *page_list() const { return reinterpret_cast<uint32_t *>(pinned + at_pages); }
     th::PlanShape plan_shape() const {
         return {n_kv_heads, head_dim, n_heads / n_kv_heads, th::most_items(n_heads, n_kv_heads, max_seqs, max_tokens),
-                th::most_joins(n_heads, n_kv_heads, max_seqs, max_tokens), kv_dtype == TH_KV_BF16, classes};
+                th::most_joins(n_heads, n_kv_heads, max_seqs, max_tokens), kv_dtype == TH_KV_BF16, classes, all_classes};
     }
     th::BatchView view() const {
         return {reinterpret_cast<const th::BatchHead *>(device),

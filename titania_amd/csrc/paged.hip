@@ -449,13 +449,10 @@ int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const
     TH_PAGED_CURRENT(dev);
     th::PagedAttnArgs a{b->view(), out->ptr, q->ptr, c->ptr, (int)b->n_heads, (int)b->n_kv_heads,
                         (int)(b->n_heads / b->n_kv_heads), 1.0f / sqrtf((float)hd), dev->part};
-    TH_HIP(th::launch_paged_attention(dev->stream, a, *b->head(), hd, c->kv_dtype == TH_KV_BF16, dev->capturing));
+    const unsigned captured = dev->capturing ? th::classes_of(b->plan_shape(), *b->head(), b->seqs()) : 0;
+    TH_HIP(th::launch_paged_attention(dev->stream, a, *b->head(), hd, c->kv_dtype == TH_KV_BF16, captured));
     note_capture(dev, b);
-    if (dev->capturing) {
-        unsigned launched = 1;
-        for (int i = 0; i < th::kClasses; ++i) launched |= (b->head()->first[i + 1] > b->head()->first[i]) << i;
-        const_cast<th_batch *>(b)->classes &= launched;
-    }
+    if (captured) const_cast<th_batch *>(b)->classes &= captured;
     return TH_OK;
 }
 
@@ -566,6 +563,13 @@ int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, cons
         }
     }
     TH_HIP(flush());
+    return TH_OK;
+}
+
+int th_test_batch_classes(th_batch *b, unsigned classes) {
+    TH_REQUIRE(b && classes < 1u << th::kClasses && classes & 1, "th_test_batch_classes: %u", classes);
+    b->classes = classes;
+    b->all_classes = true;
     return TH_OK;
 }
 

@@ -400,11 +400,9 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // of a tile 0.81. A tree of 60 tokens at 12001 takes 55 to 59 us, 8.5 of them
 // the join: 256 blocks of 6 tiles of 5.6 us, and 34 MB of partial results.
 // Not kept: two groups of four waves that halve a tile's positions, for up to
-// 64 rows (bf16 41 -> 44 us, f32 66 -> 63); 256 rows as two tiles of 128, which
-// is faster for that tree over f32 at 1900 (31.5 -> 27.3 us), equal at 8100 and
-// slower past it (at 48800 169 -> 199) and over bf16; two tiles requested ahead
-// (no change); blocks' rows on turned waves, so that the few that have some
-// share the SIMDs (no change).
+// 64 rows (bf16 41 -> 44 us, f32 66 -> 63); two tiles requested ahead, or the
+// first one before the queries are converted (no change); blocks' rows on turned
+// waves, so that the few that have some share the SIMDs (no change).
 template <int HD, int SETS, typename KV>
 __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2) void paged_many_kernel(PagedAttnArgs a, Launch launch) {
     constexpr bool F32 = sizeof(KV) == 4;
@@ -979,11 +977,11 @@ hipError_t many(hipStream_t s, const PagedAttnArgs &a, const Launch &l, unsigned
 }
 
 template <int HD>
-hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, bool bf16, bool captured) {
+hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, bool bf16, unsigned captured) {
     for (int c = 0; c < kClasses; ++c) {
-        const Launch l{count.first[c], count.first[c + 1] - count.first[c], c, captured};
+        const Launch l{count.first[c], count.first[c + 1] - count.first[c], c, captured != 0};
         const size_t blocks = (size_t)l.n * a.n_kv_heads;
-        if (!blocks && !(captured && c == 0)) continue;
+        if (!blocks && !(captured >> c & 1)) continue;
         // (The few-row kernel's blocks walk the items past 2^22, too.)
         const unsigned grid = c == 0 ? (unsigned)std::min<size_t>(captured ? kCapturedBlocks : blocks, (size_t)1 << 22)
                                      : captured ? captured_blocks(a, count) : (unsigned)blocks;
@@ -1005,7 +1003,7 @@ hipError_t attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &cou
 }  // namespace
 
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, size_t head_dim, bool bf16,
-                                  bool captured) {
+                                  unsigned captured) {
     if (count.n_tokens == 0 && !captured) return hipSuccess;
     return head_dim == 64    ? attention<64>(s, a, count, bf16, captured)
            : head_dim == 128 ? attention<128>(s, a, count, bf16, captured)

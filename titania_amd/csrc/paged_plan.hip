@@ -12,19 +12,42 @@ namespace {
 // or registers hold no more. (Trees of 14 to 25 tokens over bf16, whose class 1
 // fits twice in 128 registers a thread, 50 -> 43 us.)
 constexpr size_t kSlots[kClasses] = {512, 256, 256}, kSlotsBf16[kClasses] = {512, 512, 256};
-// An estimate of a block's time in us, with the chip full of them: for each 64
-// positions, and for the rest of it. (Splits into one round, whatever the
-// lengths, 64 tokens at 120 to 8000 228 -> 209 us, those trees 61 -> 50.)
-constexpr double kStepUs[kClasses] = {5.0, 3.5, 6.0}, kBlockUs[kClasses] = {5.0, 8.0, 10.0};
-// Of the second launch that joins split tiles.
-constexpr double kJoinUs = 5.0;
+// An estimate of a block's time in us: for each 64 positions, alone and with the
+// chip full of others, and for the rest of it and its launch; fitted to measured
+// calls. (Splits into one round, whatever the lengths, 64 tokens at 120 to 8000
+// 228 -> 209 us, those trees 61 -> 50.)
+constexpr double kAloneUs[kClasses] = {1.5, 2.8, 4.5}, kAloneUsBf16[kClasses] = {1.5, 2.5, 3.5};
+constexpr double kFullUs[kClasses] = {5.7, 3.7, 6.0}, kFullUsBf16[kClasses] = {3.2, 4.1, 3.7};
+constexpr double kBlockUs[kClasses] = {5.0, 8.0, 10.0};
+// Of the second launch that joins split tiles, by their class, and the bytes of
+// partial results that are written, or read, in a microsecond.
+constexpr double kJoinUs[kClasses] = {2.5, 6.5, 6.5}, kBytesUs = 6e6;
 // The most rounds of blocks that a class is split into.
 constexpr size_t kRounds = 4;
 static_assert(kRounds * kSlotsBf16[0] <= kMostSplitBlocks && kRounds * kSlotsBf16[1] <= kMostSplitBlocks, "splits");
 // A block's fewest positions: one step of its waves.
 constexpr size_t kStep = 64;
 
+// A sequence takes the smallest class that holds its rows, or the largest there
+// is, with all of its tiles: a few rows that are left over run beside the others.
+int class_of(const PlanShape &shape, size_t rows, unsigned classes) {
+    int best = 0;
+    for (int c = 0; c < kClasses; ++c)
+        if (classes >> c & 1 && (shape.head_dim < 256 || c == 0)) {
+            best = c;
+            if (rows <= (size_t)kClassRows[c]) break;
+        }
+    return best;
+}
+
 }  // namespace
+
+unsigned classes_of(const PlanShape &shape, const BatchHead &head, const SeqAt *seqs) {
+    unsigned classes = 1;
+    for (uint32_t s = 0; s < head.n_seqs; ++s) classes |= 1u << class_of(shape, seqs[s].n_new * shape.group, shape.classes);
+    for (int c = 0; c < kClasses; ++c) classes |= (unsigned)(head.first[c + 1] > head.first[c]) << c;
+    return classes;
+}
 
 size_t most_joins(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max_tokens) {
     return max_tokens * (n_heads / n_kv_heads) / kClassRows[0] + max_seqs;
@@ -35,53 +58,53 @@ size_t most_items(size_t n_heads, size_t n_kv_heads, size_t max_seqs, size_t max
 }
 
 void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, ItemAt *items, JoinAt *joins) {
-    // A sequence takes the smallest class that holds its rows, or the largest
-    // there is, with all of its tiles: a few rows that are left over run beside
-    // the others.
-    auto class_of = [&](size_t rows) {
-        int best = 0;
-        for (int c = 0; c < kClasses; ++c)
-            if (shape.classes >> c & 1 && (shape.head_dim < 256 || c == 0)) {
-                best = c;
-                if (rows <= (size_t)kClassRows[c]) break;
-            }
-        return best;
-    };
     // f(sequence, first row, positions) for each tile of a class, in order.
-    auto each_tile = [&](int c, auto f) {
+    auto each_tile = [&](int c, unsigned classes, auto f) {
         for (uint32_t s = 0; s < head->n_seqs; ++s) {
             const size_t rows = seqs[s].n_new * shape.group;
-            if (rows == 0 || class_of(rows) != c) continue;
+            if (rows == 0 || class_of(shape, rows, classes) != c) continue;
             for (size_t r = 0; r < rows; r += kClassRows[c]) {
                 const size_t end = std::min(rows, r + kClassRows[c]);
                 f(s, (uint32_t)r, (size_t)seqs[s].context + (end - 1) / shape.group + 1);
             }
         }
     };
-    uint32_t n_items = 0, part = 0;
-    const uint32_t parts = (uint32_t)slabs_of(shape.head_dim);
-    head->n_joins = head->join_rows = 0;
-    for (int c = 0; c < kClasses; ++c) {
-        head->first[c] = n_items;
+    // The most steps of a class's items, and an estimate of its time without the
+    // join: as they are, in ceil(blocks / slots) rounds or what the longest first
+    // leaves of them, or such that the blocks fill 1 to kRounds rounds.
+    struct Cut {
+        size_t most;
+        double us;
+        bool split;
+    };
+    auto cut_of = [&](int c, unsigned classes) {
         size_t steps = 0, tiles = 0, longest = 0;
-        each_tile(c, [&](uint32_t, uint32_t, size_t len) {
+        each_tile(c, classes, [&](uint32_t, uint32_t, size_t len) {
             const size_t n = (len + kStep - 1) / kStep;
             steps += n;
             ++tiles;
             longest = std::max(longest, n);
         });
-        if (!tiles) continue;
-        // The most steps of an item: as they are, in ceil(blocks / slots)
-        // rounds or what the longest first leaves of them, or such that the
-        // blocks fill 1 to kRounds rounds.
+        if (!tiles) return Cut{0, 0, false};
         auto items_at = [&](size_t most) {
             size_t items = 0;
-            each_tile(c, [&](uint32_t, uint32_t, size_t len) { items += ((len + kStep - 1) / kStep + most - 1) / most; });
+            each_tile(c, classes, [&](uint32_t, uint32_t, size_t len) { items += ((len + kStep - 1) / kStep + most - 1) / most; });
             return items;
         };
+        // Partial results, written and read once.
+        auto parts_us = [&](size_t most) {
+            size_t rows = 0;
+            each_tile(c, classes, [&](uint32_t s, uint32_t row0, size_t len) {
+                const size_t splits = ((len + kStep - 1) / kStep + most - 1) / most;
+                if (splits > 1) rows += splits * std::min<size_t>(kClassRows[c], seqs[s].n_new * shape.group - row0);
+            });
+            return (double)(rows * shape.n_kv_heads * (shape.head_dim + 2)) * 8 / kBytesUs;
+        };
         const double slots = (double)(shape.bf16 ? kSlotsBf16 : kSlots)[c] / shape.n_kv_heads;  // of items
-        size_t most = longest;
-        double best = std::max((double)longest, steps / slots) * kStepUs[c] + std::max(1.0, tiles / slots) * kBlockUs[c];
+        const double alone = (shape.bf16 ? kAloneUsBf16 : kAloneUs)[c], full = (shape.bf16 ? kFullUsBf16 : kFullUs)[c];
+        auto step_us = [&](double items) { return alone + (full - alone) * std::min(1.0, items / slots); };
+        Cut best{longest, std::max(longest * step_us(tiles), steps / slots * full) + std::max(1.0, tiles / slots) * kBlockUs[c],
+                 false};
         for (size_t r = 1; r <= kRounds; ++r) {
             const size_t room = std::max<size_t>(1, (size_t)(r * slots));
             if (room <= tiles) continue;
@@ -91,13 +114,52 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
                 if (items_at(mid) <= room) high = mid;
                 else low = mid + 1;
             }
-            const double us = r * (low * kStepUs[c] + kBlockUs[c]) + (low < longest ? kJoinUs : 0);
-            if (us < best) {
-                best = us;
-                most = low;
-            }
+            if (low == longest) continue;
+            const double us = r * (low * step_us((double)items_at(low) / r) + kBlockUs[c]) + parts_us(low);
+            if (us + kJoinUs[c] < best.us + (best.split ? kJoinUs[c] : 0)) best = {low, us, true};
         }
-        each_tile(c, [&](uint32_t s, uint32_t row0, size_t len) {
+        return best;
+    };
+    // Each class is a launch, and the launches run one after another; large tiles
+    // have more partial results and a longer start, small ones read keys and values
+    // more often. So fewer classes where that is less, by an estimate that is off
+    // by up to a twentieth. Of 260 mixed batches 61 are cut differently so, and
+    // take 11.8 us where they took 15.7 (geometric means; at worst 1.03 times as
+    // long). f32, 32 / 8 heads, with the smallest class for each and now: 16 trees
+    // of up to 6 tokens at 800 44 -> 35, 24 chunks of up to 38 at 5 to 30 24 -> 12, a
+    // tree of 60 at 300 23 -> 18, at 3900 39 -> 32, and from 8100 on, where tiles of
+    // 128 take as long, then longer (at 48800 199, not 169), as it was.
+    Cut cuts[kClasses] = {};
+    unsigned classes = 0;
+    double least = 0;
+    for (unsigned now : {7u, 3u, 1u}) {
+        now &= shape.classes;
+        bool other = !classes;  // than what there is: without a class that has tiles
+        for (int c = 0; c < kClasses; ++c) other = other || ((classes & ~now) >> c & 1 && cuts[c].most);
+        if (!other) continue;
+        Cut mine[kClasses];
+        double us = 0, join = 0;
+        for (int c = 0; c < kClasses; ++c) {
+            mine[c] = cut_of(c, now);
+            us += mine[c].us;
+            if (mine[c].split) join = std::max(join, kJoinUs[c]);
+        }
+        us += join;
+        if (!classes || us < 0.95 * least) {
+            std::copy(mine, mine + kClasses, cuts);
+            classes = now;
+            least = us;
+        }
+        if (shape.all_classes) break;
+    }
+    uint32_t n_items = 0, part = 0;
+    const uint32_t parts = (uint32_t)slabs_of(shape.head_dim);
+    head->n_joins = head->join_rows = 0;
+    for (int c = 0; c < kClasses; ++c) {
+        head->first[c] = n_items;
+        const size_t most = cuts[c].most;
+        if (!most) continue;
+        each_tile(c, classes, [&](uint32_t s, uint32_t row0, size_t len) {
             const size_t n = (len + kStep - 1) / kStep;
             size_t splits = (n + most - 1) / most;
             const uint32_t slabs = kClassRows[c] / 16, each = slabs * (uint32_t)shape.n_kv_heads;
