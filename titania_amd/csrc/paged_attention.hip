@@ -384,9 +384,11 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // operand of O^T = V^T P^T.
 //
 // Where a tile has an infinity or a NaN, or where rows do not see all positions
-// and these differ by more than 2^12, the item is done again from memory, in
-// f32, a position at a time and each row for itself: what it does not see does
-// not reach it. (These are no numbers to be fast with.)
+// and these differ by more than 2^12 (of a tree's values, over its tiles so
+// far: a row may see none of an earlier tile whose scale is its own tile's), the
+// item is done again from memory, in f32, a position at a time and each row for
+// itself: what it does not see does not reach it. (These are no numbers to be
+// fast with.)
 //
 // Bound by the matrix units, at what they and the conversions leave each other:
 // chunks of 2048, 1946 and 1592 tokens at 2500, 0 and 5000, 32 / 8 heads, f32,
@@ -618,6 +620,9 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
     };
     int shift = 1 << 20;  // of the last tile's values; at first more than any
     int kshift = 0;       // of the last tile's keys
+    // The largest magnitude of a tree's values behind its context so far, of
+    // which a row may see none while its own are scaled with it.
+    uint32_t drafted = 0;
     // The tile in registers to LDS.
     auto store = [&](uint32_t tile) {
         // A wave's part a lane, the eight of them over each 16 lanes.
@@ -625,9 +630,13 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
         const uint4 w = looked[tile & 1][tid & 7];
         auto uniform_max = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(v)); };
         const uint32_t ktop = uniform_max(w.x), vtop = uniform_max(w.y), kleast = ~uniform_max(~w.z), vleast = ~uniform_max(~w.w);
-        // Infinities and NaN; positions 2^12 apart that not all rows see.
+        const bool branches = seq.is_tree && it.k0 + (tile + 1) * KT > seq.context;
+        if (branches) drafted = max(drafted, vtop);
+        const uint32_t vmost = branches ? drafted : vtop;
+        // Infinities and NaN; positions 2^12 apart that not all rows see, whose
+        // values have a scale in common also over a tree's tiles.
         const bool odd = max(ktop, vtop) >= 0x7f800000u || (kleast < ktop && (ktop >> 23) - (kleast >> 23) > 12) ||
-                         (vleast < vtop && (vtop >> 23) - (vleast >> 23) > 12);
+                         (vleast < vmost && (vmost >> 23) - (vleast >> 23) > 12);
         if (!odd) shift = min(shift, shift_of(vtop));
         kshift = shift_of(ktop);
         const uint32_t buf = (tile & 1) * kBuf;
