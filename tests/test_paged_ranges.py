@@ -59,3 +59,39 @@ def test_one_large_value_among_zeros(hip, large, context, kv, kernels):  # noqa:
     pool = scaled(step, pool_of(r, step.pages, 32, 2, 128, TH_KV_F32), kv, factors)
     q = r.standard_normal((step.tokens, 8, 128), dtype=np.float32)
     check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("context", [2000, 6400])
+@pytest.mark.parametrize("new", [1, 20, 70])
+@pytest.mark.parametrize("size,signs", [(1e33, True), (1e34, False), (1e35, True), (3e38, False)])
+def test_flat_scores_over_values_near_the_largest(hip, size, signs, new, context, kv, kernels):  # noqa: F811
+    """Averages of thousands of values whose sums f32 does not hold, of one sign
+    or both, where a plan splits the positions. (The kernel for few rows adds
+    f32 values up with weights of at most one: at 1e35, of both signs, within
+    range.)"""
+    if size > 1e37 and (kernels == 0 or new * 4 <= 16):
+        pytest.skip("sums past f32's range in the kernel for few rows")
+    r = np.random.default_rng(new + context)
+    step = Step(r, [context], [new], 64)
+    pool = pool_of(r, step.pages, 64, 2, 128, TH_KV_F32)
+    pool[:, 1] = r.uniform(0.1, 1, pool[:, 1].shape) * size
+    if signs:
+        pool[:, 1] *= r.choice([-1, 1], pool[:, 1].shape)
+    pool = bf16_to_f32(f32_to_bf16(pool)) if kv == TH_KV_BF16 else pool
+    q = np.float32(0.01) * r.standard_normal((step.tokens, 8, 128), dtype=np.float32)
+    check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("context,new", [([20000], [1]), ([40000] + [400] * 9, [16] * 10)])
+def test_joins_of_more_parts_than_lanes(hip, context, new, kv, kernels):  # noqa: F811
+    """One KV head, so that the chip is filled by one long sequence's parts:
+    hundreds of a few rows, and of many beside others of two."""
+    r = np.random.default_rng(len(context))
+    step = Step(r, context, new, 256)
+    pool = pool_of(r, step.pages, 256, 1, 128, kv)
+    q = r.standard_normal((step.tokens, 16, 128), dtype=np.float32)
+    check(run_attention(hip, step, q, pool, 16, kv, kernels), *attention64(step, q, pool, 16))

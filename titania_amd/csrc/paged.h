@@ -50,7 +50,7 @@ struct ItemAt {
 struct JoinAt {
     uint32_t token0, rows, row0, part, n_parts, slabs;
 };
-// A slab: the unnormalized results of 16 rows, then their maxima and sums.
+// A slab: 16 rows' results of their part, then the parts' maxima and sums.
 constexpr size_t slab_floats(size_t head_dim) { return 16 * (head_dim + 2); }
 constexpr size_t slabs_of(size_t head_dim) { return kAttnRoundFloats / slab_floats(head_dim); }
 

@@ -294,7 +294,8 @@ __global__ __launch_bounds__(kFewThreads, HD < 256 ? 2 : 1) void paged_few_kerne
                 *reinterpret_cast<float4 *>(dst + col) = make_float4(sum.x / ls, sum.y / ls, sum.z / ls, sum.w / ls);
             } else {
                 float *slab = a.part + (size_t)(it.part + kvh) * slab_floats(HD);
-                *reinterpret_cast<float4 *>(slab + row * HD + col) = sum;
+                const float f = ls == 0.f ? 1.f : 1.f / ls;  // (zero: the row sees nothing here)
+                *reinterpret_cast<float4 *>(slab + row * HD + col) = make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
                 if (col == 0) *reinterpret_cast<float2 *>(slab + 16 * HD + 2 * row) = make_float2(ms, ls);
             }
         }
@@ -795,19 +796,19 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
         }
     };
     // A row set's results, or partial ones: x[d][e] 2^-by is dimension
-    // 16 d + 4 lg + e of the lane's row, of weights exp2(. - top).
+    // 16 d + 4 lg + e of the lane's row, of weights exp2(. - top) that add up
+    // to `sum` (2^15 for each position at most: over them first).
     auto put = [&](int s, const f32x4 (&x)[HD / 16], float top, float sum, int by) {
         const int tid = thread(), li = tid & 15, g4 = 4 * (tid >> 4 & 3);
         const uint32_t r = wrow + 16 * s + li;
         if (r >= rows) return;
         float *dst;
-        float f;
+        float f = 1.f / sum;
         if (it.part == kNoPart) {
             dst = a.out + row_at(it.row0 + r);
-            f = 1.f / sum;
         } else {
             dst = a.part + (size_t)(it.part + kvh * 8 * SETS + r / 16) * slab_floats(HD);
-            f = 1.f;
+            if (sum == 0.f) f = 1.f;  // it sees nothing here
             if (g4 == 0) *reinterpret_cast<float2 *>(dst + 16 * HD + 2 * li) = make_float2(top, sum);
             dst += li * HD;
         }
@@ -891,60 +892,82 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
 
 // Joins a split tile's parts, `W` waves a row: four for few rows of many parts,
 // which then wait for a quarter of them, one for many rows (1920 rows of 32
-// parts, 32 MB, 8.5 us; 16 rows of 64 parts 4.9).
+// parts, 32 MB, 8.5 us; 16 rows of 64 parts 4.9). A part counts for its share of
+// the weights: no sum here is larger than the values.
 template <int HD, int W>
 __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, const BatchHead &head) {
     constexpr int E = HD / 64, ROWS = 4 / W;  // a block's rows
-    __shared__ float red[W == 1 ? 1 : 4][W == 1 ? 1 : HD], stat[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float red[W == 1 ? 1 : 4][W == 1 ? 1 : HD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // gridDim.y walks the tiles, gridDim.x their rows, for each KV head.
     for (uint32_t j = blockIdx.y; j < head.n_joins; j += gridDim.y) {
         const JoinAt join = scalar_load(a.b.joins, j);
-        const uint32_t rows = join.rows;
+        const uint32_t rows = join.rows, n = join.n_parts;
         for (uint32_t i = blockIdx.x * ROWS + (W == 1 ? wave : 0); i < rows * a.n_kv_heads; i += gridDim.x * ROWS) {
             const uint32_t row = i % rows, kvh = i / rows;
-            const float *part = a.part + (size_t)(join.part + kvh * join.slabs + row / 16) * slab_floats(HD);
+            const float *const part = a.part + (size_t)(join.part + kvh * join.slabs + row / 16) * slab_floats(HD);
             const size_t step = (size_t)join.slabs * a.n_kv_heads * slab_floats(HD);
-            // The maximum first, so that the parts' sums wait for nothing.
-            float top = -INFINITY;
-            for (uint32_t p = lane; p < join.n_parts; p += 64) top = fmaxf(top, part[p * step + 16 * HD + 2 * (row % 16)]);
+            auto stat = [&](uint32_t p) {
+                return *reinterpret_cast<const float2 *>(part + p * step + 16 * HD + 2 * (row % 16));
+            };
+            auto fetch = [&](float (&x)[E], uint32_t p) {
+                const float *s = part + p * step + (row % 16) * HD + E * lane;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = s[e];
+            };
+            // The maximum and the sum of all parts, a part a lane; with one wave a
+            // row, while the first parts are on their way.
+            const float2 mine = lane < (int)n ? stat(lane) : make_float2(-INFINITY, 0.f);
+            float ahead[W == 1 ? 8 : 1][E];
+            auto fetch8 = [&](uint32_t p) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k)
+                    if (p + k < n) fetch(ahead[k], p + k);
+            };
+            if constexpr (W == 1) fetch8(0);
+            float top = mine.x, acc[E];
+            for (uint32_t p = 64 + lane; p < n; p += 64) top = fmaxf(top, stat(p).x);
             top = wave_max_dpp(top);
-            float l = 0.f, acc[E];
+            // A part's weights, by the largest of all: none where it has no
+            // maximum, unless they are NaN.
+            auto weight = [&](const float2 &ml) { return ml.y * __builtin_amdgcn_exp2f(ml.x - top); };
+            float l = weight(mine);
+            for (uint32_t p = 64 + lane; p < n; p += 64) l += weight(stat(p));
+            const float over = 1.f / wave_sum_dpp(l);
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 8
-            for (uint32_t p = W == 1 ? 0 : wave; p < join.n_parts; p += W) {
-                const float *s = part + p * step;
-                const float2 ml = *reinterpret_cast<const float2 *>(s + 16 * HD + 2 * (row % 16));
-                float x[E];
-                if constexpr (E == 2) {
-                    const float2 v = *reinterpret_cast<const float2 *>(s + (row % 16) * HD + 2 * lane);
-                    x[0] = v.x;
-                    x[1] = v.y;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = s[(row % 16) * HD + E * lane + e];
-                }
-                // A part of no weight has no maximum; one of NaN has none either.
-                const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - top);
-                l = fmaf(ml.y, f, l);
+            auto add = [&](const float (&x)[E], float f) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e]);
+            };
+            if constexpr (W == 1) {
+                for (uint32_t p = 0; p < n; p += 8) {
+                    if (p) fetch8(p);
+                    const float share = (p < 64 ? weight(mine) : weight(stat(min((p & ~63u) + lane, n - 1)))) * over;
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k)
+                        if (p + k < n)
+                            add(ahead[k], __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), (p + k) & 63)));
+                }
+            } else {
+#pragma unroll 8
+                for (uint32_t p = wave; p < n; p += W) {
+                    float x[E];
+                    fetch(x, p);
+                    add(x, weight(stat(p)) * over);
+                }
             }
             const uint32_t r = join.row0 + row;
             float *out = a.out + ((size_t)(join.token0 + r / a.group) * a.n_heads + (size_t)kvh * a.group + r % a.group) * HD;
             if constexpr (W == 1) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) out[E * lane + e] = acc[e] / l;
+                for (int e = 0; e < E; ++e) out[E * lane + e] = acc[e];
             } else {
-                if (lane == 0) stat[wave] = l;
 #pragma unroll
                 for (int e = 0; e < E; ++e) red[wave][E * lane + e] = acc[e];
                 __syncthreads();
-                if (threadIdx.x < HD) {
-                    const float sum = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-                    out[threadIdx.x] = sum / ((stat[0] + stat[1]) + (stat[2] + stat[3]));
-                }
+                if (threadIdx.x < HD)
+                    out[threadIdx.x] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
                 __syncthreads();
             }
         }
