@@ -95,3 +95,27 @@ def test_joins_of_more_parts_than_lanes(hip, context, new, kv, kernels):  # noqa
     pool = pool_of(r, step.pages, 256, 1, 128, kv)
     q = r.standard_normal((step.tokens, 16, 128), dtype=np.float32)
     check(run_attention(hip, step, q, pool, 16, kv, kernels), *attention64(step, q, pool, 16))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize("heads,kvh,first,new", [(32, 8, 64, 128), (512, 256, 128, 256)])
+def test_what_all_rows_see_is_not_taken_one_by_one(hip, what, heads, kvh, first, new, kv):
+    """A prompt with a position whose key, or values, are 2^-14 of its
+    neighbours': the tokens of later tiles, all of which see it, get the bits that
+    they get when the positions before them are their context. (Tiles of 256 rows
+    of so few positions, or so many heads, that no plan splits either.)"""
+    r = np.random.default_rng(first + what)
+    step = Step(r, [0], [new], 32, spare=0)
+    after = Step(r, [first], [new - first], 32, spare=0)
+    after.lists = step.lists
+    pool = pool_of(r, step.pages, 32, kvh, 128, TH_KV_F32)
+    page, row = step.place(0, 20)
+    pool[page, what, row] *= np.float32(2.0**-14)
+    pool = bf16_to_f32(f32_to_bf16(pool)) if kv == TH_KV_BF16 else pool
+    q = r.standard_normal((new, heads, 128), dtype=np.float32)
+    got = run_attention(hip, step, q, pool, heads, kv, 7)
+    check(got, *attention64(step, q, pool, heads))
+    same = got[first:] == run_attention(hip, after, q[first:], pool, heads, kv, 7)
+    assert same.all(), f"{(~same).sum()} of {same.size} differ"

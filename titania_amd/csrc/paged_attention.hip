@@ -384,12 +384,14 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // the tile's four sixteens, which with V^T's columns in that order are the
 // operand of O^T = V^T P^T.
 //
-// Where a tile has an infinity or a NaN, or where rows do not see all positions
-// and these differ by more than 2^12 (of a tree's values, over its tiles so
-// far: a row may see none of an earlier tile whose scale is its own tile's), the
-// item is done again from memory, in f32, a position at a time and each row for
-// itself: what it does not see does not reach it. (These are no numbers to be
-// fast with.)
+// Where a tile has an infinity or a NaN, or where not all of the item's rows see
+// all positions and these differ by more than 2^12 (of a tree's values, over its
+// tiles so far: a row may see none of an earlier tile whose scale is its own
+// tile's), the item is done again from memory, in f32, a position at a time and
+// each row for itself: what it does not see does not reach it. (These are no
+// numbers to be fast with: a prompt of 2048 one of whose positions has 2^-14 of
+// its neighbours' values takes 2.9 ms, not 0.14, for that position's own rows;
+// 512 tokens at 8000 with an infinity in their context 11 ms, not 0.2.)
 //
 // Bound by the matrix units, at what they and the conversions leave each other:
 // chunks of 2048, 1946 and 1592 tokens at 2500, 0 and 5000, 32 / 8 heads, f32,
@@ -471,6 +473,8 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
             ql[s][c] = make_uint4(l[0], l[1], l[2], l[3]);
         }
     }
+    // The first position that one of the item's rows does not see.
+    const uint32_t in_common = seq.context + (seq.is_tree ? 0 : it.row0 / a.group + 1);
     // Of the wave's rows: the first position that one does not see, and the
     // first that none sees (zero: there are no such rows).
     const uint32_t w0 = wrow, w1 = min(w0 + RW, rows) - 1;
@@ -565,7 +569,9 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
         else return e & 1 ? bf16_hi(__float_as_uint(kraw[i][e / 2])) : bf16_lo(__float_as_uint(kraw[i][e / 2]));
     };
     // The largest magnitude of the wave's keys and values, and, where some
-    // row does not see some position, the smallest of a position's largest.
+    // row does not see some position, the smallest of a position's largest
+    // (which takes lane exchanges for each: wherever a position was new, a
+    // prompt of 2048 from its start took 151 us, not 136).
     auto look = [&](uint32_t c0, uint32_t tile) {
         uint32_t ktop = 0, vtop = 0, kleast = 0x7f000000u, vleast = 0x7f000000u;
         if (c0 + KT > it.k1) {  // past the last position is anything: zero
@@ -581,7 +587,7 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
                 for (int d = 0; d < (F32 ? VD : 1); ++d)
                     vraw[j][d] = c0 + vkey + (j & 3) + 16 * (j >> 2) < it.k1 ? vraw[j][d] : 0.f;
         }
-        if (c0 + KT > seq.context) {
+        if (c0 + KT > in_common) {
 #pragma unroll
             for (int i = 0; i < KU; ++i) {
                 uint32_t own = 0;
@@ -631,7 +637,7 @@ __global__ __launch_bounds__(kManyThreads, SETS == 1 && sizeof(KV) == 2 ? 4 : 2)
         const uint4 w = looked[tile & 1][tid & 7];
         auto uniform_max = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)row_max(v)); };
         const uint32_t ktop = uniform_max(w.x), vtop = uniform_max(w.y), kleast = ~uniform_max(~w.z), vleast = ~uniform_max(~w.w);
-        const bool branches = seq.is_tree && it.k0 + (tile + 1) * KT > seq.context;
+        const bool branches = seq.is_tree && it.k0 + (tile + 1) * KT > in_common;
         if (branches) drafted = max(drafted, vtop);
         const uint32_t vmost = branches ? drafted : vtop;
         // Infinities and NaN; positions 2^12 apart that not all rows see, whose
