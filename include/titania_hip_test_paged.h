@@ -1,7 +1,7 @@
 /*
- * titania_hip_test_paged.h: for tests/test_paged.py and tests/test_paged_plan.py
- * alone: the attention's kernels where a plan would take others, and what
- * th_batch_set checks and plans, without a GPU.
+ * titania_hip_test_paged.h: for tests/test_paged*.py alone: the attention's
+ * kernels where a plan would take others, how th_batch_accept cuts its rows, and
+ * what th_batch_set checks and plans, without a GPU.
  */
 #ifndef TITANIA_HIP_TEST_PAGED_H
 #define TITANIA_HIP_TEST_PAGED_H
@@ -16,6 +16,10 @@ extern "C" {
  * and of 256), each for the sequences of 1 to 16, to 128 and of more rows, and for
  * the others the next there is, whatever would be fastest. */
 TH_API int th_test_batch_classes(th_batch *batch, unsigned classes);
+
+/* How th_batch_accept cuts `rows` rows of `cols` logits: rows a launch, parts a
+ * row, values a part (the last one's are fewer). */
+TH_API int th_test_accept_parts(size_t rows, size_t cols, size_t *rows_at_once, size_t *splits, size_t *part);
 
 /* th_batch_set for a batch of shape {pages, page_len, n_kv_heads, head_dim,
  * kv_dtype, n_heads, max_seqs, max_tokens, max_pages} whose captured calls

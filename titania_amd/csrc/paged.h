@@ -2,6 +2,8 @@
 // layout in memory, and the launchers of their kernels.
 #pragma once
 
+#include <algorithm>
+
 #include "common.h"
 
 // One layer's keys and values of many sequences, in pages of `page_len`
@@ -118,8 +120,22 @@ struct PagedAttnArgs {
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs &a, const BatchHead &count, size_t head_dim, bool bf16,
                                   unsigned captured);
 
+// How many of `n` rows one launch of the argmax takes, in how many parts a row:
+// [i * part, (i + 1) * part), the last to the row's end, so that none is empty.
+// About 2048 blocks, of 4096 values at least; `rows * splits` results at most
+// kMostPicks.
+constexpr size_t kMostPicks = kPinnedFloats / 2;
+struct RowParts {
+    size_t rows, splits, part;
+};
+inline RowParts row_parts(size_t n, size_t cols) {
+    const size_t rows = std::min(n, kMostPicks);
+    const size_t most = std::max<size_t>(1, std::min({(cols + 4095) / 4096, (2048 + rows - 1) / rows, kMostPicks / rows}));
+    const size_t part = ((cols + most - 1) / most + 3) / 4 * 4;
+    return {rows, (cols + part - 1) / part, part};
+}
 // picks[row * splits + split] = the packed argmax of a part of a row.
-hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, int splits, uint64_t *picks);
+hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, const RowParts &parts, uint64_t *picks);
 
 // Rows to move in every layer's cache, as kernel arguments: of segment i (a
 // sequence) moves [start[i], start[i + 1]), in order.

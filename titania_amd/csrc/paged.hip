@@ -470,18 +470,17 @@ int th_batch_accept(th_device *dev, const th_batch *b, const th_buffer *logits, 
         TH_REQUIRE(vocab < 0xffffffffu, "rows of %zu logits", vocab);
         TH_PAGED_CURRENT(dev);
         // Each block leaves its part's maximum in pinned memory; the host
-        // takes the largest. About 2048 blocks, of 4096 values at least.
-        auto *part = reinterpret_cast<uint64_t *>(dev->pinned);
-        const size_t room = th::kPinnedFloats / 2, rows = std::min(n, room);
-        const size_t splits = std::max<size_t>(
-            1, std::min({(vocab + 4095) / 4096, (2048 + rows - 1) / rows, room / rows}));
-        for (size_t r = 0; r < n; r += rows) {
-            const size_t now = std::min(rows, n - r);
-            memset(part, 0, now * splits * sizeof(uint64_t));  // no part's maximum: an index is below 2^32 - 1
-            TH_HIP(th::launch_argmax_rows(dev->stream, logits->ptr + r * vocab, now, vocab, (int)splits, part));
-            if (!arrive(part, now * splits)) TH_HIP(hipStreamSynchronize(dev->stream));
+        // takes the largest.
+        auto *picked = reinterpret_cast<uint64_t *>(dev->pinned);
+        const th::RowParts parts = th::row_parts(n, vocab);
+        const size_t splits = parts.splits;
+        for (size_t r = 0; r < n; r += parts.rows) {
+            const size_t now = std::min(parts.rows, n - r);
+            memset(picked, 0, now * splits * sizeof(uint64_t));  // no part's maximum: an index is below 2^32 - 1
+            TH_HIP(th::launch_argmax_rows(dev->stream, logits->ptr + r * vocab, now, vocab, parts, picked));
+            if (!arrive(picked, now * splits)) TH_HIP(hipStreamSynchronize(dev->stream));
             for (size_t i = 0; i < now; ++i) {
-                const uint64_t best = *std::max_element(part + i * splits, part + (i + 1) * splits);
+                const uint64_t best = *std::max_element(picked + i * splits, picked + (i + 1) * splits);
                 picks[r + i] = 0xffffffffu - (uint32_t)best;
             }
         }
@@ -563,6 +562,14 @@ int th_paged_keep(th_device *dev, th_paged *const *caches, size_t n_caches, cons
         }
     }
     TH_HIP(flush());
+    return TH_OK;
+}
+
+int th_test_accept_parts(size_t rows, size_t cols, size_t *rows_at_once, size_t *splits, size_t *part) {
+    const th::RowParts parts = th::row_parts(rows, cols);
+    *rows_at_once = parts.rows;
+    *splits = parts.splits;
+    *part = parts.part;
     return TH_OK;
 }
 

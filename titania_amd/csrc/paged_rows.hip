@@ -160,9 +160,8 @@ hipError_t launch_paged_moves(hipStream_t s, const PagedMoves &m) {
     return hipGetLastError();
 }
 
-hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, int splits, uint64_t *picks) {
-    const size_t part = ((cols + splits - 1) / splits + 3) / 4 * 4;
-    argmax_rows_kernel<<<(unsigned)(rows * splits), 256, 0, s>>>(x, cols, splits, part, picks);
+hipError_t launch_argmax_rows(hipStream_t s, const float *x, size_t rows, size_t cols, const RowParts &parts, uint64_t *picks) {
+    argmax_rows_kernel<<<(unsigned)(rows * parts.splits), 256, 0, s>>>(x, cols, (int)parts.splits, parts.part, picks);
     return hipGetLastError();
 }
 
