@@ -278,7 +278,8 @@ TH_API void th_batch_free(th_device *dev, th_batch *batch);
  * written to position context[s] + i; it is rotated by context[s] plus its
  * depth, i in a chain, and sees the context, itself and what it follows, up to
  * the root. The arrays are copied before the call returns, to the device in
- * its stream's order; a failed call changes nothing.
+ * its stream's order. A call that is refused (TH_ERR_INVALID) changes nothing;
+ * after any other error nothing is set.
  *
  * Captured calls (th_graph_begin) read what is set when they run, so that one
  * graph serves any step: from then on th_batch_set refuses more tokens than

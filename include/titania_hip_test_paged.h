@@ -36,6 +36,13 @@ TH_API int th_test_batch_set(const size_t *shape, unsigned classes, size_t captu
                              const int32_t *parents, uint32_t *tokens, uint64_t *tree, uint32_t *items, size_t *n_items,
                              uint32_t *joins, size_t *n_joins, uint32_t *first);
 
+/* What a set that the GPU fails leaves of a batch of this shape: sequences,
+ * tokens, pages and positions of the host, then of what launches are counted by
+ * sequences, tokens, joins, their rows and items: nine numbers. Returns
+ * th_batch_set's error. */
+TH_API int th_test_batch_set_failed(const size_t *shape, size_t n_seqs, const uint32_t *context, const uint32_t *n_new,
+                                    const uint32_t *pages, size_t n_pages, size_t *left);
+
 #ifdef __cplusplus
 }
 #endif

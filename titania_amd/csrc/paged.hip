@@ -210,6 +210,15 @@ bool place_arrays(th_batch *b, size_t *bytes) {
     return b->parents && b->stamp;
 }
 
+// After a set that the GPU failed: the host's arrays may be the new step's and
+// the device's another's, so nothing is set any more.
+int set_failed(th_batch *b, hipError_t e) {
+    if (b->dev) (void)hipStreamSynchronize(b->dev->stream);  // (a copy that did start)
+    b->n_seqs = b->n_tokens = b->n_pages = b->positions = 0;
+    *b->head() = {};
+    return hip_failed(e, "setting a batch");
+}
+
 // Whether n words that a launch writes to pinned memory have all become other
 // than zero, waited for without the runtime for a short while: what it takes to
 // see a stream's end is more than what small launches take (24 rows of 151936
@@ -235,6 +244,28 @@ void note_capture(const th_device *dev, const th_batch *batch, size_t positions 
     b->captured_tokens = std::min(b->captured_tokens, b->n_tokens);
     b->captured_positions = std::min(b->captured_positions, positions);
 }
+
+// A batch without a device, in plain host memory.
+struct HostBatch : th_batch {
+    explicit HostBatch(const size_t *shape) {
+        pages = shape[0];
+        page_len = shape[1];
+        n_kv_heads = shape[2];
+        head_dim = shape[3];
+        kv_dtype = (int)shape[4];
+        n_heads = shape[5];
+        max_seqs = shape[6];
+        max_tokens = shape[7];
+        max_pages = shape[8];
+        size_t bytes = 0;
+        if (place_arrays(this, &bytes)) pinned = static_cast<char *>(calloc(1, bytes));
+    }
+    ~HostBatch() {
+        free(pinned);
+        free(parents);
+        free(stamp);
+    }
+};
 
 }  // namespace
 
@@ -394,8 +425,10 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     TH_NOT_CAPTURING(dev, "th_batch_set");
     TH_BATCH_OF(dev, b);
     TRY(check_set(b, n_seqs, context, n_new, pages, n_pages, parents));
-    TH_PAGED_CURRENT(dev);
-    TH_HIP(hipEventSynchronize(b->copied));  // the copy before has read the pinned memory
+    th::Current current(dev);
+    hipError_t e = current.error;
+    if (e == hipSuccess) e = hipEventSynchronize(b->copied);  // the copy before has read the pinned memory
+    if (e != hipSuccess) return set_failed(b, e);
     const size_t trees = lay_out(b, n_seqs, context, n_new, pages, n_pages, parents);
     const th::BatchHead *head = b->head();
     th::Upload u{};
@@ -412,9 +445,9 @@ int th_batch_set(th_device *dev, th_batch *b, size_t n_seqs, const uint32_t *con
     add(b->at_tree, trees * th::kTreeWords * sizeof(uint64_t));
     add(b->at_items, head->first[th::kClasses] * sizeof(th::ItemAt));
     add(b->at_joins, head->n_joins * sizeof(th::JoinAt));
-    TH_HIP(th::launch_upload(dev->stream, u));
-    TH_HIP(hipEventRecord(b->copied, dev->stream));
-    return TH_OK;
+    e = th::launch_upload(dev->stream, u);
+    if (e == hipSuccess) e = hipEventRecord(b->copied, dev->stream);
+    return e == hipSuccess ? TH_OK : set_failed(b, e);
 }
 
 int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q, const th_buffer *k, const th_buffer *v,
@@ -584,22 +617,11 @@ int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tok
                       const uint32_t *context, const uint32_t *n_new, const uint32_t *pages, size_t n_pages,
                       const int32_t *parents, uint32_t *tokens, uint64_t *tree, uint32_t *items, size_t *n_items,
                       uint32_t *joins, size_t *n_joins, uint32_t *first) {
-    th_batch b;
-    b.pages = shape[0];
-    b.page_len = shape[1];
-    b.n_kv_heads = shape[2];
-    b.head_dim = shape[3];
-    b.kv_dtype = (int)shape[4];
-    b.n_heads = shape[5];
-    b.max_seqs = shape[6];
-    b.max_tokens = shape[7];
-    b.max_pages = shape[8];
+    HostBatch b(shape);
     b.classes = classes;
     b.captured_tokens = captured_tokens;
     b.captured_positions = captured_positions;
-    size_t bytes = 0;
-    const bool held = place_arrays(&b, &bytes) && (b.pinned = static_cast<char *>(calloc(1, bytes)));
-    int rc = held ? check_set(&b, n_seqs, context, n_new, pages, n_pages, parents) : fail(TH_ERR_NOMEM, "out of host memory");
+    int rc = b.pinned ? check_set(&b, n_seqs, context, n_new, pages, n_pages, parents) : fail(TH_ERR_NOMEM, "out of host memory");
     if (rc == TH_OK) {
         lay_out(&b, n_seqs, context, n_new, pages, n_pages, parents);
         const th::BatchHead *head = b.head();
@@ -616,9 +638,20 @@ int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tok
             memcpy(first, head->first, sizeof head->first);
         }
     }
-    free(b.pinned);
-    free(b.parents);
-    free(b.stamp);
+    return rc;
+}
+
+int th_test_batch_set_failed(const size_t *shape, size_t n_seqs, const uint32_t *context, const uint32_t *n_new,
+                             const uint32_t *pages, size_t n_pages, size_t *left) {
+    HostBatch b(shape);
+    if (!b.pinned) return fail(TH_ERR_NOMEM, "out of host memory");
+    TRY(check_set(&b, n_seqs, context, n_new, pages, n_pages, nullptr));
+    lay_out(&b, n_seqs, context, n_new, pages, n_pages, nullptr);
+    const int rc = set_failed(&b, hipErrorLaunchFailure);
+    const th::BatchHead *head = b.head();
+    const size_t now[] = {b.n_seqs, b.n_tokens, b.n_pages, b.positions, head->n_seqs, head->n_tokens, head->n_joins,
+                          head->join_rows, head->first[th::kClasses]};
+    memcpy(left, now, sizeof now);
     return rc;
 }
 

@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import HipError, InvalidArgument, check, lib
 
 
 @dataclass
@@ -418,8 +418,13 @@ class Hip:
         tokens = int(n.sum(dtype=np.int64))
         if t is not None and t.size != tokens:
             raise ValueError(f"{t.size} parents of {tokens} tokens")
-        check(lib().th_batch_set(self.handle, batch.handle, n.size, c.ctypes.data, n.ctypes.data, p.ctypes.data, p.size,
-                                 None if t is None else t.ctypes.data))
+        try:
+            check(lib().th_batch_set(self.handle, batch.handle, n.size, c.ctypes.data, n.ctypes.data, p.ctypes.data, p.size,
+                                     None if t is None else t.ctypes.data))
+        except HipError as e:
+            if not isinstance(e, InvalidArgument):  # nothing is set
+                batch.n_seqs = batch.n_tokens = 0
+            raise
         batch.n_seqs, batch.n_tokens = n.size, tokens
 
     def paged_append(self, q_out: Buffer, q: Buffer, k: Buffer, v: Buffer, q_norm: Weight | None, k_norm: Weight | None,
