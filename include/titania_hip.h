@@ -282,11 +282,12 @@ TH_API void th_batch_free(th_device *dev, th_batch *batch);
  * after any other error nothing is set.
  *
  * Captured calls (th_graph_begin) read what is set when they run, so that one
- * graph serves any step: from then on th_batch_set refuses more tokens than
+ * graph serves any step: until th_graph_free, th_batch_set refuses more tokens than
  * were set at the capture and positions past the end of a captured append's
- * table, and plans the attention for the kernels that all the graphs hold: those
- * for 1 to 16 query rows a KV head, always, and for up to 128 and for more where
- * the step set at the capture had such sequences. Rows of activations behind
+ * table, and plans the attention, of eager calls too, for the kernels that all the
+ * batch's graphs hold: those for 1 to 16 query rows a KV head, always, and for up
+ * to 128 and for more where the step set at the capture had such sequences (so
+ * graphs of different sizes take a batch each). Rows of activations behind
  * the last token stay as they are. */
 TH_API int th_batch_set(th_device *dev, th_batch *batch, size_t n_seqs, const uint32_t *context, const uint32_t *n_new,
                         const uint32_t *pages, size_t n_pages, const int32_t *parents);

@@ -47,6 +47,10 @@ struct th_device {
     float *pinned = nullptr;
     // Between th_graph_begin and th_graph_end: the stream is being captured.
     bool capturing = false;
+    // The open capture's number, or the last one's: no two of a process are alike.
+    uint64_t capture = 0;
+    // The batches allocated with it, as a list.
+    th_batch *batches = nullptr;
 };
 
 // A model takes ownership of weight handles it frees on destruction (the
@@ -82,6 +86,12 @@ int read_back(th_device *dev, const float *src, size_t len, float *out, const un
 
 // Makes sure the device scratch holds at least `bytes`; returns its pointer or null.
 void *scratch(th_device *dev, size_t bytes);
+
+// What a capture that was discarded, or whose graph is freed, asked of the
+// device's batches no longer counts.
+void release_capture(th_device *dev, uint64_t capture);
+// The device goes: its batches can only be freed.
+void leave_batches(th_device *dev);
 
 // The device made current, as allocations and launches want it, for a call.
 struct Current {

@@ -1,8 +1,9 @@
 // The C ABI of the hip device: one entry point per method of the reference's
 // Device trait (model/device.rs:9-89), argument checks mirroring the
 // reference's asserts, and the fused extensions.
-#include <cstdint>
 #include <algorithm>
+#include <atomic>
+#include <cstdint>
 #include <cstdio>
 #include <cstring>
 #include <new>
@@ -162,12 +163,14 @@ void th_device_destroy(th_device *dev) {
     if (dev->ev_begin) (void)hipEventDestroy(dev->ev_begin);
     if (dev->ev_end) (void)hipEventDestroy(dev->ev_end);
     if (dev->stream) (void)hipStreamDestroy(dev->stream);
+    th::leave_batches(dev);
     delete dev;
 }
 
 struct th_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
+    uint64_t capture = 0;
 };
 
 int th_graph_begin(th_device *dev) {
@@ -175,6 +178,8 @@ int th_graph_begin(th_device *dev) {
     TH_REQUIRE(!dev->capturing, "the device's stream is already being captured");
     TH_HIP(hipSetDevice(dev->ordinal));
     TH_HIP(hipStreamBeginCapture(dev->stream, hipStreamCaptureModeThreadLocal));
+    static std::atomic<uint64_t> captures{0};
+    dev->capture = ++captures;
     dev->capturing = true;
     dev->captured = true;
     return TH_OK;
@@ -185,16 +190,22 @@ int th_graph_end(th_device *dev, th_graph **out) {
     TH_REQUIRE(dev->capturing, "th_graph_end without th_graph_begin");
     dev->capturing = false;
     hipGraph_t graph = nullptr;
-    TH_HIP(hipStreamEndCapture(dev->stream, &graph));
+    if (const hipError_t e = hipStreamEndCapture(dev->stream, &graph); e != hipSuccess) {
+        th::release_capture(dev, dev->capture);
+        TH_HIP(e);
+    }
     auto *g = new (std::nothrow) th_graph();
     if (!g) {
         (void)hipGraphDestroy(graph);
+        th::release_capture(dev, dev->capture);
         return fail(TH_ERR_NOMEM, "out of host memory");
     }
     g->graph = graph;
+    g->capture = dev->capture;
     const hipError_t e = hipGraphInstantiate(&g->exec, graph, nullptr, nullptr, 0);
     if (e != hipSuccess) {
         (void)hipGraphDestroy(graph);
+        th::release_capture(dev, g->capture);
         delete g;
         return fail(TH_ERR_HIP, "hipGraphInstantiate failed: %s", hipGetErrorString(e));
     }
@@ -218,6 +229,7 @@ void th_graph_free(th_device *dev, th_graph *g) {
     if (dev) (void)hipStreamSynchronize(dev->stream);
     if (g->exec) (void)hipGraphExecDestroy(g->exec);
     if (g->graph) (void)hipGraphDestroy(g->graph);
+    if (dev) th::release_capture(dev, g->capture);
     delete g;
 }
 

@@ -153,6 +153,13 @@ struct PagedMoves {
 static_assert(sizeof(PagedMoves) <= 4096, "kernel arguments");
 hipError_t launch_paged_moves(hipStream_t s, const PagedMoves &m);
 
+// What the calls of one capture, or of the graph that it became, can take.
+struct Captured {
+    uint64_t capture;
+    size_t tokens, positions;
+    unsigned classes;
+};
+
 // Copies of up to eight arrays from pinned host memory in one launch (16-byte
 // units; the addresses are multiples of 16).
 struct Upload {
@@ -172,7 +179,7 @@ struct th_batch {
     // What its caches are.
     size_t pages = 0, page_len = 0, n_kv_heads = 0, head_dim = 0;
     int kv_dtype = TH_KV_F32;
-    const th_device *dev = nullptr;  // whose stream it is copied on
+    th_device *dev = nullptr;  // whose stream it is copied on
     int page_shift = 0;
     size_t n_heads = 0, max_seqs = 0, max_tokens = 0, max_pages = 0;
     // Of what is set: sequences, tokens, entries of pages, the positions that a
@@ -181,8 +188,13 @@ struct th_batch {
     // The fewest tokens that a captured call was launched for, and the fewest
     // positions that a rotation's table of one holds.
     size_t captured_tokens = SIZE_MAX, captured_positions = SIZE_MAX;
-    // The classes of the attention's items that every captured call launches.
-    unsigned classes = (1u << th::kClasses) - 1;
+    // The classes of the attention's items that every captured call launches, of
+    // those that there are.
+    unsigned classes = (1u << th::kClasses) - 1, all = classes;
+    // The captures whose graphs there are, or that are open, and the least of each.
+    th::Captured *captures = nullptr;
+    size_t n_captures = 0, captures_room = 0;
+    th_batch *next = nullptr;  // of the device's
     bool all_classes = false;
     char *device = nullptr, *pinned = nullptr;
     // Offsets, the same in both.

@@ -235,14 +235,42 @@ bool arrive(const uint64_t *words, size_t n) {
     return true;
 }
 
-// A captured call is launched for the tokens that are set now, and an append
-// reads the table it was given: later sets may have no more tokens, and none
-// that are rotated by a position past the table's end.
-void note_capture(const th_device *dev, const th_batch *batch, size_t positions = SIZE_MAX) {
-    if (!dev->capturing) return;
+// What all captures of a batch can take.
+void weigh_captures(th_batch *b) {
+    b->captured_tokens = b->captured_positions = SIZE_MAX;
+    b->classes = b->all;
+    for (size_t i = 0; i < b->n_captures; ++i) {
+        b->captured_tokens = std::min(b->captured_tokens, b->captures[i].tokens);
+        b->captured_positions = std::min(b->captured_positions, b->captures[i].positions);
+        b->classes &= b->captures[i].classes;
+    }
+}
+
+// A captured call is launched for the tokens that are set now, an append reads
+// the table it was given, an attention launches some classes: as long as there is
+// a graph of it, later sets may have no more tokens, none that are rotated by
+// a position past the table's end, and a plan of those classes.
+int note_capture(const th_device *dev, const th_batch *batch, size_t positions, unsigned classes) {
+    if (!dev->capturing) return TH_OK;
     auto *b = const_cast<th_batch *>(batch);
-    b->captured_tokens = std::min(b->captured_tokens, b->n_tokens);
-    b->captured_positions = std::min(b->captured_positions, positions);
+    size_t i = 0;
+    while (i < b->n_captures && b->captures[i].capture != dev->capture) ++i;
+    if (i == b->n_captures) {
+        if (i == b->captures_room) {
+            const size_t room = std::max<size_t>(8, 2 * i);
+            auto *more = static_cast<th::Captured *>(realloc(b->captures, room * sizeof(th::Captured)));
+            if (!more) return fail(TH_ERR_NOMEM, "out of host memory");
+            b->captures = more;
+            b->captures_room = room;
+        }
+        b->captures[b->n_captures++] = {dev->capture, SIZE_MAX, SIZE_MAX, ~0u};
+    }
+    th::Captured &c = b->captures[i];
+    c.tokens = std::min(c.tokens, b->n_tokens);
+    c.positions = std::min(c.positions, positions);
+    c.classes &= classes;
+    weigh_captures(b);
+    return TH_OK;
 }
 
 // A batch without a device, in plain host memory.
@@ -268,6 +296,28 @@ struct HostBatch : th_batch {
 };
 
 }  // namespace
+
+namespace th {
+
+void release_capture(th_device *dev, uint64_t capture) {
+    for (th_batch *b = dev->batches; b; b = b->next)
+        for (size_t i = 0; i < b->n_captures; ++i)
+            if (b->captures[i].capture == capture) {
+                b->captures[i] = b->captures[--b->n_captures];
+                weigh_captures(b);
+                break;
+            }
+}
+
+void leave_batches(th_device *dev) {
+    while (th_batch *b = dev->batches) {
+        dev->batches = b->next;
+        b->dev = nullptr;
+        b->next = nullptr;
+    }
+}
+
+}  // namespace th
 
 extern "C" {
 
@@ -369,6 +419,12 @@ void th_batch_free(th_device *dev, th_batch *b) {
     if (b->device) (void)hipFree(b->device);
     if (b->pinned) (void)hipHostFree(b->pinned);
     if (b->copied) (void)hipEventDestroy(b->copied);
+    for (th_batch **at = b->dev ? &b->dev->batches : nullptr; at && *at; at = &(*at)->next)
+        if (*at == b) {
+            *at = b->next;
+            break;
+        }
+    free(b->captures);
     free(b->parents);
     free(b->stamp);
     delete b;
@@ -415,6 +471,8 @@ int th_batch_alloc(th_device *dev, const th_paged *c, size_t n_heads, size_t max
         return hip_failed(e, "the allocation of a batch");
     }
     memset(b->pinned, 0, at);
+    b->next = dev->batches;
+    dev->batches = b;
     *out = b;
     return TH_OK;
 }
@@ -467,8 +525,8 @@ int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q, const 
     TH_PAGED_CURRENT(dev);
     th::PagedAppendArgs a{b->view(), q_out->ptr, q->ptr, k->ptr, v->ptr, q_norm ? q_norm->ptr : nullptr,
                           k_norm ? k_norm->ptr : nullptr, rope->ptr, c->ptr, (int)b->n_heads, (int)b->n_kv_heads, eps};
+    TRY(note_capture(dev, b, rope->len / hd, ~0u));
     TH_HIP(th::launch_paged_append(dev->stream, a, n, hd, c->kv_dtype == TH_KV_BF16));
-    note_capture(dev, b, rope->len / hd);
     return TH_OK;
 }
 
@@ -483,9 +541,8 @@ int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const
     th::PagedAttnArgs a{b->view(), out->ptr, q->ptr, c->ptr, (int)b->n_heads, (int)b->n_kv_heads,
                         (int)(b->n_heads / b->n_kv_heads), 1.0f / sqrtf((float)hd), dev->part};
     const unsigned captured = dev->capturing ? th::classes_of(b->plan_shape(), *b->head(), b->seqs()) : 0;
+    TRY(note_capture(dev, b, SIZE_MAX, captured));
     TH_HIP(th::launch_paged_attention(dev->stream, a, *b->head(), hd, c->kv_dtype == TH_KV_BF16, captured));
-    note_capture(dev, b);
-    if (captured) const_cast<th_batch *>(b)->classes &= captured;
     return TH_OK;
 }
 
@@ -608,8 +665,9 @@ int th_test_accept_parts(size_t rows, size_t cols, size_t *rows_at_once, size_t 
 
 int th_test_batch_classes(th_batch *b, unsigned classes) {
     TH_REQUIRE(b && classes < 1u << th::kClasses && classes & 1, "th_test_batch_classes: %u", classes);
-    b->classes = classes;
+    b->all = classes;
     b->all_classes = true;
+    weigh_captures(b);
     return TH_OK;
 }
 
