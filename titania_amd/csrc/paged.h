@@ -24,10 +24,9 @@ constexpr size_t kPagedMaxGroup = 16;  // query heads per KV head
 constexpr size_t kMostPositions = (size_t)1 << 30;  // of a sequence, whose kernels count in 32 bits
 
 // What the kernels read of a batch. A token: the row of the cache that it is
-// written to (page * page_len + row), the position of its rotation, its
-// sequence and its place among that sequence's tokens.
+// written to (page * page_len + row) and the position of its rotation.
 struct TokenAt {
-    uint32_t slot, pos, seq, index;
+    uint32_t slot, pos;
 };
 // A sequence: its first token, its tokens, the positions before them, where
 // its pages begin in the list of pages, and whether its tokens form a tree

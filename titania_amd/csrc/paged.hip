@@ -167,8 +167,6 @@ size_t lay_out(th_batch *b, size_t n_seqs, const uint32_t *context, const uint32
             th::TokenAt &t = toks[t0 + i];
             t.slot = pages[p0 + at / L] << b->page_shift | (uint32_t)(at & (L - 1));
             t.pos = par[i] < 0 ? ctx : toks[t0 + par[i]].pos + 1;
-            t.seq = (uint32_t)s;
-            t.index = i;
             positions = std::max<size_t>(positions, (size_t)t.pos + 1);
             if (chain) continue;
             uint64_t *bits = tree + (t0 + i) * th::kTreeWords;
@@ -689,7 +687,13 @@ int th_test_batch_set(const size_t *shape, unsigned classes, size_t captured_tok
         if (*n_items > std::min(most_items, b.plan_shape().max_items) || *n_joins > std::min(most_joins, b.plan_shape().max_joins)) {
             rc = fail(TH_ERR_INVALID, "%zu items and %zu joins", *n_items, *n_joins);
         } else {
-            memcpy(tokens, b.pinned + b.at_tokens, b.n_tokens * sizeof(th::TokenAt));
+            const auto *at = reinterpret_cast<const th::TokenAt *>(b.pinned + b.at_tokens);
+            for (uint32_t s = 0; s < head->n_seqs; ++s)
+                for (uint32_t i = 0; i < b.seqs()[s].n_new; ++i) {
+                    const uint32_t t = b.seqs()[s].token0 + i;
+                    const uint32_t now[] = {at[t].slot, at[t].pos, s, i};
+                    memcpy(tokens + 4 * t, now, sizeof now);
+                }
             memcpy(tree, b.pinned + b.at_tree, b.n_tokens * th::kTreeWords * sizeof(uint64_t));
             memcpy(items, b.pinned + b.at_items, *n_items * sizeof(th::ItemAt));
             memcpy(joins, b.pinned + b.at_joins, *n_joins * sizeof(th::JoinAt));
