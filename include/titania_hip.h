@@ -262,7 +262,10 @@ typedef struct th_batch th_batch;
  * all (max_tokens * n_heads <= 2^24) and max_pages entries of pages (at most
  * 2^26), over caches of the shape and type of `cache`; n_heads: query heads, 1 to 16 for
  * each KV head. Nothing is set. A batch belongs to `dev`: calls with another
- * device refuse it. */
+ * device refuse it, and th_graph_launch with another one a graph that has such
+ * calls (a set is copied on dev's stream, which no other one waits for). What the
+ * calls name, the batch and its caches too, has to be there when a graph of
+ * them is launched. */
 TH_API int th_batch_alloc(th_device *dev, const th_paged *cache, size_t n_heads, size_t max_seqs, size_t max_tokens,
                           size_t max_pages, th_batch **out);
 TH_API void th_batch_free(th_device *dev, th_batch *batch);

@@ -7,7 +7,7 @@ import pytest
 
 from test_paged import EPS, Step, buf, cache_of, pool_of, rope_table
 from titania_amd import TH_KV_BF16, TH_KV_F32, Hip, InvalidArgument
-from titania_amd._lib import lib
+from titania_amd._lib import check, lib
 
 gpu = pytest.mark.gpu
 HEADS, KVH, HD, PAGE = 32, 8, 128, 16
@@ -109,3 +109,26 @@ def test_batches_outlive_graphs_and_devices():
     for b in (batches[2], batches[0]):
         lib().th_batch_free(None, b.batch.handle)
         b.batch.handle = None
+
+
+@gpu
+def test_a_batch_is_replayed_on_its_own_stream(hip):
+    """Another device's stream would not wait for a set: a graph with a batch's
+    calls is refused there, one of other calls is not."""
+    b = Batch(hip, np.random.default_rng(4))
+    other = Hip(0)
+    graph, x = b.capture(0, 3, 100)
+    hip.graph_begin()
+    hip.add(x[1], x[2])
+    plain = hip.graph_end()
+    hip.write(x[1], np.zeros(len(x[1])))
+    with pytest.raises(InvalidArgument, match="captured with"):
+        check(lib().th_graph_launch(other.handle, graph.handle))
+    check(lib().th_graph_launch(other.handle, plain.handle))
+    other.synchronize()
+    assert np.array_equal(hip.read(x[1]), b.k[:3].ravel())
+    graph.launch()
+    hip.synchronize()
+    for g in (graph, plain):
+        g.free()
+    other.close()

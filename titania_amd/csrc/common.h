@@ -49,6 +49,8 @@ struct th_device {
     bool capturing = false;
     // The open capture's number, or the last one's: no two of a process are alike.
     uint64_t capture = 0;
+    // It has calls of a batch, which only this device's stream may run.
+    bool captured_batch = false;
     // The batches allocated with it, as a list.
     th_batch *batches = nullptr;
 };

@@ -171,6 +171,7 @@ struct th_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
     uint64_t capture = 0;
+    const th_device *only = nullptr;  // that may launch it, or any
 };
 
 int th_graph_begin(th_device *dev) {
@@ -180,6 +181,7 @@ int th_graph_begin(th_device *dev) {
     TH_HIP(hipStreamBeginCapture(dev->stream, hipStreamCaptureModeThreadLocal));
     static std::atomic<uint64_t> captures{0};
     dev->capture = ++captures;
+    dev->captured_batch = false;
     dev->capturing = true;
     dev->captured = true;
     return TH_OK;
@@ -202,6 +204,7 @@ int th_graph_end(th_device *dev, th_graph **out) {
     }
     g->graph = graph;
     g->capture = dev->capture;
+    if (dev->captured_batch) g->only = dev;
     const hipError_t e = hipGraphInstantiate(&g->exec, graph, nullptr, nullptr, 0);
     if (e != hipSuccess) {
         (void)hipGraphDestroy(graph);
@@ -216,6 +219,7 @@ int th_graph_end(th_device *dev, th_graph **out) {
 int th_graph_launch(th_device *dev, const th_graph *g) {
     TH_REQUIRE(dev && g, "th_graph_launch: null argument");
     TH_NOT_CAPTURING(dev, "th_graph_launch");
+    TH_REQUIRE(!g->only || g->only == dev, "a graph with a batch's calls is launched with the device it was captured with");
     TH_HIP(hipGraphLaunch(g->exec, dev->stream));
     return TH_OK;
 }

@@ -251,6 +251,7 @@ void weigh_captures(th_batch *b) {
 int note_capture(const th_device *dev, const th_batch *batch, size_t positions, unsigned classes) {
     if (!dev->capturing) return TH_OK;
     auto *b = const_cast<th_batch *>(batch);
+    b->dev->captured_batch = true;
     size_t i = 0;
     while (i < b->n_captures && b->captures[i].capture != dev->capture) ++i;
     if (i == b->n_captures) {
