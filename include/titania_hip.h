@@ -305,9 +305,14 @@ TH_API int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q,
                            const th_batch *batch, float eps);
 /* For each token of the batch: attention of its n_heads queries over what it
  * sees, whose rows th_paged_append has written (th_attention over a paged
- * cache; a sequence alone and in a chain gives its result within rounding).
- * What a token does not see does not reach its result, NaN and infinities
- * included. */
+ * cache; a sequence alone and in a chain gives its result within the rounding
+ * below). What a token does not see does not reach its result, NaN and
+ * infinities included.
+ * Sums are in f32. Where the plan takes few query rows at a time, so are
+ * products, and sums of values with weights of at most one have to be in f32's
+ * range. Where it takes many (more than 16 of a KV head, as a rule), queries, keys,
+ * values and weights have 22 bits: a product is off by up to 2^-21 of
+ * itself and by 2^-38 of the largest key, or value, that the token sees. */
 TH_API int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const th_paged *cache,
                               const th_batch *batch);
 /* The greedy verification of drafted tokens. logits: a row for each token of

@@ -34,14 +34,15 @@ def scaled(step, pool, kv, factors):
     ((64, 30), (2.0**20, 1)), ((64, 30), (2.0**40, 1)), ((64, 30), (1e20, 1)), ((64, 30), (1, 1e20)), ((64, 30), (2.0**-20, 1)),
     ((64, 64, 64, 20), (2.0**30, 2.0**20, 2.0**10, 1)), ((64, 64, 128), (1, 1e20, 1)), ((30, 100), (1e20, 1)),
 ], ids=str)
-def test_branches_of_other_sizes(hip, lengths, factors, context, kv, kernels):  # noqa: F811
+@pytest.mark.parametrize("hd", [64, 128])
+def test_branches_of_other_sizes(hip, hd, lengths, factors, context, kv, kernels):  # noqa: F811
     """Branches of a tree, of which the first fills whole 64 positions, whose
     values are larger or smaller than other branches' by so much that together
     they have no scale: each branch's results are its own."""
     r = np.random.default_rng(sum(lengths) + context)
     step = Step(r, [context], [sum(lengths)], 32, [branches(*lengths)])
-    pool = scaled(step, pool_of(r, step.pages, 32, 2, 128, TH_KV_F32), kv, np.repeat(factors, lengths))
-    q = r.standard_normal((step.tokens, 8, 128), dtype=np.float32)
+    pool = scaled(step, pool_of(r, step.pages, 32, 2, hd, TH_KV_F32), kv, np.repeat(factors, lengths))
+    q = r.standard_normal((step.tokens, 8, hd), dtype=np.float32)
     check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
 
 

@@ -393,17 +393,20 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // its neighbours' values takes 2.9 ms, not 0.14, for that position's own rows;
 // 512 tokens at 8000 with an infinity in their context 11 ms, not 0.2.)
 //
-// Bound by the matrix units, at what they and the conversions leave each other:
-// chunks of 2048, 1946 and 1592 tokens at 2500, 0 and 5000, 32 / 8 heads, f32,
-// take 0.82 ms, products at 1.06 to 1.1 PFLOP/s, the units busy half of the time
-// (a large matrix product of a library: 1.24 PFLOP/s). That case, step by step:
+// Bound by the matrix and the vector units in turn: a wave's products wait for
+// its conversions and its softmax, and a SIMD's two waves hide half of that from
+// each other. Chunks of 2048, 1946 and 1592 tokens at 2500, 0 and 5000, 32 / 8
+// heads, f32, take 0.81 ms, products at 1.1 PFLOP/s, the matrix units busy 51% of
+// the time (a large matrix product of a library: 1.24 PFLOP/s). That case, step by step:
 // f32 products 3.87 ms; two f16 terms 1.60; one exponent for a tile's keys and
 // maxima by lane exchanges 1.12; rows swizzled in LDS, not padded, 1.07;
 // remainders by one mixed-precision fma, maxima of three 0.98; references that
 // move by 2^5 only 0.95; products before other waves' conversions 0.91; the
 // longest items first 0.85; half of the waves converting between their halves
-// of a tile 0.81. A tree of 60 tokens at 12001 takes 55 to 59 us, 8.5 of them
-// the join: 256 blocks of 6 tiles of 5.6 us, and 34 MB of partial results.
+// of a tile 0.81 to 0.83; positions compared only where not all rows see them
+// 0.81 (0.83 in the same minutes without). A tree of 60 tokens at 12001 takes 56 to 60
+// us, 8.5 of them the join: 256 blocks of 6 tiles of 5.6 us, and 34 MB of
+// partial results.
 // Not kept: two groups of four waves that halve a tile's positions, for up to
 // 64 rows (bf16 41 -> 44 us, f32 66 -> 63); two tiles requested ahead, or the
 // first one before the queries are converted (no change); blocks' rows on turned

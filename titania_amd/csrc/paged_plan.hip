@@ -10,7 +10,10 @@ namespace {
 
 // What the chip holds of a class's blocks at once: two a CU, or one where LDS
 // or registers hold no more. (Trees of 14 to 25 tokens over bf16, whose class 1
-// fits twice in 128 registers a thread, 50 -> 43 us.)
+// fits twice in 128 registers a thread, 50 -> 43 us.) These numbers and the
+// estimates below are of head_dim 128, and 64 and 256 take them as they are: 64
+// tokens at 120 to 8000 still run at 5.6 (f32) and 4.8 TB/s (bf16) of keys and
+// values with heads of 64, 5.8 and 4.6 with 256, where 128 has 5.8 and 5.2.
 constexpr size_t kSlots[kClasses] = {512, 256, 256}, kSlotsBf16[kClasses] = {512, 512, 256};
 // An estimate of a block's time in us: for each 64 positions, alone and with the
 // chip full of others, and for the rest of it and its launch; fitted to measured
@@ -123,12 +126,13 @@ void plan_attention(const PlanShape &shape, const SeqAt *seqs, BatchHead *head, 
     // Each class is a launch, and the launches run one after another; large tiles
     // have more partial results and a longer start, small ones read keys and values
     // more often. So fewer classes where that is less, by an estimate that is off
-    // by up to a twentieth. Of 260 mixed batches 61 are cut differently so, and
-    // take 11.8 us where they took 15.7 (geometric means; at worst 1.03 times as
-    // long). f32, 32 / 8 heads, with the smallest class for each and now: 16 trees
-    // of up to 6 tokens at 800 44 -> 35, 24 chunks of up to 38 at 5 to 30 24 -> 12, a
-    // tree of 60 at 300 23 -> 18, at 3900 39 -> 32, and from 8100 on, where tiles of
-    // 128 take as long, then longer (at 48800 199, not 169), as it was.
+    // by up to a twentieth. Of the first 260 attentions that
+    // perf/more_operators.py draws with random.Random(5), 78 are cut differently
+    // so, and take 13.1 us where they took 18.2 (geometric means; at worst 1.07
+    // times as long, at best 0.28: profiles/paged_plan.md). f32, 32 / 8 heads, with
+    // the smallest class for each and now: 16 trees of up to 6 tokens at 800
+    // 38 -> 32, 24 chunks of up to 38 at 30 28 -> 13, a tree of 60 at 300 23 -> 18, at
+    // 3900 38 -> 33, and from 8100 on as it was.
     Cut cuts[kClasses] = {};
     unsigned classes = 0;
     double least = 0;

@@ -142,7 +142,7 @@ unsafe extern "C" {
     pub fn th_silu_mul_q8(dev: *mut th_device, q: *mut th_q8, gate: *const th_buffer, up: *const th_buffer) -> c_int;
     pub fn th_matmul_q8(dev: *mut th_device, out: *mut th_buffer, w: *const th_q8, x: *const th_q8) -> c_int;
 
-    // The forward pass (model/model.rs) and the decode loops on the device.
+    // Paged caches and batches.
     pub fn th_paged_alloc(dev: *mut th_device, pages: usize, page_len: usize, n_kv_heads: usize, head_dim: usize,
                           kv_dtype: c_int, out: *mut *mut th_paged) -> c_int;
     pub fn th_paged_free(dev: *mut th_device, cache: *mut th_paged);
@@ -164,6 +164,8 @@ unsafe extern "C" {
                            picks: *mut u32, n_kept: *mut u32, kept: *mut i32) -> c_int;
     pub fn th_paged_keep(dev: *mut th_device, caches: *const *mut th_paged, n_caches: usize, batch: *const th_batch,
                          n_kept: *const u32, kept: *const i32) -> c_int;
+
+    // The forward pass (model/model.rs) and the decode loops on the device.
     pub fn th_model_create(dev: *mut th_device, config: *const th_config, weights: *const *const th_weight,
                            n_weights: usize, out: *mut *mut th_model) -> c_int;
     pub fn th_model_destroy(model: *mut th_model);
