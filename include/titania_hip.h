@@ -312,7 +312,8 @@ TH_API int th_paged_append(th_device *dev, th_buffer *q_out, const th_buffer *q,
  * products, and sums of values with weights of at most one have to be in f32's
  * range. Where it takes many (more than 16 of a KV head, as a rule), queries, keys,
  * values and weights have 22 bits: a product is off by up to 2^-21 of
- * itself and by 2^-38 of the largest key, or value, that the token sees. */
+ * itself and by 2^-38 of the largest key, or value, that the token sees, or
+ * 2^-25 of it where tokens of the step that it does not see have larger ones. */
 TH_API int th_paged_attention(th_device *dev, th_buffer *out, const th_buffer *q, const th_paged *cache,
                               const th_batch *batch);
 /* The greedy verification of drafted tokens. logits: a row for each token of

@@ -120,3 +120,33 @@ def test_what_all_rows_see_is_not_taken_one_by_one(hip, what, heads, kvh, first,
     check(got, *attention64(step, q, pool, heads))
     same = got[first:] == run_attention(hip, after, q[first:], pool, heads, kv, 7)
     assert same.all(), f"{(~same).sum()} of {same.size} differ"
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize("factor", [2.0**8, 2.0**11, 2.0**-11])
+@pytest.mark.parametrize("context", [0, 50])
+def test_branches_of_sizes_that_have_a_scale(hip, context, factor, what, kv, kernels):  # noqa: F811
+    """Keys or values of another branch up to 2^13 times a token's own take as
+    many of the bits of 2^-38 that its terms leave out: 2^-25 of the largest
+    that it sees, for each value as it is, for each key times the query's."""
+    r = np.random.default_rng(int(abs(np.log2(factor))) + context)
+    step = Step(r, [context], [100], 32, [branches(64, 36)])
+    pool = pool_of(r, step.pages, 32, 2, 128, TH_KV_F32)
+    for i in range(64):
+        page, row = step.place(0, context + i)
+        pool[page, what, row] *= np.float32(factor)
+    pool = bf16_to_f32(f32_to_bf16(pool)) if kv == TH_KV_BF16 else pool
+    q = r.standard_normal((100, 8, 128), dtype=np.float32)
+    want, tol = attention64(step, q, pool, 8)
+    sees = np.concatenate([np.ones((100, context), bool), step.sees[0]], 1)
+    largest = np.array([np.abs(step.rows(pool, 0, what)[s]).max((0, 2)) for s in sees])  # [token][KV head]
+    largest = np.repeat(largest, 4, 1).astype(np.float64)
+    if what:
+        tol += 2.0**-25 * largest[:, :, None]
+    else:
+        value = np.array([np.abs(step.rows(pool, 0, 1)[s]).max((0, 2)) for s in sees])
+        d = 2.0**-25 * largest * np.abs(q).sum(-1) / np.sqrt(128)
+        tol += 2 * (d * np.repeat(value, 4, 1))[:, :, None]
+    check(run_attention(hip, step, q, pool, 8, kv, kernels), want, tol)

@@ -378,7 +378,7 @@ __device__ __forceinline__ uint64_t seen64(const SeqAt &seq, const uint64_t *tre
 // the weights are of exp2(x - r + 10), r the row's maximum, or within
 // 2^5 of it. Results are those of f32 but for
 // 2^-21 of a product, and for what lies 2^38 below the largest value that a
-// row sees.
+// row sees, or 2^25 below where unseen ones are larger (by 2^13 at most, as follows).
 //
 // S^T = K Q^T leaves a lane four neighbouring positions of its row in each of
 // the tile's four sixteens, which with V^T's columns in that order are the
