@@ -62,18 +62,9 @@ def test_one_large_value_among_zeros(hip, large, context, kv, kernels):  # noqa:
     check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
 
 
-@gpu
-@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
-@pytest.mark.parametrize("context", [2000, 6400])
-@pytest.mark.parametrize("new", [1, 20, 70])
-@pytest.mark.parametrize("size,signs", [(1e33, True), (1e34, False), (1e35, True), (3e38, False)])
-def test_flat_scores_over_values_near_the_largest(hip, size, signs, new, context, kv, kernels):  # noqa: F811
+def flat_scores(hip, size, signs, new, context, kv, kernels):
     """Averages of thousands of values whose sums f32 does not hold, of one sign
-    or both, where a plan splits the positions. (The kernel for few rows adds
-    f32 values up with weights of at most one: at 1e35, of both signs, within
-    range.)"""
-    if size > 1e37 and (kernels == 0 or new * 4 <= 16):
-        pytest.skip("sums past f32's range in the kernel for few rows")
+    or both, where a plan splits the positions."""
     r = np.random.default_rng(new + context)
     step = Step(r, [context], [new], 64)
     pool = pool_of(r, step.pages, 64, 2, 128, TH_KV_F32)
@@ -83,6 +74,26 @@ def test_flat_scores_over_values_near_the_largest(hip, size, signs, new, context
     pool = bf16_to_f32(f32_to_bf16(pool)) if kv == TH_KV_BF16 else pool
     q = np.float32(0.01) * r.standard_normal((step.tokens, 8, 128), dtype=np.float32)
     check(run_attention(hip, step, q, pool, 8, kv, kernels), *attention64(step, q, pool, 8))
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("context", [2000, 6400])
+@pytest.mark.parametrize("new", [1, 20, 70])
+@pytest.mark.parametrize("size,signs", [(1e33, True), (1e34, False), (1e35, True)])
+def test_flat_scores_over_large_values(hip, size, signs, new, context, kv, kernels):  # noqa: F811
+    """(Sums with weights of at most one are in range: the kernel for few rows has those.)"""
+    flat_scores(hip, size, signs, new, context, kv, kernels)
+
+
+@gpu
+@pytest.mark.parametrize("kv", [TH_KV_F32, TH_KV_BF16])
+@pytest.mark.parametrize("context", [2000, 6400])
+@pytest.mark.parametrize("new", [20, 70])
+@pytest.mark.parametrize("large_tiles", [7, 5])
+def test_flat_scores_over_values_near_the_largest(hip, large_tiles, new, context, kv):
+    """The kernels for many rows, where sums are past f32's range and averages are not."""
+    flat_scores(hip, 3e38, False, new, context, kv, large_tiles)
 
 
 @gpu
