@@ -132,3 +132,33 @@ def test_a_batch_is_replayed_on_its_own_stream(hip):
     for g in (graph, plain):
         g.free()
     other.close()
+
+
+@gpu
+def test_one_graph_of_two_batches(hip):
+    """What a graph asks of two batches ends for both; for one that is freed
+    before it there is nothing left to end."""
+    r = np.random.default_rng(5)
+    for gone in (None, 0, 1):
+        batches = [Batch(hip, r) for _ in range(2)]
+        x = [[buf(hip, a[:n]) for a in (b.q, b.k, b.k)] for b, n in zip(batches, (4, 9))]
+        rope = buf(hip, rope_table(50, HD))
+        for b, n in zip(batches, (4, 9)):
+            b.set(10, n)
+        hip.graph_begin()
+        for b, (q, k, v) in zip(batches, x):
+            hip.paged_append(q, q, k, v, None, None, rope, b.cache, b.batch, EPS)
+        graph = hip.graph_end()
+        for b, n in zip(batches, (4, 9)):
+            b.refuses(f"captured with this batch at {n}", 0, n + 1)
+            b.refuses("position 50", 50, 1)
+            b.set(49, 1)
+        graph.launch()
+        hip.synchronize()
+        if gone is not None:
+            batches[gone].batch.free()
+        graph.free()
+        for i, b in enumerate(batches):
+            if i != gone:
+                b.set(0, 100)
+                b.set(300, 1)
